@@ -228,6 +228,57 @@ int smoe_single2scatter(const void* X, int64_t x_rows, int64_t stride_xm, int64_
                         int64_t stride_yn, const int64_t* expert_idxs, int32_t k, int32_t K, int32_t N, int32_t E,
                         int32_t dtype, void* stream);
 
+/* ---- the MoE layer for a few tokens (decode; no counterpart in the reference, which only has single2scatter) ----------
+ * With slot s = t*k + j, e = expert_idxs[t, j]:
+ *     h_s = activation(X[t] W1[e] + b1[e]);   Y[t] = sum_j gates[t, j] * (h_s W2[e] + b2[e])
+ * X (T, d) with inner stride 1, W1 (E, d, n_up), W2 (E, F, d_out) and the biases in element strides, layouts / functions as
+ * for smoe_activation_forward (n_up = F or 2F); gates (T, k) in element strides and a dtype of their own, nullable (a
+ * plain sum); expert_idxs (T, k) in element strides, ids outside [0, E) contribute nothing. Every element of Y is written.
+ * Limits: T <= smoe_few_token_max_tokens(), T * k <= 1024, E <= 1024. The slots are sorted inside the kernels. `workspace`
+ * (16-byte aligned, smoe_few_token_workspace_bytes) belongs to this call until its work has finished: two calls that may
+ * overlap need two. Nothing in it has to be cleared, nothing is read from it that the call did not write. */
+int32_t smoe_few_token_max_tokens(void);
+size_t smoe_few_token_workspace_bytes(int64_t T, int32_t k, int32_t F, int32_t d_out);
+int smoe_few_token_mlp(const void* X, int64_t T, int64_t stride_xm,
+                       const void* W1, int64_t stride_w1e, int64_t stride_w1k, int64_t stride_w1n,
+                       const void* b1, int64_t stride_b1e, int64_t stride_b1n,
+                       const void* W2, int64_t stride_w2e, int64_t stride_w2k, int64_t stride_w2n,
+                       const void* b2, int64_t stride_b2e, int64_t stride_b2n,
+                       const void* gates, int64_t stride_gt, int64_t stride_gk, int32_t gates_dtype,
+                       const int64_t* expert_idxs, int64_t stride_it, int64_t stride_ik, void* Y, int64_t stride_ym,
+                       int32_t k, int32_t d, int32_t F, int32_t d_out, int32_t E, int32_t act_layout, int32_t act,
+                       float alpha, float limit, int32_t dtype, int32_t flags, void* workspace, size_t workspace_bytes,
+                       void* stream);
+/* The router in front of it: logits X Wr^T + br in fp32, then ids and gates as smoe_route_topk defines them (mode,
+ * renormalize; descending, equal logits by lower id, a NaN counts as the largest). Wr is (E, d), inner stride 1; X, Wr, br
+ * in `dtype`. E <= 1024, k <= min(E, 32). expert_idxs, gates: (T, k) contiguous. */
+int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void* Wr, int64_t stride_wm, const void* br,
+                         int64_t stride_bn, int32_t E, int32_t d, int32_t k, int32_t mode, int32_t renormalize,
+                         int64_t* expert_idxs, float* gates, int32_t dtype, void* stream);
+
+/* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference) ---------------------
+ * Each row names its adapter a = adapter_idxs[t]; ids outside [0, n) mean none. Three products make both directions:
+ * smoe_adapter_shrink:  H[t, j] = s_a sum_c X[t, c] M[a][j, c]     fp32 (T, r), zero rows without an adapter;
+ *     s_a = scaling[a], or `scale` where `scaling` is null. M: lora_a forward, lora_b seen as (n, r, out) backward.
+ * smoe_adapter_linear:  Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum_j H[t, j] M[a][j, o]      (bias nullable, contiguous)
+ * smoe_adapter_grad:    D[a][j, c] = sum over the rows t of adapter a of U[t, j] V[t, c], U fp32 (T, r), rows listed by
+ *     smoe_sort_count of adapter_idxs (sorted_scattered_idxs, expert_offsets); every element of D is written.
+ * smoe_column_sum:      out[c] = sum_t V[t, c]   (the bias's gradient). Fixed summation order everywhere.
+ * X, Y, V rows have inner stride 1; W, M, D in element strides. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31. */
+int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma, int64_t stride_mj,
+                        int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling, float scale, float* H, int32_t n,
+                        int32_t C, int32_t r, int32_t dtype, void* stream);
+int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk, int64_t stride_wn,
+                        const void* bias, const float* H, const void* M, int64_t stride_ma, int64_t stride_mj,
+                        int64_t stride_mo, const int64_t* adapter_idxs, void* Y, int64_t stride_ym, int32_t n, int32_t C,
+                        int32_t O, int32_t r, int32_t dtype, int32_t* status, void* stream);
+int smoe_adapter_grad(const float* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
+                      const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc, int32_t n,
+                      int32_t C, int32_t r, int32_t dtype, void* stream);
+size_t smoe_column_sum_workspace_bytes(int64_t T, int32_t C);
+int smoe_column_sum(const void* V, int64_t T, int64_t stride_vm, int32_t C, void* out, int32_t dtype, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* ---- expert-parallel row exchange over NVLink peer memory -----------------------------------------------
  * No counterpart in the reference (it has no multi-GPU code). `peer_*` arguments are HOST arrays of `world` device
  * pointers, entry w = that buffer of rank w mapped into this process (e.g. a symmetric-memory allocation); entry

@@ -13,6 +13,10 @@ from . import kernels
 from . import mlp
 from . import utils
 from .routing import route_topk
+from .few_token import few_token_mlp, few_token_moe
+from .adapters import AdapterLinear, adapter_linear
+from . import adapters
+from . import few_token
 from ._lib import check_device_status, library_path
 
 __all__ = [
@@ -21,6 +25,12 @@ __all__ = [
     "parallel_linear_act",
     "expert_mlp",
     "route_topk",
+    "few_token_mlp",
+    "few_token_moe",
+    "adapter_linear",
+    "AdapterLinear",
+    "adapters",
+    "few_token",
     "ParallelExperts",
     "parallel_experts",
     "kernels",

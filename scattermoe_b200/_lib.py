@@ -89,6 +89,23 @@ SIGNATURES = {
     "smoe_ep_combine": ([_P, _I64, _I64, _P, _P, _I64, _P, _I32, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P], c_int32),
     "smoe_ep_sum_parts": ([_P, _I64, _P, _I32, _P, _I64, _I64, _I32, _I32, _P], c_int32),
     "smoe_status_poison": ([_P, _P, _I64, _P], c_int32),
+    "smoe_few_token_max_tokens": ([], c_int32),
+    "smoe_few_token_workspace_bytes": ([_I64, _I32, _I32, _I32], c_size_t),
+    "smoe_few_token_mlp": ([_P, _I64, _I64,                  # X
+                            _P, _I64, _I64, _I64, _P, _I64, _I64,   # W1 b1
+                            _P, _I64, _I64, _I64, _P, _I64, _I64,   # W2 b2
+                            _P, _I64, _I64, _I32,            # gates
+                            _P, _I64, _I64,                  # ids
+                            _P, _I64,                        # Y
+                            _I32, _I32, _I32, _I32, _I32,    # k d F d_out E
+                            _I32, _I32, c_float, c_float, _I32, _I32, _P, c_size_t, _P], c_int32),
+    "smoe_few_token_route": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _I32, _P], c_int32),
+    "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P], c_int32),
+    "smoe_adapter_linear": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32,
+                             _I32, _P, _P], c_int32),
+    "smoe_adapter_grad": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P], c_int32),
+    "smoe_column_sum_workspace_bytes": ([_I64, _I32], c_size_t),
+    "smoe_column_sum": ([_P, _I64, _I64, _I32, _P, _I32, _P, c_size_t, _P], c_int32),
 }
 
 

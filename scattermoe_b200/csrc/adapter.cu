@@ -1,0 +1,305 @@
+// Low-rank adapters on CUDA cores (fp32, and 16-bit operands the tensor-core kernels cannot address), and the C entry points.
+#include "adapter.cuh"
+
+namespace smoe {
+namespace ad {
+
+// ---- shrink: a warp per (token, 4 rank rows), lanes over the contracted axis -------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256)
+shrink_simt_kernel(const ShrinkArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blocks = (a.r + 3) / 4;
+  const int64_t total = a.T * blocks;
+  for (int64_t it = static_cast<int64_t>(blockIdx.x) * 8 + warp; it < total; it += static_cast<int64_t>(gridDim.x) * 8) {
+    const int64_t t = it / blocks;
+    const int j0 = static_cast<int>(it % blocks) * 4;
+    const int64_t id = a.ids[t];
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float s = 0.f;
+    if (id >= 0 && id < a.n) {
+      s = a.scaling ? a.scaling[id] : a.scale;
+      const T* x = static_cast<const T*>(a.X) + t * a.sxm;
+      const T* m = static_cast<const T*>(a.M) + id * a.sma;
+      for (int c = lane; c < a.C; c += 32) {
+        const float xv = to_f32<T>(__ldg(x + c));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (j0 + i < a.r) acc[i] = fmaf(xv, to_f32<T>(__ldg(m + (j0 + i) * a.smj + c * a.smc)), acc[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+      // an adapter that is not there leaves a zero row, whatever the inputs hold
+      if (lane == 0 && j0 + i < a.r) a.H[t * a.r + j0 + i] = (id >= 0 && id < a.n) ? acc[i] * s : 0.f;
+    }
+  }
+}
+
+// ---- shared product + expansion: 64 x 64 tiles, 4 x 4 outputs per thread ----------------------------------------
+constexpr int TM = 64, TN = 64, TK = 16;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+linear_simt_kernel(const LinearArgs a) {
+  __shared__ float xs[TK][TM + 4];
+  __shared__ float ws[TK][TN + 4];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.y) * TM;
+  const int o0 = blockIdx.x * TN;
+  const bool k_contig = a.swk == 1;
+  float acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  for (int k0 = 0; k0 < a.C; k0 += TK) {
+#pragma unroll
+    for (int i = 0; i < TM * TK / 256; ++i) {
+      const int idx = tid + i * 256, kk = idx % TK, m = idx / TK;
+      const int64_t t = t0 + m;
+      xs[kk][m] = (t < a.T && k0 + kk < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.X) + t * a.sxm + k0 + kk)) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < TN * TK / 256; ++i) {
+      const int idx = tid + i * 256;
+      const int kk = k_contig ? idx % TK : idx / TN, n = k_contig ? idx / TK : idx % TN;
+      ws[kk][n] = (o0 + n < a.O && k0 + kk < a.C)
+                      ? to_f32<T>(__ldg(static_cast<const T*>(a.W) + (k0 + kk) * a.swk + (o0 + n) * a.swn)) : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < TK; ++kk) {
+      const float4 x4 = *reinterpret_cast<const float4*>(&xs[kk][ty * 4]);
+      const float4 w4 = *reinterpret_cast<const float4*>(&ws[kk][tx * 4]);
+      const float xv[4] = {x4.x, x4.y, x4.z, x4.w}, wv[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(xv[i], wv[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t t = t0 + ty * 4 + i;
+    if (t >= a.T) continue;
+    const int64_t id = a.ids[t];
+    if (id >= 0 && id < a.n) {
+      const T* m = static_cast<const T*>(a.M) + id * a.sma;
+      const float* h = a.H + t * a.r;
+      for (int jj = 0; jj < a.r; ++jj) {
+        const float hv = h[jj];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int o = o0 + tx * 4 + j;
+          if (o < a.O) acc[i][j] = fmaf(hv, to_f32<T>(__ldg(m + jj * a.smj + o * a.smo)), acc[i][j]);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int o = o0 + tx * 4 + j;
+      if (o >= a.O) continue;
+      const float b = a.bias ? to_f32<T>(static_cast<const T*>(a.bias)[o]) : 0.f;
+      static_cast<T*>(a.Y)[t * a.sym + o] = from_f32<T>(acc[i][j] + b);
+    }
+  }
+}
+
+// ---- per-adapter outer products: a block per (64 columns, 16 rank rows, adapter), over the adapter's rows in order ----
+template <typename T>
+__global__ void __launch_bounds__(256)
+grad_simt_kernel(const GradArgs a) {
+  __shared__ float us[32][17];
+  __shared__ float vs[32][65];
+  __shared__ int64_t rows[32];
+  const int tid = threadIdx.x, cx = tid & 63, jg = tid >> 6;
+  const int c0 = blockIdx.x * 64, j0 = blockIdx.y * 16, e = blockIdx.z;
+  const int64_t beg = e ? a.offsets[e - 1] : 0, end = a.offsets[e];
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int64_t m0 = beg; m0 < end; m0 += 32) {
+    const int cnt = static_cast<int>(min(static_cast<int64_t>(32), end - m0));
+    if (tid < 32) rows[tid] = tid < cnt ? a.sorted_idx[m0 + tid] : -1;
+    __syncthreads();
+    for (int i = tid; i < 32 * 16; i += 256) {
+      const int m = i >> 4, j = i & 15;
+      us[m][j] = (m < cnt && j0 + j < a.r) ? a.U[rows[m] * a.r + j0 + j] : 0.f;
+    }
+    for (int i = tid; i < 32 * 64; i += 256) {
+      const int m = i >> 6, c = i & 63;
+      vs[m][c] = (m < cnt && c0 + c < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.V) + rows[m] * a.svm + c0 + c)) : 0.f;
+    }
+    __syncthreads();
+    for (int m = 0; m < cnt; ++m) {
+      const float v = vs[m][cx];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = fmaf(us[m][jg * 4 + i], v, acc[i]);
+    }
+    __syncthreads();
+  }
+  if (c0 + cx >= a.C) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = j0 + jg * 4 + i;
+    if (j < a.r) static_cast<T*>(a.D)[e * a.sda + j * a.sdj + (c0 + cx) * a.sdc] = from_f32<T>(acc[i]);
+  }
+}
+
+#define SMOE_AD_DTYPE(dtype, ...)                                      \
+  switch (dtype) {                                                     \
+    case SMOE_F32: { using T_ = float; __VA_ARGS__ } break;            \
+    case SMOE_BF16: { using T_ = __nv_bfloat16; __VA_ARGS__ } break;   \
+    default: { using T_ = __half; __VA_ARGS__ } break;                 \
+  }
+
+int launch_shrink_simt(const ShrinkArgs& a) {
+  const int64_t warps = a.T * cdiv(a.r, 4);
+  const int grid = static_cast<int>(min(cdiv64(warps, 8), static_cast<int64_t>(148 * 32)));
+  SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_><<<grid, 256, 0, a.stream>>>(a);)
+  SMOE_LAUNCH_CHECK();
+  return SMOE_OK;
+}
+
+int launch_linear_simt(const LinearArgs& a) {
+  // the token axis in slices of at most 65535 tiles (the grid's second axis)
+  const int64_t slice = static_cast<int64_t>(65535) * TM;
+  for (int64_t t0 = 0; t0 < a.T; t0 += slice) {
+    LinearArgs b = a;
+    const int es = dtype_size(a.dtype);
+    b.X = static_cast<const uint8_t*>(a.X) + t0 * a.sxm * es;
+    b.Y = static_cast<uint8_t*>(a.Y) + t0 * a.sym * es;
+    b.H = a.H + t0 * a.r;
+    b.ids = a.ids + t0;
+    b.T = a.T - t0 < slice ? a.T - t0 : slice;
+    dim3 grid(static_cast<unsigned>(cdiv(a.O, TN)), static_cast<unsigned>(cdiv64(b.T, TM)));
+    SMOE_AD_DTYPE(a.dtype, linear_simt_kernel<T_><<<grid, 256, 0, a.stream>>>(b);)
+    SMOE_LAUNCH_CHECK();
+  }
+  return SMOE_OK;
+}
+
+int launch_grad_simt(const GradArgs& a) {
+  dim3 grid(static_cast<unsigned>(cdiv(a.C, 64)), static_cast<unsigned>(cdiv(a.r, 16)), static_cast<unsigned>(a.n));
+  SMOE_AD_DTYPE(a.dtype, grad_simt_kernel<T_><<<grid, 256, 0, a.stream>>>(a);)
+  SMOE_LAUNCH_CHECK();
+  return SMOE_OK;
+}
+
+static int check_common(const char* who, int64_t T, int n, int C, int r, int dtype) {
+  SMOE_CHECK_ARG(dtype == SMOE_F32 || dtype == SMOE_BF16 || dtype == SMOE_F16, "%s: unknown dtype %d", who, dtype);
+  SMOE_CHECK_ARG(T >= 0 && T < (int64_t(1) << 31), "%s: T=%lld out of range [0, 2^31)", who, (long long)T);
+  SMOE_CHECK_ARG(n >= 1 && n <= 4096, "%s: %d adapters, 1 to 4096 are taken", who, n);
+  SMOE_CHECK_ARG(r >= 1 && r <= MAX_RANK, "%s: rank %d, 1 to %d are taken", who, r, MAX_RANK);
+  SMOE_CHECK_ARG(C >= 1 && C < (1 << 28), "%s: bad width %d", who, C);
+  return SMOE_OK;
+}
+
+}  // namespace ad
+}  // namespace smoe
+
+using namespace smoe;
+
+extern "C" int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma,
+                                   int64_t stride_mj, int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling,
+                                   float scale, float* H, int32_t n, int32_t C, int32_t r, int32_t dtype, void* stream) {
+  if (int rc = ad::check_common("adapter_shrink", T, n, C, r, dtype)) return rc;
+  if (T == 0) return SMOE_OK;
+  SMOE_CHECK_ARG(X && M && adapter_idxs && H, "adapter_shrink: null pointer");
+  ad::ShrinkArgs a{X, T, stride_xm, M, stride_ma, stride_mj, stride_mc, adapter_idxs, scaling, scale, H, n, C, r, dtype,
+                   static_cast<cudaStream_t>(stream)};
+  return ad::launch_shrink_simt(a);
+}
+
+extern "C" int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk,
+                                   int64_t stride_wn, const void* bias, const float* H, const void* M, int64_t stride_ma,
+                                   int64_t stride_mj, int64_t stride_mo, const int64_t* adapter_idxs, void* Y,
+                                   int64_t stride_ym, int32_t n, int32_t C, int32_t O, int32_t r, int32_t dtype,
+                                   int32_t* status, void* stream) {
+  if (int rc = ad::check_common("adapter_linear", T, n, C, r, dtype)) return rc;
+  SMOE_CHECK_ARG(O >= 1 && O < (1 << 28), "adapter_linear: bad width %d", O);
+  if (T == 0) return SMOE_OK;
+  SMOE_CHECK_ARG(X && W && H && M && adapter_idxs && Y, "adapter_linear: null pointer");
+  ad::LinearArgs a{X, T, stride_xm, W, stride_wk, stride_wn, bias, H, M, stride_ma, stride_mj, stride_mo, adapter_idxs, Y,
+                   stride_ym, n, C, O, r, dtype, status, static_cast<cudaStream_t>(stream)};
+  return ad::launch_linear_simt(a);
+}
+
+extern "C" int smoe_adapter_grad(const float* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
+                                 const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc,
+                                 int32_t n, int32_t C, int32_t r, int32_t dtype, void* stream) {
+  if (int rc = ad::check_common("adapter_grad", T, n, C, r, dtype)) return rc;
+  SMOE_CHECK_ARG(D && offsets && (T == 0 || (U && V && sorted_idx)), "adapter_grad: null pointer");
+  ad::GradArgs a{U, T, V, stride_vm, sorted_idx, offsets, D, stride_da, stride_dj, stride_dc, n, C, r, dtype,
+                 static_cast<cudaStream_t>(stream)};
+  return ad::launch_grad_simt(a);
+}
+
+// ---- column sums (the shared bias's gradient): fp32 partial sums over slices of the rows, added up in order ----
+namespace smoe {
+namespace ad {
+
+constexpr int SUM_COLS = 256, SUM_MAX_SLICES = 64;
+
+static int sum_slices(int64_t T, int C) {
+  const int64_t by_rows = cdiv64(T, 64), by_grid = cdiv64(148 * 4, cdiv(C, SUM_COLS));
+  const int64_t s = by_rows < by_grid ? by_rows : by_grid;
+  return static_cast<int>(s < 1 ? 1 : (s > SUM_MAX_SLICES ? SUM_MAX_SLICES : s));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SUM_COLS)
+column_partial_kernel(const T* __restrict__ V, int64_t rows, int64_t svm, int C, float* __restrict__ partial) {
+  const int c = blockIdx.x * SUM_COLS + threadIdx.x;
+  if (c >= C) return;
+  const int64_t per = (rows + gridDim.y - 1) / gridDim.y;
+  const int64_t beg = min(rows, per * blockIdx.y), end = min(rows, beg + per);
+  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  int64_t t = beg;
+  for (; t + 4 <= end; t += 4) {
+    s0 += to_f32<T>(__ldg(V + t * svm + c));
+    s1 += to_f32<T>(__ldg(V + (t + 1) * svm + c));
+    s2 += to_f32<T>(__ldg(V + (t + 2) * svm + c));
+    s3 += to_f32<T>(__ldg(V + (t + 3) * svm + c));
+  }
+  for (; t < end; ++t) s0 += to_f32<T>(__ldg(V + t * svm + c));
+  partial[static_cast<int64_t>(blockIdx.y) * C + c] = (s0 + s1) + (s2 + s3);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(SUM_COLS)
+column_total_kernel(const float* __restrict__ partial, int slices, int C, T* __restrict__ out) {
+  const int c = blockIdx.x * SUM_COLS + threadIdx.x;
+  if (c >= C) return;
+  float s = 0.f;
+  for (int i = 0; i < slices; ++i) s += partial[static_cast<int64_t>(i) * C + c];
+  out[c] = from_f32<T>(s);
+}
+
+}  // namespace ad
+}  // namespace smoe
+
+extern "C" size_t smoe_column_sum_workspace_bytes(int64_t T, int32_t C) {
+  if (T < 0 || C < 1) return 0;
+  return static_cast<size_t>(ad::sum_slices(T, C)) * C * 4;
+}
+
+extern "C" int smoe_column_sum(const void* V, int64_t T, int64_t stride_vm, int32_t C, void* out, int32_t dtype, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (int rc = ad::check_common("column_sum", T, 1, C, 1, dtype)) return rc;
+  SMOE_CHECK_ARG(out && (T == 0 || V), "column_sum: null pointer");
+  if (workspace == nullptr || workspace_bytes < smoe_column_sum_workspace_bytes(T, C)) {
+    set_error("column_sum: workspace of %zu bytes needed, %zu given", smoe_column_sum_workspace_bytes(T, C), workspace_bytes);
+    return SMOE_ERR_WORKSPACE;
+  }
+  const int slices = ad::sum_slices(T, C);
+  float* partial = static_cast<float*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  dim3 grid(static_cast<unsigned>(cdiv(C, ad::SUM_COLS)), static_cast<unsigned>(slices));
+  SMOE_AD_DTYPE(dtype, ad::column_partial_kernel<T_><<<grid, ad::SUM_COLS, 0, st>>>(static_cast<const T_*>(V), T, stride_vm, C, partial);
+                ad::column_total_kernel<T_><<<grid.x, ad::SUM_COLS, 0, st>>>(partial, slices, C, static_cast<T_*>(out));)
+  SMOE_LAUNCH_CHECK();
+  return SMOE_OK;
+}

@@ -1,0 +1,55 @@
+// Shared by the kernels of the low-rank adapters beside a shared projection.
+//
+//   y_t = W x_t + b + B_a h_t,   h_t = s_a A_a x_t,   a = ids[t]      (an id outside [0, n): y_t = W x_t + b)
+//
+// and its gradients  g_t = s_a B_a^T dy_t;  dx_t = W^T dy_t + A_a^T g_t;  dA_a = sum g_t x_t^T;  dB_a = sum dy_t h_t^T.
+// Three products cover both directions: the SHRINK into the rank (h, g), the shared product with the EXPANSION out of the rank
+// added while the accumulators are at hand (y, dx), and the per-adapter sum of outer products (dA, dB).
+// h and g are fp32 (T, r) rows.
+#pragma once
+
+#include "smoe_common.cuh"
+
+namespace smoe {
+namespace ad {
+
+constexpr int MAX_RANK = 256;
+
+struct ShrinkArgs {           // H[t, j] = s_a sum_c X[t, c] M[a][j, c]
+  const void* X; int64_t T, sxm;
+  const void* M; int64_t sma, smj, smc;
+  const int64_t* ids;
+  const float* scaling; float scale;
+  float* H;
+  int n, C, r, dtype;
+  cudaStream_t stream;
+};
+
+struct LinearArgs {           // Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum_j H[t, j] M[a][j, o]
+  const void* X; int64_t T, sxm;
+  const void* W; int64_t swk, swn;
+  const void* bias;
+  const float* H;
+  const void* M; int64_t sma, smj, smo;
+  const int64_t* ids;
+  void* Y; int64_t sym;
+  int n, C, O, r, dtype;
+  int32_t* status;
+  cudaStream_t stream;
+};
+
+struct GradArgs {             // D[a][j, c] = sum over rows t of adapter a of U[t, j] V[t, c]
+  const float* U; int64_t T;
+  const void* V; int64_t svm;
+  const int64_t* sorted_idx; const int64_t* offsets;
+  void* D; int64_t sda, sdj, sdc;
+  int n, C, r, dtype;
+  cudaStream_t stream;
+};
+
+int launch_shrink_simt(const ShrinkArgs& a);
+int launch_linear_simt(const LinearArgs& a);
+int launch_grad_simt(const GradArgs& a);
+
+}  // namespace ad
+}  // namespace smoe

@@ -10,6 +10,7 @@ from torch import nn
 
 from . import _lib
 from . import activation as _act
+from . import few_token
 from .parallel_experts import ParallelExperts, expert_mlp, flatten_sort_count
 
 
@@ -52,6 +53,23 @@ class _ExpertMLPBase(nn.Module):
             up = self.experts(tokens, self.top_k, *routing, grouped_out=True)
             hidden = self._activate(up)
             y = self.output_experts(hidden, 1, *routing, grouped_in=True, gates=expert_p)
+        return y.view(*lead, y.size(-1))
+
+    def decode(self, x: torch.Tensor, expert_p: torch.Tensor, expert_idxs: torch.Tensor):
+        """`forward` for a few tokens without gradients (an addition to the reference's surface): `few_token_mlp` on this
+        module's weights. Same arguments and result, but ids outside [0, num_experts) contribute nothing. Refuses more than
+        `few_token.max_tokens()` tokens and activations this library does not fuse: call `forward` for those."""
+        lead = x.shape[:-1]
+        tokens = x.reshape(-1, x.shape[-1])
+        code = _act.resolve_activation(self.activation)
+        if code is None:
+            raise RuntimeError("decode: the activation %r is not one this library fuses" % (self.activation,))
+        ids = expert_idxs.reshape(tokens.size(0), expert_idxs.shape[-1])
+        with torch.no_grad():
+            y = few_token.few_token_mlp(
+                tokens, self.experts.weight.permute(0, 2, 1), self.output_experts.weight.permute(0, 2, 1),
+                expert_p.reshape(ids.shape) if expert_p is not None else None, ids, self.act_layout, code,
+                up_biases=self.experts.bias, down_biases=self.output_experts.bias)
         return y.view(*lead, y.size(-1))
 
 
