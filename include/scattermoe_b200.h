@@ -41,7 +41,9 @@ enum smoe_flags {
   SMOE_FLAG_ALLOW_TF32 = 1,   /* fp32 inputs may use reduced-precision tensor cores (ops.py:7 ALLOW_TF32) */
   SMOE_FLAG_FORCE_SIMT = 2,   /* take the CUDA-core kernel even where a tensor-core kernel exists */
   SMOE_FLAG_FORCE_TC = 4,     /* fail with SMOE_ERR_UNSUPPORTED instead of taking the CUDA-core kernel */
-  SMOE_FLAG_GATHER_ROWS = 8   /* feed grouped inputs through the row-gather path too (testing / comparison) */
+  SMOE_FLAG_GATHER_ROWS = 8,  /* feed grouped inputs through the row-gather path too (testing / comparison) */
+  SMOE_FLAG_AFTER_ROUTER = 16 /* smoe_few_token_mlp: the call just before on this stream is the smoe_few_token_route that
+                                 writes expert_idxs and gates; the kernels may be scheduled while it still runs */
 };
 
 int smoe_version(void);
@@ -248,7 +250,7 @@ int smoe_few_token_mlp(const void* X, int64_t T, int64_t stride_xm,
                        const int64_t* expert_idxs, int64_t stride_it, int64_t stride_ik, void* Y, int64_t stride_ym,
                        int32_t k, int32_t d, int32_t F, int32_t d_out, int32_t E, int32_t act_layout, int32_t act,
                        float alpha, float limit, int32_t dtype, int32_t flags, void* workspace, size_t workspace_bytes,
-                       void* stream);
+                       int32_t* status, void* stream);
 /* The router in front of it: logits X Wr^T + br in fp32, then ids and gates as smoe_route_topk defines them (mode,
  * renormalize; descending, equal logits by lower id, a NaN counts as the largest). Wr is (E, d), inner stride 1; X, Wr, br
  * in `dtype`. E <= 1024, k <= min(E, 32). expert_idxs, gates: (T, k) contiguous. */

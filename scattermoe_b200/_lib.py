@@ -27,6 +27,7 @@ FLAG_ALLOW_TF32 = 1
 FLAG_FORCE_SIMT = 2
 FLAG_FORCE_TC = 4
 FLAG_GATHER_ROWS = 8
+FLAG_AFTER_ROUTER = 16
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -98,7 +99,7 @@ SIGNATURES = {
                             _P, _I64, _I64,                  # ids
                             _P, _I64,                        # Y
                             _I32, _I32, _I32, _I32, _I32,    # k d F d_out E
-                            _I32, _I32, c_float, c_float, _I32, _I32, _P, c_size_t, _P], c_int32),
+                            _I32, _I32, c_float, c_float, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
     "smoe_few_token_route": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _I32, _P], c_int32),
     "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P], c_int32),
     "smoe_adapter_linear": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32,

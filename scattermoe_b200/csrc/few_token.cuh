@@ -29,20 +29,23 @@ struct Args {
   int T, k, d, F, d_out, E, act_layout, act, dtype;
   float alpha, limit;
   void* ws; size_t ws_bytes;
+  int32_t* status;
+  int after_router;     // the launch before on this stream is the router that writes ids and gates
   cudaStream_t stream;
 };
 
-int n_up(const Args& a);
+inline int n_up(const Args& a) { return a.act_layout == 0 ? a.F : 2 * a.F; }
 
 // CUDA-core kernels: fp32, and 16-bit operands the streaming kernels cannot address (any strides, any sizes).
 int launch_simt(const Args& a);
 size_t simt_workspace_bytes(int64_t T, int k, int F, int d_out);
 // Streaming tensor-core kernels; SMOE_ERR_UNSUPPORTED (no error text) when the operands do not fit them.
 int launch_stream(const Args& a);
+size_t stream_workspace_bytes(int64_t T, int k, int F, int d_out);
 
 // ---- plan --------------------------------------------------------------------------------------------
 // Slots sorted by expert (stable, so that equal inputs give bit-equal outputs) and cut into jobs.
-struct Plan {
+struct alignas(16) Plan {
   uint16_t slots[MAX_R];
   uint16_t job_expert[MAX_R];
   uint16_t job_begin[MAX_R];

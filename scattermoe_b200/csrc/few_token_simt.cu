@@ -412,7 +412,8 @@ extern "C" int32_t smoe_few_token_max_tokens(void) { return ft::MAX_T; }
 
 extern "C" size_t smoe_few_token_workspace_bytes(int64_t T, int32_t k, int32_t F, int32_t d_out) {
   if (T < 0 || k < 1 || F < 1 || d_out < 1) return 0;
-  return ft::simt_workspace_bytes(T, k, F, d_out) + 256;
+  const size_t a = ft::simt_workspace_bytes(T, k, F, d_out), b = ft::stream_workspace_bytes(T, k, F, d_out);
+  return a > b ? a : b;
 }
 
 extern "C" int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void* Wr, int64_t stride_wm,
@@ -442,7 +443,7 @@ extern "C" int smoe_few_token_mlp(const void* X, int64_t T, int64_t stride_xm, c
                                   const int64_t* expert_idxs, int64_t stride_it, int64_t stride_ik, void* Y,
                                   int64_t stride_ym, int32_t k, int32_t d, int32_t F, int32_t d_out, int32_t E,
                                   int32_t act_layout, int32_t act, float alpha, float limit, int32_t dtype, int32_t flags,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
+                                  void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   SMOE_CHECK_ARG(dtype == SMOE_F32 || dtype == SMOE_BF16 || dtype == SMOE_F16, "few_token_mlp: unknown dtype %d", dtype);
   SMOE_CHECK_ARG(gates_dtype >= 0 && gates_dtype <= 2, "few_token_mlp: unknown dtype %d of the gates", gates_dtype);
   SMOE_CHECK_ARG(T >= 0 && T <= ft::MAX_T, "few_token_mlp: %lld tokens, at most %d are taken", (long long)T, ft::MAX_T);
@@ -464,6 +465,18 @@ extern "C" int smoe_few_token_mlp(const void* X, int64_t T, int64_t stride_xm, c
              W2, stride_w2e, stride_w2k, stride_w2n, b2, stride_b2e, stride_b2n,
              gates, stride_gt, stride_gk, gates_dtype, expert_idxs, stride_it, stride_ik, Y, stride_ym,
              static_cast<int>(T), k, d, F, d_out, E, act_layout, act, dtype, alpha, limit,
-             workspace, workspace_bytes, static_cast<cudaStream_t>(stream)};
+             workspace, workspace_bytes, status, (flags & SMOE_FLAG_AFTER_ROUTER) ? 1 : 0, static_cast<cudaStream_t>(stream)};
+  if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
+    const int rc = ft::launch_stream(a);
+    if (rc != SMOE_ERR_UNSUPPORTED) {
+      if (rc == SMOE_OK) set_last_path(1);
+      return rc;
+    }
+    if (flags & SMOE_FLAG_FORCE_TC) {
+      set_error("few_token_mlp: no tensor-core kernel for this dtype/alignment (dtype=%d d=%d F=%d)", dtype, d, F);
+      return rc;
+    }
+  }
+  set_last_path(0);
   return ft::launch_simt(a);
 }

@@ -48,7 +48,7 @@ def _same(what, x, **tensors):
 
 def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Optional[torch.Tensor], ids: torch.Tensor,
               act_layout: int, act: int, up_b: Optional[torch.Tensor], down_b: Optional[torch.Tensor], alpha: float,
-              limit: float) -> torch.Tensor:
+              limit: float, after_router: bool = False) -> torch.Tensor:
     T, d = x.shape
     E, F, d_out = down.shape
     k = ids.size(1)
@@ -67,7 +67,8 @@ def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Opti
             *((gates.data_ptr(), gates.stride(0), gates.stride(1), _lib.DTYPE_CODE[gates.dtype]) if gates is not None
               else (None, 0, 0, 0)),
             ids.data_ptr(), ids.stride(0), ids.stride(1), y.data_ptr(), y.stride(0), k, d, F, d_out, E, act_layout, act,
-            alpha, limit, _lib.DTYPE_CODE[x.dtype], _path_flags(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+            alpha, limit, _lib.DTYPE_CODE[x.dtype], _path_flags() | (_lib.FLAG_AFTER_ROUTER if after_router else 0),
+            ws.data_ptr(), ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_few_token_mlp")
     return y
 
@@ -116,9 +117,9 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
 
 
-def _run_mlp(x, up, down, gates, ids, act_layout, act, up_b, down_b, alpha, limit):
+def _run_mlp(x, up, down, gates, ids, act_layout, act, up_b, down_b, alpha, limit, after_router=False):
     args = (x, up, down, gates, ids, act_layout, act, up_b, down_b, float(alpha), float(limit))
-    return few_token_mlp_compileable(*args) if torch.compiler.is_compiling() else _mlp_impl(*args)
+    return few_token_mlp_compileable(*args) if torch.compiler.is_compiling() else _mlp_impl(*args, after_router=after_router)
 
 
 def few_token_mlp(inputs, up_weights, down_weights, gates, expert_idxs, act_layout, act, up_biases=None, down_biases=None,
@@ -204,5 +205,5 @@ def few_token_moe(inputs, router_weight, up_weights, down_weights, k, act_layout
     x = _rows(inputs)
     route = few_token_route_compileable if torch.compiler.is_compiling() else _route_impl
     gates, ids = route(x, _rows(router_weight), router_bias, int(k), MODES[mode], bool(renormalize))
-    y = _run_mlp(x, up_weights, down_weights, gates, ids, act_layout, act, up_biases, down_biases, alpha, limit)
+    y = _run_mlp(x, up_weights, down_weights, gates, ids, act_layout, act, up_biases, down_biases, alpha, limit, after_router=True)
     return y, gates, ids

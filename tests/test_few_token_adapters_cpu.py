@@ -10,7 +10,7 @@ def mlp_args(**kw):
     """smoe_few_token_mlp's arguments for a small valid call on pointers that are never read."""
     a = dict(X=256, T=4, sxm=64, W1=256, w1e=64 * 128, w1k=1, w1n=64, b1=None, b1e=0, b1n=0, W2=256, w2e=64 * 64, w2k=1, w2n=64,
              b2=None, b2e=0, b2n=0, gates=256, sgt=2, sgk=1, gdt=1, ids=256, sit=2, sik=1, Y=256, sym=64, k=2, d=64, F=64, d_out=64,
-             E=4, layout=2, act=0, alpha=1.0, limit=1.0, dtype=1, flags=0, ws=256, ws_bytes=1 << 20, stream=None)
+             E=4, layout=2, act=0, alpha=1.0, limit=1.0, dtype=1, flags=0, ws=256, ws_bytes=1 << 24, status=None, stream=None)
     assert set(kw) <= set(a)
     return list({**a, **kw}.values())
 
