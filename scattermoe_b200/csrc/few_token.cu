@@ -2,14 +2,16 @@
 // down-projection with the sum over a token's experts.
 //
 // Bound: the weights of the experts that occur cross HBM once; everything else is small. So the kernels are built around
-// that stream. One block per SM; one warp keeps a ring of weight pieces in flight (up to ~190 KB per SM), eight warps multiply what has
-// arrived with mma.sync: 16 weight rows x 8 slots x 16 of K per instruction. Weights are the M side, the job's slots the N side, so a
+// that stream. One block per SM; one thread keeps a ring of weight pieces in flight by TMA, two warps gather the token rows beside them
+// (cp.async), eight warps multiply what has arrived with mma.sync: 16 weight rows x 8 slots x 16 of K per instruction. Weights are the M side, the job's slots the N side, so a
 // job of 1 to 8 slots costs one instruction per 16x16 weights and the tensor pipe stays far below its limit; a
 // tcgen05 tile would need 128 weight rows at a time, and with a handful of active experts the rows could not be spread evenly over
 // 148 SMs. Here the split is exact: a block owns a contiguous range of hidden values (up) or of output columns (down).
 //
-// Weights with contiguous inputs ("K-major", nn.Linear storage): one bulk copy per weight row and piece of K, so a block loads
-// exactly its own rows, whole and in order. Weights with contiguous outputs ("N-major"): TMA boxes of 32 columns x a piece of K, read
+// Weights with contiguous inputs ("K-major", nn.Linear storage): boxes of 64 of K x (16 hidden values x their 2 columns, or the block's
+// output columns), starting at any row, so that a range may begin anywhere (rows that two blocks load come from L2). One bulk copy
+// per weight row instead of boxes moved 1.2-3 TB/s: a block could issue one only every 40-50 ns.
+// Weights with contiguous outputs ("N-major"): boxes of 32 columns x a piece of K, read
 // through transposing ldmatrix; the columns of the down-projection are too few to fill the SMs, so there the list
 // (column tile, job, piece of K) is cut into equal parts and partial sums are joined in a fixed order by the last block of a tile.
 //
@@ -20,6 +22,7 @@
 #include <string.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "act_math.cuh"
 #include "few_token.cuh"
@@ -32,7 +35,8 @@ namespace ft {
 using namespace ptx;
 
 constexpr int CONSUMERS = 8;                       // warps that multiply
-constexpr int THREADS = (CONSUMERS + 1) * 32;      // and the one that loads
+constexpr int GATHERERS = 2;                       // warps that fetch the slots' rows
+constexpr int THREADS = (CONSUMERS + 1 + GATHERERS) * 32;      // and one whose first thread loads the weights
 constexpr int MAX_STAGES = 16;
 constexpr int BOX = 32;                            // columns of an N-major TMA box (64 bytes)
 constexpr int MAX_CTAS = 160;
@@ -46,8 +50,9 @@ struct StreamParams {
   int n_counters;
   int32_t* status;
   int NT;                     // slots of a job
-  int KC, n_chunks, K;        // piece of K (a multiple of 16), pieces, K
-  int stages, stage_bytes, x_offset, x_pitch, ring_bytes;
+  int KC, n_chunks, K;        // piece of K (a multiple of 64), pieces, K
+  int box_bytes, load_bytes;  // K-major: bytes a box of 64 of K takes in the ring, and bytes it loads
+  int stages, stage_bytes, x_offset, ring_bytes;
 };
 
 template <typename T> struct Mma;
@@ -77,14 +82,28 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldsm2(uint32_t& r0, uint32_t& r1, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr) : "memory");
 }
-// Untiled bulk copy: 16-byte aligned ends, a multiple of 16 bytes.
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+// one arrival once every cp.async this thread has issued is complete
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// Position in the ring: stage and the parity of its current pass.
+struct RingPos {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) { stage = 0; phase ^= 1; }
+  }
+};
 
 // ---- the list of runs of a block --------------------------------------------------------------------------
 // A run is a stretch of K of one (weight tile, job) pair. Up-projection: the whole K of a tile of hidden values. Down-projection: the
@@ -205,12 +224,12 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full_bar(s), 1);
+      mbar_init(full_bar(s), 1 + GATHERERS * 32);      // the weights (expect_tx) and the gatherers' threads
       mbar_init(empty_bar(s), CONSUMERS);
     }
     *abort_flag = 0;
     fence_mbar_init();
-    if (!KMAJOR) tma_prefetch_desc(&tmap);
+    tma_prefetch_desc(&tmap);
   }
   if (UP) {
     wait_for_previous_kernel();        // ids, gates (and everything else) come from it when it is the router
@@ -239,78 +258,67 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   const bool halves = pairs && a.act_layout != LAYOUT_GPT_OSS;
 
   if (warp == CONSUMERS) {
-    // ---------------- loads ------------------------------------------------------------------------------------
-    const uint8_t* W = static_cast<const uint8_t*>(UP ? a.W1 : a.W2);
-    const int64_t swe = UP ? a.s1e : a.s2e, swn = UP ? a.s1n : a.s2n;
-    auto piece = [&](int c) { return min(p.KC, p.K - c * p.KC); };
-    auto weight_rows = [&](const Run& r) { return KMAJOR ? (pairs ? 2 * r.count : r.count) : 0; };
-    auto boxes = [&](const Run& r) { return UP ? (halves ? 2 : r.count) : (r.count + BOX - 1) / BOX; };
-    auto expect = [&](int s, const Run& r, int c) {
-      const uint32_t x_bytes = static_cast<uint32_t>(plan->job_count[r.job]) * piece(c) * 2;
-      const uint32_t w_bytes = KMAJOR ? static_cast<uint32_t>(weight_rows(r)) * piece(c) * 2
-                                      : static_cast<uint32_t>(boxes(r)) * p.KC * BOX * 2;
-      if (lane == 0) mbar_arrive_expect_tx(full_bar(s), x_bytes + w_bytes);
-      __syncwarp();
-    };
-    auto load_w = [&](int s, const Run& r, int c) {
-      const uint32_t dst = ring0 + s * p.stage_bytes;
-      const int e = plan->job_expert[r.job];
-      if (KMAJOR) {
-        const int in = pairs ? lane & 15 : lane, half = pairs ? lane >> 4 : 0;
-        if (in < r.count) {
-          const int v = r.p0 + in;
-          const int64_t col = UP ? (pairs ? (halves ? static_cast<int64_t>(half) * a.F + v : 2 * static_cast<int64_t>(v) + half) : v) : v;
-          bulk_load(dst + lane * p.x_pitch, W + (e * swe + col * swn + static_cast<int64_t>(c) * p.KC) * 2, piece(c) * 2, full_bar(s));
-        }
-      } else if (lane < boxes(r)) {
-        const int col = UP ? (halves ? lane * a.F + r.p0 * BOX : (r.p0 + lane) * BOX) : r.p0 + lane * BOX;
-        tma_load_3d(dst + lane * p.KC * BOX * 2, &tmap, full_bar(s), col, c * p.KC, e);
-      }
-    };
-    auto load_x = [&](int s, const Run& r, int c) {
-      if (lane < plan->job_count[r.job]) {
-        const int at = plan->job_begin[r.job] + lane;
-        const uint8_t* src = UP ? static_cast<const uint8_t*>(a.X) + (static_cast<int64_t>(token[at]) * a.sxm + c * p.KC) * 2
-                                : p.hidden + (static_cast<int64_t>(plan->slots[at]) * a.F + c * p.KC) * 2;
-        bulk_load(ring0 + s * p.stage_bytes + p.x_offset + lane * p.x_pitch, src, piece(c) * 2, full_bar(s));
-      }
-    };
+    // ---------------- weights: they depend on no kernel before, so nothing is waited for -----------------------------
+    if (lane != 0) return;
     Run r;
-    int it = 0;
+    RingPos at;
     bool ok = true;
-    if (!UP) {
-      // fill the ring with weights, wait for the hidden rows, then fetch those of the pieces already under way
-      Walker<UP, KMAJOR> ahead = walk;
-      int filled = 0;
-      while (filled < p.stages && ahead.next(r))
-        for (int c = r.c0; c < r.c1 && filled < p.stages; ++c, ++filled) {
-          expect(filled, r, c);
-          load_w(filled, r, c);
-        }
-      wait_for_previous_kernel();
-      asm volatile("fence.proxy.async;" ::: "memory");       // hidden rows: ordinary stores there, bulk copies here
-      while (walk.next(r) && ok)
-        for (int c = r.c0; c < r.c1; ++c, ++it) {
-          const int s = it % p.stages;
-          if (it >= filled) {
-            if (!mbar_wait_warp(empty_bar(s), ((it / p.stages) & 1) ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
-            expect(s, r, c);
-            load_w(s, r, c);
+    while (walk.next(r) && ok) {
+      const int e = plan->job_expert[r.job];
+      for (int c = r.c0; c < r.c1; ++c, at.next(p.stages)) {
+        const int s = at.stage;
+        if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
+        const uint32_t dst = ring0 + s * p.stage_bytes;
+        if (KMAJOR) {
+          const int steps = (min(p.KC, p.K - c * p.KC) + 63) >> 6;
+          mbar_arrive_expect_tx(full_bar(s), steps * p.load_bytes);
+          for (int b = 0; b < steps; ++b)
+            tma_load_4d(dst + b * p.box_bytes, &tmap, full_bar(s), c * p.KC + b * 64, r.p0, 0, e);
+        } else {
+          const int n_box = UP ? (halves ? 2 : r.count) : (r.count + BOX - 1) / BOX;
+          mbar_arrive_expect_tx(full_bar(s), n_box * p.KC * BOX * 2);
+          for (int b = 0; b < n_box; ++b) {
+            const int col = UP ? (halves ? b * a.F + r.p0 * BOX : (r.p0 + b) * BOX) : r.p0 + b * BOX;
+            tma_load_3d(dst + b * p.KC * BOX * 2, &tmap, full_bar(s), col, c * p.KC, e);
           }
-          load_x(s, r, c);
         }
-    } else {
-      while (walk.next(r) && ok)
-        for (int c = r.c0; c < r.c1; ++c, ++it) {
-          const int s = it % p.stages;
-          if (!mbar_wait_warp(empty_bar(s), ((it / p.stages) & 1) ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
-          expect(s, r, c);
-          load_w(s, r, c);
-          load_x(s, r, c);
-        }
+      }
     }
     if (!ok)      // give copies already in flight time to land before the block goes away
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    return;
+  }
+  if (warp > CONSUMERS) {
+    // ---------------- the slots' rows: 16 bytes per thread, zeros beyond K ---------------------------------------------
+    if (!UP) wait_for_previous_kernel();
+    const int g = tid - (CONSUMERS + 1) * 32, chunk = g & 7, row0 = g >> 3;      // rows row0, row0 + 8, ...
+    const uint32_t sw = static_cast<uint32_t>((chunk ^ row0) << 4);              // row & 7 == row0
+    Run r;
+    RingPos at;
+    bool ok = true;
+    while (walk.next(r) && ok) {
+      const int n = plan->job_count[r.job], beg = plan->job_begin[r.job];
+      const uint8_t* src[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = beg + min(row0 + 8 * i, n - 1);
+        src[i] = UP ? static_cast<const uint8_t*>(a.X) + static_cast<int64_t>(token[j]) * a.sxm * 2
+                    : p.hidden + static_cast<int64_t>(plan->slots[j]) * a.F * 2;
+      }
+      for (int c = r.c0; c < r.c1; ++c, at.next(p.stages)) {
+        const int s = at.stage;
+        if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 23)) { ok = false; break; }
+        const uint32_t dst = ring0 + s * p.stage_bytes + p.x_offset + row0 * 128 + sw;
+        const int k0 = c * p.KC + chunk * 8, k_end = min((c + 1) * p.KC, (p.K + 63) & ~63);
+        for (int kk = k0, b = 0; kk < k_end; kk += 64, ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (row0 + 8 * i < n)
+              cp_async16(dst + (b * p.NT + 8 * i) * 128, src[i] + (kk < p.K ? kk * 2 : 0), kk < p.K ? 16 : 0);
+        cp_async_arrive(full_bar(s));
+      }
+    }
+    cp_async_wait<0>();
     return;
   }
 
@@ -318,11 +326,28 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   // a wait that runs out does not leave the loops: the barriers below stay matched, the results are reported as invalid
   if (!UP) wait_for_previous_kernel();
   bool ok = true;
-  int it = 0;
+  RingPos at;
   Run r;
   const int my_box = KMAJOR ? 0 : warp >> 2;
-  constexpr int SLICES = KMAJOR ? 8 : 4;
-  const int my_slice = KMAJOR ? warp : warp & 3;
+  // ldmatrix addresses of this lane inside a stage; the loop over K only adds multiples of a block of 64
+  uint32_t a_lane[2], x_lane[2], x_lane4[2];       // K-major: the two 16-wide steps of the warp's half of a block of 64
+  {
+    const int row = (lane & 7) + ((lane >> 3) & 1) * 8, xrow4 = (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int step = KMAJOR ? (warp & 1) * 2 + i : warp & 3;
+      a_lane[i] = KMAJOR ? row * 128 + (((step * 2 + (lane >> 4)) ^ (row & 7)) << 4) : 0;
+      x_lane[i] = (lane & 7) * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
+      x_lane4[i] = xrow4 * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (xrow4 & 7)) << 4);
+    }
+    if (!KMAJOR) {
+      const int krow = (warp & 3) * 16 + (lane & 7) + (lane >> 4) * 8, chunk = (lane >> 3) & 1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)                  // N-major: the two 16-column halves of the warp's box
+        a_lane[i] = my_box * p.KC * BOX * 2 + krow * (BOX * 2) + (((chunk + 2 * i) ^ ((krow >> 1) & 3)) << 4);
+    }
+  }
+  const int x_block = p.NT * 128;
   auto total_of = [&](int i, int row) {       // sum over the warps that share this row
     float v = 0.f;
     if (KMAJOR) {
@@ -355,51 +380,60 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
       for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int q = 0; q < 4; ++q) acc[m][g][q] = 0.f;
-    for (int c = r.c0; c < r.c1; ++c, ++it) {
-      const int s = it % p.stages;
-      if (ok) ok = mbar_wait_warp(full_bar(s), (it / p.stages) & 1, abort_flag, p.status, 22);
-      if (ok && use0) {
-        const int len = min(p.KC, p.K - c * p.KC);
-        const uint32_t wst = ring0 + s * p.stage_bytes, xst = wst + p.x_offset;
-        for (int k0 = my_slice * 16; k0 < len; k0 += SLICES * 16) {
-          uint32_t a0[4], a1[4] = {0, 0, 0, 0}, b[4][2];
-          if (KMAJOR) {
-            const uint32_t at = wst + ((lane & 7) + ((lane >> 3) & 1) * 8) * p.x_pitch + (k0 + (lane >> 4) * 8) * 2;
-            ldsm4(a0, at);
-            if (use1) ldsm4(a1, at + 16 * p.x_pitch);
-          } else {
-            const int krow = k0 + (lane & 7) + (lane >> 4) * 8, chunk = (lane >> 3) & 1;
-            const uint32_t row = wst + my_box * p.KC * BOX * 2 + krow * (BOX * 2);
-            ldsm4_trans(a0, row + ((chunk ^ ((krow >> 1) & 3)) << 4));
-            if (use1) ldsm4_trans(a1, row + (((chunk + 2) ^ ((krow >> 1) & 3)) << 4));
-          }
-          if (groups == 1) {
-            ldsm2(b[0][0], b[0][1], xst + (lane & 7) * p.x_pitch + (k0 + ((lane >> 3) & 1) * 8) * 2);
-          } else {
+    auto stream = [&](auto G_) {
+      constexpr int G = decltype(G_)::value;           // groups of 8 slots, rounded up to 1, 2 or 4
+      for (int c = r.c0; c < r.c1; ++c, at.next(p.stages)) {
+        const int s = at.stage;
+        if (ok) ok = mbar_wait_warp(full_bar(s), at.phase, abort_flag, p.status, 22);
+        if (ok && use0) {
+          const int blocks = (min(p.KC, p.K - c * p.KC) + 63) >> 6;
+          const uint32_t wst = ring0 + s * p.stage_bytes, xst = wst + p.x_offset;
+          auto step = [&](uint32_t w0, uint32_t w1, uint32_t x1, uint32_t x4) {
+            uint32_t a0[4], a1[4] = {0, 0, 0, 0}, b[G][2];
+            if (KMAJOR) {
+              ldsm4(a0, w0);
+              if (use1) ldsm4(a1, w1);
+            } else {
+              ldsm4_trans(a0, w0);
+              if (use1) ldsm4_trans(a1, w1);
+            }
+            if (G == 1) {
+              ldsm2(b[0][0], b[0][1], x1);
+            } else {
 #pragma unroll
-            for (int g = 0; g < 4; g += 2)
-              if (g < groups) {
+              for (int g = 0; g < G; g += 2) {
                 uint32_t t[4];
-                ldsm4(t, xst + ((lane & 7) + (lane >> 4) * 8 + g * 8) * p.x_pitch + (k0 + ((lane >> 3) & 1) * 8) * 2);
+                ldsm4(t, x4 + g * 8 * 128);
                 b[g][0] = t[0]; b[g][1] = t[1]; b[g + 1][0] = t[2]; b[g + 1][1] = t[3];
               }
-          }
-          if (k0 + 16 > len) {                // half a step is left (K is a multiple of 8): nothing was loaded beyond it
-            a0[2] = a0[3] = a1[2] = a1[3] = 0;
+            }
 #pragma unroll
-            for (int g = 0; g < 4; ++g) b[g][1] = 0;
-          }
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            if (g < groups) {
+            for (int g = 0; g < G; ++g) {
               Mma<T>::run(acc[0][g], a0, b[g][0], b[g][1]);
               if (use1) Mma<T>::run(acc[1][g], a1, b[g][0], b[g][1]);
             }
+          };
+          if (KMAJOR) {
+            for (int b = warp >> 1; b < blocks; b += 4) {
+              const uint32_t w = wst + b * p.box_bytes, x = xst + b * x_block;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) step(w + a_lane[i], w + a_lane[i] + 16 * 128, x + x_lane[i], x + x_lane4[i]);
+            }
+          } else {
+#pragma unroll 2
+            for (int b = 0; b < blocks; ++b) {
+              const uint32_t w = wst + b * (64 * BOX * 2), x = xst + b * x_block;
+              step(w + a_lane[0], w + a_lane[1], x + x_lane[0], x + x_lane4[0]);
+            }
+          }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty_bar(s));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty_bar(s));
-    }
+    };
+    if (groups == 1) stream(std::integral_constant<int, 1>{});
+    else if (groups == 2) stream(std::integral_constant<int, 2>{});
+    else stream(std::integral_constant<int, 4>{});
     // ---- join the warps' parts of K
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -407,11 +441,11 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
           if (g < groups) {
-            float* at = red + (warp * p.NT + g * 8 + (lane & 3) * 2) * RED_PITCH + m * 16 + (lane >> 2);
-            at[0] = acc[m][g][0];
-            at[RED_PITCH] = acc[m][g][1];
-            at[8] = acc[m][g][2];
-            at[RED_PITCH + 8] = acc[m][g][3];
+            float* out = red + (warp * p.NT + g * 8 + (lane & 3) * 2) * RED_PITCH + m * 16 + (lane >> 2);
+            out[0] = acc[m][g][0];
+            out[RED_PITCH] = acc[m][g][1];
+            out[8] = acc[m][g][2];
+            out[RED_PITCH + 8] = acc[m][g][3];
           }
     consumers_sync();
     if (UP) {
@@ -519,9 +553,36 @@ size_t stream_workspace_bytes(int64_t T, int k, int F, int d_out) {
 
 struct Order { bool k_major, n_major; };
 static Order weight_order(const void* W, int64_t se, int64_t sk, int64_t sn, int K, int N) {
-  if (!al16(W) || se % 8) return {false, false};
-  return {sk == 1 && sn % 8 == 0, sn == 1 && sk % 8 == 0 && sk >= N && se >= 0 && N % 8 == 0};
+  if (!al16(W) || se % 8 || se < 0) return {false, false};
+  return {sk == 1 && sn % 8 == 0 && sn >= K, sn == 1 && sk % 8 == 0 && sk >= N && N % 8 == 0};
 }
+
+// Pieces of K: multiples of 64, at most `most`, all but the last alike.
+static int piece_of(int K, int most) {
+  const int blocks = cdiv(K, 64), n = cdiv(blocks, most / 64);
+  return cdiv(blocks, n) * 64;
+}
+
+// K-major boxes: 64 of K x `rows` x `halves` (the two columns of a hidden value; 1 without a gate) of one expert.
+static bool encode_k_major(CUtensorMap* map, bool bf16, const void* W, int K, int rows_total, int64_t row_stride, int halves,
+                           int64_t half_stride, int E, int64_t se, int box_rows) {
+  const uint64_t dim[4] = {static_cast<uint64_t>(K), static_cast<uint64_t>(rows_total), static_cast<uint64_t>(halves),
+                           static_cast<uint64_t>(E)};
+  // the stride of an axis of one element is never used, but has to be valid
+  const uint64_t stride[3] = {static_cast<uint64_t>(row_stride) * 2, static_cast<uint64_t>(halves > 1 ? half_stride : row_stride) * 2,
+                              static_cast<uint64_t>(E > 1 ? se : row_stride) * 2};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), static_cast<uint32_t>(halves), 1};
+  return encode_tensor_map(map, bf16, W, 4, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+static bool encode_n_major(CUtensorMap* map, bool bf16, const void* W, int N, int K, int64_t row_stride, int E, int64_t se, int box_k) {
+  const uint64_t dim[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(K), static_cast<uint64_t>(E)};
+  const uint64_t stride[2] = {static_cast<uint64_t>(row_stride) * 2, static_cast<uint64_t>(E > 1 ? se : row_stride) * 2};
+  const uint32_t box[3] = {BOX, static_cast<uint32_t>(box_k), 1};
+  return encode_tensor_map(map, bf16, W, 3, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// rows of a K-major box: the hidden values of a tile, or the output columns of a block (at most 32)
+static int down_rows(int d_out, int grid) { return cdiv(d_out, grid) < 32 ? cdiv(d_out, grid) : 32; }
 
 template <typename T, bool UP, bool KMAJOR>
 static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& di, int grid) {
@@ -531,33 +592,27 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
                     (UP ? 0 : a.T * ((KMAJOR ? 32 : 2 * BOX) + 1) * 4) + 1024 + 64;
   const int budget = (di.max_smem_optin < 232448 ? di.max_smem_optin : 232448) - fixed;
   if (KMAJOR) {
-    // A stage is a piece of K of up to 32 weight rows and NT token rows, each row padded by 16 bytes (conflict-free ldmatrix). About
-    // five stages: pieces long enough that a bulk copy per row is cheap, enough of them that the stream never stops.
-    const int rows = (UP ? 32 : (cdiv(a.d_out, grid) < 32 ? cdiv(a.d_out, grid) : 32)) + p.NT;
-    int kc = (budget / (5 * rows) - 16) / 2 / 16 * 16;
-    kc = kc > 1024 ? 1024 : (kc < 64 ? 64 : kc);
-    p.n_chunks = cdiv(p.K, kc);
-    p.KC = cdiv(cdiv(p.K, p.n_chunks), 16) * 16;
-    p.n_chunks = cdiv(p.K, p.KC);
-    p.x_pitch = p.KC * 2 + 16;
-    p.x_offset = (rows - p.NT) * p.x_pitch;
-    p.stage_bytes = rows * p.x_pitch;
-    p.stages = (budget - 16 * p.x_pitch) / p.stage_bytes;
+    const int rows = UP ? 32 : down_rows(a.d_out, grid);
+    p.load_bytes = rows * 128;
+    p.box_bytes = cdiv(rows, 8) * 1024;                    // boxes start on the swizzle's period
+    // Stages of up to 32 KB of weights where the ring then still holds four, else 16 KB: enough of them that the stream never stops,
+    // few enough that a stage is worth its waits (16 KB stages with one slot per job were bound by the warps' loop overhead).
+    const int block = p.box_bytes + p.NT * 128;            // bytes of 64 of K: weights and slots
+    p.KC = piece_of(p.K, 64 * (32768 / p.box_bytes));
+    if ((budget - 2048) / (p.KC / 64 * block) < 4) p.KC = piece_of(p.K, 64 * (16384 / p.box_bytes));
+    p.x_offset = p.KC / 64 * p.box_bytes;
   } else {
-    // two boxes of 32 columns and the token rows; boxes are 512-byte aligned
-    int kc = 256;
-    p.n_chunks = cdiv(p.K, kc);
-    p.KC = cdiv(cdiv(p.K, p.n_chunks), 16) * 16;
-    p.n_chunks = cdiv(p.K, p.KC);
-    p.x_pitch = p.KC * 2 + 16;
+    p.load_bytes = p.box_bytes = 0;
+    p.KC = piece_of(p.K, 256);                             // as the tensor map's boxes
     p.x_offset = 2 * p.KC * BOX * 2;
-    p.stage_bytes = (p.x_offset + p.NT * p.x_pitch + 1023) / 1024 * 1024;
-    p.stages = budget / p.stage_bytes;
   }
+  p.n_chunks = cdiv(p.K, p.KC);
+  p.stage_bytes = p.x_offset + p.KC / 64 * p.NT * 128;
+  p.stages = (budget - (KMAJOR ? 2048 : 0)) / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   if (p.stages < 2) return SMOE_ERR_UNSUPPORTED;
-  // ldmatrix reads whole 16-row blocks: up to 15 rows past a stage whose weight rows are fewer (never used, but inside the ring)
-  p.ring_bytes = p.stages * p.stage_bytes + (KMAJOR ? 16 * p.x_pitch : 0);
+  // ldmatrix reads whole 16-row blocks: up to 8 rows past a box of fewer rows (never used, but inside the ring)
+  p.ring_bytes = p.stages * p.stage_bytes + (KMAJOR ? 2048 : 0);
   const int scratch = (plan_scratch_bytes(a.E) + 15) / 16 * 16;      // the plan sorts in the ring before the first copy
   if (scratch > budget) return SMOE_ERR_UNSUPPORTED;
   if (p.ring_bytes < scratch) p.ring_bytes = scratch;
@@ -604,15 +659,13 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
   CUtensorMap m1, m2;
   memset(&m1, 0, sizeof(m1));
   memset(&m2, 0, sizeof(m2));
-  auto box_rows = [](int K) { const int n = cdiv(K, 256); return cdiv(cdiv(K, n), 16) * 16; };
-  if (!o1.k_major &&
-      !encode_tensor_map(&m1, bf16, a.W1, n_up_cols, a.d, a.E, static_cast<uint64_t>(a.s1k) * 2,
-                         (a.E > 1 ? static_cast<uint64_t>(a.s1e) : static_cast<uint64_t>(a.s1k) * a.d) * 2, BOX, box_rows(a.d), CU_TENSOR_MAP_SWIZZLE_64B))
-    return SMOE_ERR_UNSUPPORTED;
-  if (!o2.k_major &&
-      !encode_tensor_map(&m2, bf16, a.W2, a.d_out, a.F, a.E, static_cast<uint64_t>(a.s2k) * 2,
-                         (a.E > 1 ? static_cast<uint64_t>(a.s2e) : static_cast<uint64_t>(a.s2k) * a.F) * 2, BOX, box_rows(a.F), CU_TENSOR_MAP_SWIZZLE_64B))
-    return SMOE_ERR_UNSUPPORTED;
+  const bool pairs = a.act_layout != LAYOUT_PLAIN, woven = a.act_layout == LAYOUT_GPT_OSS;
+  const bool ok1 = o1.k_major ? encode_k_major(&m1, bf16, a.W1, a.d, a.F, woven ? 2 * a.s1n : a.s1n, pairs ? 2 : 1,
+                                               woven ? a.s1n : a.s1n * a.F, a.E, a.s1e, pairs ? 16 : 32)
+                              : encode_n_major(&m1, bf16, a.W1, n_up_cols, a.d, a.s1k, a.E, a.s1e, piece_of(a.d, 256));
+  const bool ok2 = o2.k_major ? encode_k_major(&m2, bf16, a.W2, a.F, a.d_out, a.s2n, 1, 0, a.E, a.s2e, down_rows(a.d_out, grid))
+                              : encode_n_major(&m2, bf16, a.W2, a.d_out, a.F, a.s2k, a.E, a.s2e, piece_of(a.F, 256));
+  if (!ok1 || !ok2) return SMOE_ERR_UNSUPPORTED;
   p.K = a.d;
   if (int rc = o1.k_major ? launch_one<T, true, true>(p, m1, di, grid) : launch_one<T, true, false>(p, m1, di, grid)) return rc;
   p.K = a.F;

@@ -24,18 +24,22 @@ inline TensorMapEncodeFn tensor_map_encoder() {
   return fn;
 }
 
-// Axis 0 is contiguous; `stride1` / `stride2` in bytes (multiples of 16). Elements outside the axes read as zero.
-inline bool encode_tensor_map(CUtensorMap* map, bool bf16, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t stride1,
-                              uint64_t stride2, uint32_t box0, uint32_t box1, CUtensorMapSwizzle swizzle) {
+// Axis 0 is contiguous; `stride[i]` of axis i + 1 in bytes (multiples of 16). Elements outside the axes read as zero.
+inline bool encode_tensor_map(CUtensorMap* map, bool bf16, const void* base, int rank, const uint64_t* dim, const uint64_t* stride,
+                              const uint32_t* box, CUtensorMapSwizzle swizzle) {
   TensorMapEncodeFn fn = tensor_map_encoder();
   if (!fn) return false;
-  const cuuint64_t dims[3] = {d0, d1, d2};
-  const cuuint64_t strides[2] = {stride1, stride2};
-  const cuuint32_t box[3] = {box0, box1, 1};
-  const cuuint32_t step[3] = {1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base), dims, strides,
-            box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t boxes[5], step[5];
+  for (int i = 0; i < rank; ++i) {
+    dims[i] = dim[i];
+    boxes[i] = box[i];
+    step[i] = 1;
+    if (i + 1 < rank) strides[i] = stride[i];
+  }
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
+            const_cast<void*>(base), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace smoe
