@@ -2,18 +2,28 @@
 // down-projection with the sum over a token's experts.
 //
 // Bound: the weights of the experts that occur cross HBM once; everything else is small. So the kernels are built around
-// that stream. One block per SM; one thread keeps a ring of weight pieces in flight by TMA, two warps gather the token rows beside them
-// (cp.async), eight warps multiply what has arrived with mma.sync: 16 weight rows x 8 slots x 16 of K per instruction. Weights are the M side, the job's slots the N side, so a
-// job of 1 to 8 slots costs one instruction per 16x16 weights and the tensor pipe stays far below its limit; a
-// tcgen05 tile would need 128 weight rows at a time, and with a handful of active experts the rows could not be spread evenly over
-// 148 SMs. Here the split is exact: a block owns a contiguous range of hidden values (up) or of output columns (down).
+// that stream. One block per SM; four threads keep a ring of weight boxes in flight by TMA (4 KB each: 32 weight rows x 64 of K), two
+// warps gather the slots' rows beside them (cp.async), eight warps multiply what has arrived with mma.sync: 16 weight rows x 8 slots x
+// 16 of K per instruction. Weights are the M side, the job's slots the N side, so a job of 1 to 8 slots costs one instruction
+// per 16x16 weights and the tensor pipe stays far below its limit; a tcgen05 tile would need 128 weight rows at a time,
+// and with a handful of active experts the rows could not be spread evenly over 148 SMs. Here the split is exact: a block owns a
+// contiguous range of hidden values (up) or of output columns (down).
 //
-// Weights with contiguous inputs ("K-major", nn.Linear storage): boxes of 64 of K x (16 hidden values x their 2 columns, or the block's
-// output columns), starting at any row, so that a range may begin anywhere (rows that two blocks load come from L2). One bulk copy
-// per weight row instead of boxes moved 1.2-3 TB/s: a block could issue one only every 40-50 ns.
-// Weights with contiguous outputs ("N-major"): boxes of 32 columns x a piece of K, read
-// through transposing ldmatrix; the columns of the down-projection are too few to fill the SMs, so there the list
-// (column tile, job, piece of K) is cut into equal parts and partial sums are joined in a fixed order by the last block of a tile.
+//   up    A round is up to 8 tiles of one job, a tile 32 weight rows: 16 hidden values with their two columns, or 32 without a gate. Each
+//         warp owns a tile over the whole of K and makes its hidden values in registers: no exchange between warps, no barrier; the
+//         slots' rows are fetched once per round.
+//   down  The block's output columns are one tile. The warps split every piece of K and add each job's result to
+//         token sums of their own in shared memory; the eight are joined, in order, once at the end.
+//
+// A first version gave the warps parts of K in both kernels and joined them after every tile and job: with many small jobs the
+// joins cost as much as the stream (24 tokens on 128 experts of 9.4 MB: 126 + 127 us against 97 + 49 of reading).
+// Issuing is what limits such a stream, not depth: one thread issues a box every 70-150 ns, so one thread moved 3.7 TB/s of 4 KB boxes
+// (2.5 of 1.8 KB ones) with 25 to 190 KB in flight alike, two 5.4, four 5.4-5.7 (3.7-6.5). One bulk copy per weight row: 1.2-3 TB/s.
+//
+// Weights with contiguous inputs ("K-major", nn.Linear storage) are read through ldmatrix and may start at any row, so that a range may
+// begin anywhere (rows that two blocks load come from L2); weights with contiguous outputs ("N-major") through the transposing
+// form. N-major columns are too few to give every SM its own, so there the down-projection's list (column tile, job, piece of K)
+// is cut into equal parts and partial sums are joined in a fixed order by the last block of a tile.
 //
 // The down-projection starts (programmatic launch) while the up-projection drains: it plans and fills its ring with weights, which do not
 // depend on the hidden rows, and waits only before the first hidden row is read.
@@ -35,24 +45,28 @@ namespace ft {
 using namespace ptx;
 
 constexpr int CONSUMERS = 8;                       // warps that multiply
+constexpr int LOADERS = 4;                         // warps whose first thread loads weights, each every fourth box of a stage
 constexpr int GATHERERS = 2;                       // warps that fetch the slots' rows
-constexpr int THREADS = (CONSUMERS + 1 + GATHERERS) * 32;      // and one whose first thread loads the weights
+constexpr int THREADS = (CONSUMERS + LOADERS + GATHERERS) * 32;
 constexpr int MAX_STAGES = 16;
-constexpr int BOX = 32;                            // columns of an N-major TMA box (64 bytes)
+constexpr int TILE = 32;                           // weight rows (output columns) of a tile
+constexpr int BLOCK_K = 64;                        // K of a box: one 128-byte line of 16-bit values
 constexpr int MAX_CTAS = 160;
-constexpr int RED_PITCH = 33;
 
 struct StreamParams {
   Args a;
   uint8_t* hidden;            // (R, F), storage type of the tokens
-  float* partial;             // N-major down-projection: [block][2][T][2 * BOX]
+  float* partial;             // N-major down-projection: [block][2][T][TILE]
   int* counters;              // one per column tile of it, zeroed by the up-projection
   int n_counters;
   int32_t* status;
   int NT;                     // slots of a job
-  int KC, n_chunks, K;        // piece of K (a multiple of 64), pieces, K
-  int box_bytes, load_bytes;  // K-major: bytes a box of 64 of K takes in the ring, and bytes it loads
+  int K, blocks;              // K and its boxes
+  int box_bytes, load_bytes;  // bytes a box takes in the ring, and bytes it loads
+  int slots;                  // boxes of a stage (up: at most one per warp and step of K; down: steps of K)
+  int x_slots;                // steps of K of the slots' rows a stage can hold
   int stages, stage_bytes, x_offset, ring_bytes;
+  int rows;                   // down: rows of a tile's token sums (the tile's columns)
 };
 
 template <typename T> struct Mma;
@@ -106,81 +120,80 @@ struct RingPos {
 };
 
 // ---- the list of runs of a block --------------------------------------------------------------------------
-// A run is a stretch of K of one (weight tile, job) pair. Up-projection: the whole K of a tile of hidden values. Down-projection: the
-// runs of a tile follow each other and their results add up; `last` closes the tile (for this block).
-struct Run { int job, c0, c1, p0, count, tile; bool first, last; };
+// A run is a stretch of K of one job: up, a round of `tiles` tiles over the whole of K, `nb` steps of K per stage; down, (part
+// of) the K of the block's tile. The runs of a tile follow each other; `last` closes the tile (for this block).
+struct Run { int job, b0, b1, nb, p0, count, tiles, tile; bool first, last; };
 
 template <bool UP, bool KMAJOR>
 struct Walker {
-  int lo, hi, units, jobs, chunks, width, per_tile, r1, job;
+  int lo, hi, units, jobs, blocks, width, per_tile, job, slots, x_slots;
 
-  // up: units = hidden values (K-major) or box groups (N-major) of one job; [lo, hi) is this block's part of all jobs' units.
-  // down, K-major: [lo, r1) are this block's output columns. down, N-major: [lo, hi) is its part of the flat list of pieces.
+  // up, K-major: [lo, hi) is this block's part of all jobs' hidden values; N-major: of all jobs' tiles (boxes start on a multiple).
+  // down, K-major: [lo, hi) are this block's output columns; N-major: its part of the flat list of steps of K.
   __device__ void init(const StreamParams& p, int n_jobs) {
     jobs = n_jobs;
-    chunks = p.n_chunks;
-    const int64_t b = blockIdx.x, g = gridDim.x;
-    const bool pairs = p.a.act_layout != LAYOUT_PLAIN, halves = pairs && p.a.act_layout != LAYOUT_GPT_OSS;
+    blocks = p.blocks;
+    slots = p.slots;
+    x_slots = p.x_slots;
     job = 0;
+    const int64_t b = blockIdx.x, g = gridDim.x;
+    int64_t total;
     if (UP) {
       width = p.a.F;
-      if (KMAJOR) {
-        units = p.a.F;
-        per_tile = pairs ? 16 : 32;
-      } else {
-        units = halves ? (p.a.F + BOX - 1) / BOX : ((pairs ? 2 * p.a.F : p.a.F) + BOX - 1) / BOX;
-        per_tile = halves ? 1 : 2;
-      }
-      const int64_t total = static_cast<int64_t>(units) * jobs;
-      lo = static_cast<int>(total * b / g);
-      hi = static_cast<int>(total * (b + 1) / g);
-    } else if (KMAJOR) {
-      width = p.a.d_out;
-      lo = static_cast<int>(static_cast<int64_t>(width) * b / g);
-      r1 = static_cast<int>(static_cast<int64_t>(width) * (b + 1) / g);
+      per_tile = p.a.act_layout != LAYOUT_PLAIN ? TILE / 2 : TILE;
+      units = KMAJOR ? width : (width + per_tile - 1) / per_tile;
+      total = static_cast<int64_t>(units) * jobs;
     } else {
       width = p.a.d_out;
-      units = jobs * chunks;      // pieces of one column tile
-      const int64_t total = static_cast<int64_t>(units) * ((width + 2 * BOX - 1) / (2 * BOX));
-      lo = static_cast<int>(total * b / g);
-      hi = static_cast<int>(total * (b + 1) / g);
+      units = jobs * blocks;      // steps of K of one column tile
+      total = KMAJOR ? width : static_cast<int64_t>(units) * ((width + TILE - 1) / TILE);
     }
+    lo = static_cast<int>(total * b / g);
+    hi = static_cast<int>(total * (b + 1) / g);
   }
   __device__ bool next(Run& r) {
+    if (lo >= hi) return false;
+    r.b0 = 0;
+    r.b1 = blocks;
+    r.first = r.last = true;
     if (UP) {
-      if (lo >= hi) return false;
       r.job = lo / units;
-      r.p0 = lo - r.job * units;
-      r.count = min(min(per_tile, units - r.p0), hi - lo);
-      r.c0 = 0;
-      r.c1 = chunks;
-      r.first = r.last = true;
-      lo += r.count;
+      const int in = lo - r.job * units;
+      if (KMAJOR) {
+        r.p0 = in;
+        r.count = min(min(CONSUMERS * per_tile, units - in), hi - lo);
+        lo += r.count;
+        r.tiles = (r.count + per_tile - 1) / per_tile;
+      } else {
+        r.tiles = min(min(CONSUMERS, units - in), hi - lo);
+        lo += r.tiles;
+        r.p0 = in * per_tile;
+        r.count = min(r.tiles * per_tile, width - r.p0);
+      }
+      r.nb = min(x_slots, slots / r.tiles);
       return true;
     }
+    r.tiles = 1;
+    r.nb = slots;
     if (KMAJOR) {
-      if (lo >= r1) return false;
       r.job = job;
       r.p0 = lo;
-      r.count = min(32, r1 - lo);
-      r.c0 = 0;
-      r.c1 = chunks;
+      r.count = min(TILE, hi - lo);
       r.first = job == 0;
       r.last = ++job == jobs;
       if (r.last) { job = 0; lo += r.count; }
       return true;
     }
-    if (lo >= hi) return false;
     r.tile = lo / units;
     const int in = lo - r.tile * units;
-    r.job = in / chunks;
-    r.c0 = in - r.job * chunks;
-    r.c1 = min(chunks, r.c0 + (hi - lo));
-    r.p0 = r.tile * 2 * BOX;
-    r.count = min(2 * BOX, width - r.p0);
+    r.job = in / blocks;
+    r.b0 = in - r.job * blocks;
+    r.b1 = min(blocks, r.b0 + (hi - lo));
+    r.p0 = r.tile * TILE;
+    r.count = min(TILE, width - r.p0);
     r.first = job == 0 || in == 0;     // `job` only marks "not the first run of the block" here
     job = 1;
-    lo += r.c1 - r.c0;
+    lo += r.b1 - r.b0;
     r.last = lo >= hi || lo % units == 0;
     return true;
   }
@@ -204,18 +217,15 @@ __global__ void __launch_bounds__(THREADS, 1)
 ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
-  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);      // the ring first: 64-byte swizzle wants 512-byte alignment
-  uint8_t* ring = smem;
+  uint8_t* ring = smem_raw + (((raw + 1023u) & ~1023u) - raw);      // the ring first: boxes start on the swizzle's period
   uint8_t* rest = ring + p.ring_bytes;
   Plan* plan = reinterpret_cast<Plan*>(rest);
   uint8_t* token = rest + sizeof(Plan);                              // token of every listed slot (T <= 128)
   uint64_t* bars = reinterpret_cast<uint64_t*>(token + MAX_R);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * MAX_STAGES);
   int* joined = reinterpret_cast<int*>(bars + 2 * MAX_STAGES) + 1;
-  float* red = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);   // [8][NT][RED_PITCH]
-  constexpr int RT = KMAJOR ? 32 : 2 * BOX;                           // weight rows (output columns) of a tile
-  constexpr int OP = RT + 1;
-  float* oacc = red + 8 * p.NT * RED_PITCH;                          // down: [T][OP]
+  float* sums = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // down: [warp][T][rows + 1]
+  const int pitch = p.rows + 1;
   const Args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t ring0 = smem_u32(ring), bar0 = smem_u32(bars);
@@ -224,7 +234,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full_bar(s), 1 + GATHERERS * 32);      // the weights (expect_tx) and the gatherers' threads
+      mbar_init(full_bar(s), LOADERS + GATHERERS * 32);      // the weights (expect_tx) and the gatherers' threads
       mbar_init(empty_bar(s), CONSUMERS);
     }
     *abort_flag = 0;
@@ -255,32 +265,31 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   Walker<UP, KMAJOR> walk;
   walk.init(p, plan->jobs);
   const bool pairs = UP && a.act_layout != LAYOUT_PLAIN;
-  const bool halves = pairs && a.act_layout != LAYOUT_GPT_OSS;
+  const bool woven = pairs && a.act_layout == LAYOUT_GPT_OSS;
+  const bool halves = !KMAJOR && pairs && !woven;      // N-major: a box is 16 columns of one half and 16 of the other
 
-  if (warp == CONSUMERS) {
+  if (warp >= CONSUMERS && warp < CONSUMERS + LOADERS) {
     // ---------------- weights: they depend on no kernel before, so nothing is waited for -----------------------------
     if (lane != 0) return;
+    const int mine = warp - CONSUMERS;
     Run r;
     RingPos at;
     bool ok = true;
     while (walk.next(r) && ok) {
       const int e = plan->job_expert[r.job];
-      for (int c = r.c0; c < r.c1; ++c, at.next(p.stages)) {
-        const int s = at.stage;
+      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
+        const int s = at.stage, steps = min(r.nb, r.b1 - b), total = r.tiles * steps;
         if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
         const uint32_t dst = ring0 + s * p.stage_bytes;
-        if (KMAJOR) {
-          const int steps = (min(p.KC, p.K - c * p.KC) + 63) >> 6;
-          mbar_arrive_expect_tx(full_bar(s), steps * p.load_bytes);
-          for (int b = 0; b < steps; ++b)
-            tma_load_4d(dst + b * p.box_bytes, &tmap, full_bar(s), c * p.KC + b * 64, r.p0, 0, e);
-        } else {
-          const int n_box = UP ? (halves ? 2 : r.count) : (r.count + BOX - 1) / BOX;
-          mbar_arrive_expect_tx(full_bar(s), n_box * p.KC * BOX * 2);
-          for (int b = 0; b < n_box; ++b) {
-            const int col = UP ? (halves ? b * a.F + r.p0 * BOX : (r.p0 + b) * BOX) : r.p0 + b * BOX;
-            tma_load_3d(dst + b * p.KC * BOX * 2, &tmap, full_bar(s), col, c * p.KC, e);
-          }
+        mbar_arrive_expect_tx(full_bar(s), (total - mine + LOADERS - 1) / LOADERS * p.load_bytes);
+        for (int q = mine; q < total; q += LOADERS) {
+          const int t = UP ? q / steps : 0, i = q - t * steps;
+          const uint32_t to = dst + (t * r.nb + i) * p.box_bytes;
+          const int kk = (b + i) * BLOCK_K, v = r.p0 + t * walk.per_tile;
+          // K-major: (K, value, column of the value, expert). N-major: (column, half, K, expert).
+          if (KMAJOR) tma_load_4d(to, &tmap, full_bar(s), kk, UP ? v : r.p0, 0, e);
+          else tma_load_4d(to, &tmap, full_bar(s), UP ? (woven ? 2 * v : v) : r.p0, 0, kk, e);
+          if (halves) tma_load_4d(to + 2048, &tmap, full_bar(s), v, 1, kk, e);
         }
       }
     }
@@ -288,11 +297,11 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
       for (int i = 0; i < 64; ++i) __nanosleep(1000);
     return;
   }
-  if (warp > CONSUMERS) {
+  if (warp >= CONSUMERS + LOADERS) {
     // ---------------- the slots' rows: 16 bytes per thread, zeros beyond K ---------------------------------------------
     if (!UP) wait_for_previous_kernel();
-    const int g = tid - (CONSUMERS + 1) * 32, chunk = g & 7, row0 = g >> 3;      // rows row0, row0 + 8, ...
-    const uint32_t sw = static_cast<uint32_t>((chunk ^ row0) << 4);              // row & 7 == row0
+    const int g = tid - (CONSUMERS + LOADERS) * 32, chunk = g & 7, row0 = g >> 3;      // rows row0, row0 + 8, ...
+    const uint32_t mine = row0 * 128 + static_cast<uint32_t>((chunk ^ row0) << 4);      // row & 7 == row0
     Run r;
     RingPos at;
     bool ok = true;
@@ -305,16 +314,15 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
         src[i] = UP ? static_cast<const uint8_t*>(a.X) + static_cast<int64_t>(token[j]) * a.sxm * 2
                     : p.hidden + static_cast<int64_t>(plan->slots[j]) * a.F * 2;
       }
-      for (int c = r.c0; c < r.c1; ++c, at.next(p.stages)) {
-        const int s = at.stage;
+      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
+        const int s = at.stage, steps = min(r.nb, r.b1 - b);
         if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 23)) { ok = false; break; }
-        const uint32_t dst = ring0 + s * p.stage_bytes + p.x_offset + row0 * 128 + sw;
-        const int k0 = c * p.KC + chunk * 8, k_end = min((c + 1) * p.KC, (p.K + 63) & ~63);
-        for (int kk = k0, b = 0; kk < k_end; kk += 64, ++b)
+        uint32_t dst = ring0 + s * p.stage_bytes + p.x_offset + mine;
+        int kk = b * BLOCK_K + chunk * 8;
+        for (int st = 0; st < steps; ++st, kk += BLOCK_K, dst += p.NT * 128)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (row0 + 8 * i < n)
-              cp_async16(dst + (b * p.NT + 8 * i) * 128, src[i] + (kk < p.K ? kk * 2 : 0), kk < p.K ? 16 : 0);
+            if (row0 + 8 * i < n) cp_async16(dst + i * 1024, src[i] + (kk < p.K ? kk * 2 : 0), kk < p.K ? 16 : 0);
         cp_async_arrive(full_bar(s));
       }
     }
@@ -328,51 +336,27 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   bool ok = true;
   RingPos at;
   Run r;
-  const int my_box = KMAJOR ? 0 : warp >> 2;
-  // ldmatrix addresses of this lane inside a stage; the loop over K only adds multiples of a block of 64
-  uint32_t a_lane[2], x_lane[2], x_lane4[2];       // K-major: the two 16-wide steps of the warp's half of a block of 64
+  // ldmatrix addresses of this lane inside a box and inside a step of the slots' rows; 16 of K further: see `step`
+  uint32_t w_lane, x1_lane, x4_lane;
   {
-    const int row = (lane & 7) + ((lane >> 3) & 1) * 8, xrow4 = (lane & 7) + (lane >> 4) * 8;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int step = KMAJOR ? (warp & 1) * 2 + i : warp & 3;
-      a_lane[i] = KMAJOR ? row * 128 + (((step * 2 + (lane >> 4)) ^ (row & 7)) << 4) : 0;
-      x_lane[i] = (lane & 7) * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4);
-      x_lane4[i] = xrow4 * 128 + (((step * 2 + ((lane >> 3) & 1)) ^ (xrow4 & 7)) << 4);
-    }
-    if (!KMAJOR) {
-      const int krow = (warp & 3) * 16 + (lane & 7) + (lane >> 4) * 8, chunk = (lane >> 3) & 1;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)                  // N-major: the two 16-column halves of the warp's box
-        a_lane[i] = my_box * p.KC * BOX * 2 + krow * (BOX * 2) + (((chunk + 2 * i) ^ ((krow >> 1) & 3)) << 4);
-    }
+    const int row = (lane & 7) + ((lane >> 3) & 1) * 8, xrow = (lane & 7) + (lane >> 4) * 8;
+    const int krow = (lane & 7) + (lane >> 4) * 8;
+    if (KMAJOR) w_lane = row * 128 + (((lane >> 4) ^ (row & 7)) << 4);
+    else if (halves) w_lane = krow * 32 + ((((lane >> 3) & 1) ^ ((krow >> 2) & 1)) << 4);      // 32-byte rows
+    else w_lane = krow * 64 + ((((lane >> 3) & 1) ^ ((krow >> 1) & 3)) << 4);
+    x1_lane = (lane & 7) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+    x4_lane = xrow * 128 + ((((lane >> 3) & 1) ^ (xrow & 7)) << 4);
   }
-  const int x_block = p.NT * 128;
-  auto total_of = [&](int i, int row) {       // sum over the warps that share this row
-    float v = 0.f;
-    if (KMAJOR) {
-#pragma unroll
-      for (int w = 0; w < 8; ++w) v += red[(w * p.NT + i) * RED_PITCH + row];
-    } else {
-#pragma unroll
-      for (int w = 0; w < 4; ++w) v += red[(((row >> 5) * 4 + w) * p.NT + i) * RED_PITCH + (row & 31)];
-    }
-    return v;
-  };
+  const int x_block = p.NT * 128, w_step = halves ? 512 : 1024;
   while (walk.next(r)) {
     const int n = plan->job_count[r.job], beg = plan->job_begin[r.job], e = plan->job_expert[r.job];
     const int groups = (n + 7) >> 3;
-    bool use0, use1;                          // the warp's two 16-row halves that hold anything
-    if (KMAJOR) {
-      use0 = true;
-      use1 = pairs || r.count > 16;
-    } else {
-      const int cols = UP ? (halves ? 2 * BOX : r.count * BOX) : r.count;
-      use0 = cols > my_box * BOX;
-      use1 = cols > my_box * BOX + 16;
-    }
+    // the warp's weight rows: up, tile `warp` of the round; down, the one tile
+    const int v0 = UP ? r.p0 + warp * walk.per_tile : r.p0;
+    const int count = UP ? min(walk.per_tile, r.count - warp * walk.per_tile) : r.count;
+    const bool use0 = count > 0, use1 = pairs ? (woven && !KMAJOR ? count > 8 : use0) : count > 16;
     if (!UP && r.first)
-      for (int i = tid; i < a.T * OP; i += CONSUMERS * 32) oacc[i] = 0.f;
+      for (int i = lane; i < a.T * pitch; i += 32) sums[warp * a.T * pitch + i] = 0.f;
     float acc[2][4][4];
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -382,48 +366,48 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
         for (int q = 0; q < 4; ++q) acc[m][g][q] = 0.f;
     auto stream = [&](auto G_) {
       constexpr int G = decltype(G_)::value;           // groups of 8 slots, rounded up to 1, 2 or 4
-      for (int c = r.c0; c < r.c1; ++c, at.next(p.stages)) {
+      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
         const int s = at.stage;
         if (ok) ok = mbar_wait_warp(full_bar(s), at.phase, abort_flag, p.status, 22);
         if (ok && use0) {
-          const int blocks = (min(p.KC, p.K - c * p.KC) + 63) >> 6;
-          const uint32_t wst = ring0 + s * p.stage_bytes, xst = wst + p.x_offset;
-          auto step = [&](uint32_t w0, uint32_t w1, uint32_t x1, uint32_t x4) {
-            uint32_t a0[4], a1[4] = {0, 0, 0, 0}, b[G][2];
+          const int steps = min(r.nb, r.b1 - b);
+          const uint32_t wst = ring0 + s * p.stage_bytes + (UP ? warp * r.nb * p.box_bytes : 0), xst = ring0 + s * p.stage_bytes + p.x_offset;
+          auto step = [&](uint32_t w, uint32_t x, int i) {       // the i-th 16 of K of a box
+            uint32_t a0[4], a1[4] = {0, 0, 0, 0}, bx[G][2];
             if (KMAJOR) {
-              ldsm4(a0, w0);
-              if (use1) ldsm4(a1, w1);
+              ldsm4(a0, w + (w_lane ^ (i << 5)));
+              if (use1) ldsm4(a1, w + (w_lane ^ (i << 5)) + 16 * 128);
             } else {
-              ldsm4_trans(a0, w0);
-              if (use1) ldsm4_trans(a1, w1);
+              ldsm4_trans(a0, w + w_lane + i * w_step);
+              if (use1) ldsm4_trans(a1, w + (halves ? w_lane + 2048 : w_lane ^ 32) + i * w_step);
             }
             if (G == 1) {
-              ldsm2(b[0][0], b[0][1], x1);
+              ldsm2(bx[0][0], bx[0][1], x + (x1_lane ^ (i << 5)));
             } else {
 #pragma unroll
               for (int g = 0; g < G; g += 2) {
                 uint32_t t[4];
-                ldsm4(t, x4 + g * 8 * 128);
-                b[g][0] = t[0]; b[g][1] = t[1]; b[g + 1][0] = t[2]; b[g + 1][1] = t[3];
+                ldsm4(t, x + (x4_lane ^ (i << 5)) + g * 1024);
+                bx[g][0] = t[0]; bx[g][1] = t[1]; bx[g + 1][0] = t[2]; bx[g + 1][1] = t[3];
               }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              Mma<T>::run(acc[0][g], a0, b[g][0], b[g][1]);
-              if (use1) Mma<T>::run(acc[1][g], a1, b[g][0], b[g][1]);
+              Mma<T>::run(acc[0][g], a0, bx[g][0], bx[g][1]);
+              if (use1) Mma<T>::run(acc[1][g], a1, bx[g][0], bx[g][1]);
             }
           };
-          if (KMAJOR) {
-            for (int b = warp >> 1; b < blocks; b += 4) {
-              const uint32_t w = wst + b * p.box_bytes, x = xst + b * x_block;
+          if (UP) {
+            for (int i = 0; i < steps; ++i) {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) step(w + a_lane[i], w + a_lane[i] + 16 * 128, x + x_lane[i], x + x_lane4[i]);
+              for (int q = 0; q < 4; ++q) step(wst + i * p.box_bytes, xst + i * x_block, q);
             }
           } else {
-#pragma unroll 2
-            for (int b = 0; b < blocks; ++b) {
-              const uint32_t w = wst + b * (64 * BOX * 2), x = xst + b * x_block;
-              step(w + a_lane[0], w + a_lane[1], x + x_lane[0], x + x_lane4[0]);
+            // half a box per warp and turn
+            for (int i = warp >> 1; i < steps; i += CONSUMERS / 2) {
+              const uint32_t w = wst + i * p.box_bytes, x = xst + i * x_block;
+              step(w, x, (warp & 1) * 2);
+              step(w, x, (warp & 1) * 2 + 1);
             }
           }
         }
@@ -434,95 +418,113 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     if (groups == 1) stream(std::integral_constant<int, 1>{});
     else if (groups == 2) stream(std::integral_constant<int, 2>{});
     else stream(std::integral_constant<int, 4>{});
-    // ---- join the warps' parts of K
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-      if (m == 0 ? use0 : use1)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (g < groups) {
-            float* out = red + (warp * p.NT + g * 8 + (lane & 3) * 2) * RED_PITCH + m * 16 + (lane >> 2);
-            out[0] = acc[m][g][0];
-            out[RED_PITCH] = acc[m][g][1];
-            out[8] = acc[m][g][2];
-            out[RED_PITCH + 8] = acc[m][g][3];
-          }
-    consumers_sync();
+
     if (UP) {
-      // hidden values of this tile: first value, how many, and where their columns are
-      int v0, count;
-      if (KMAJOR) { v0 = r.p0; count = r.count; }
-      else if (halves) { v0 = r.p0 * BOX; count = min(BOX, a.F - v0); }
-      else if (pairs) { v0 = r.p0 * (BOX / 2); count = min(r.count * (BOX / 2), a.F - v0); }
-      else { v0 = r.p0 * BOX; count = min(r.count * BOX, a.F - v0); }
-      const int second = KMAJOR ? 16 : BOX;
-      for (int idx = tid; idx < n * count; idx += CONSUMERS * 32) {
-        const int i = idx / count, v = idx - i * count, pv = v0 + v;
-        const bool woven = !KMAJOR && pairs && !halves;       // interleaved columns stand side by side in the boxes
-        float c0 = total_of(i, woven ? 2 * v : v);
-        float c1 = pairs ? total_of(i, woven ? 2 * v + 1 : second + v) : 0.f;
-        if (a.B1) {
-          const T* bias = static_cast<const T*>(a.B1) + e * a.sb1e;
-          c0 += to_f32<T>(bias[(pairs ? (halves ? pv : 2 * pv) : pv) * a.sb1n]);
-          if (pairs) c1 += to_f32<T>(bias[(halves ? a.F + pv : 2 * pv + 1) * a.sb1n]);
+      // accumulator q of group g: slot g*8 + 2*(lane & 3) + (q & 1), weight row (lane >> 2) + 8*(q >> 1) of each 16-row half
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (g >= groups || !use0) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
+          float c[2][2] = {{acc[0][g][q], acc[1][g][q]}, {0.f, 0.f}};       // (first, second column) of up to two values
+          int v[2] = {row, -1};
+          if (!pairs) {
+            c[1][0] = c[0][1];
+            v[1] = 16 + row;
+          } else if (woven && !KMAJOR) {      // columns side by side: the second one sits in the neighbouring row's lane
+            const float o0 = __shfl_xor_sync(0xffffffffu, c[0][0], 4), o1 = __shfl_xor_sync(0xffffffffu, c[0][1], 4);
+            c[1][0] = c[0][1]; c[1][1] = o1; c[0][1] = o0;
+            v[0] = (row & 1) ? -1 : row >> 1;
+            v[1] = (row & 1) ? -1 : 8 + (row >> 1);
+          }
+          if (i >= n) continue;
+          const int slot = plan->slots[beg + i];
+          const float gate = a.gates ? load_any(a.gates, token[beg + i] * a.sgt + (slot - token[beg + i] * a.k) * a.sgk, a.gates_dtype) : 1.f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (v[h] < 0 || v[h] >= count) continue;
+            const int pv = v0 + v[h];
+            float c0 = c[h][0], c1 = c[h][1];
+            if (a.B1) {
+              const T* bias = static_cast<const T*>(a.B1) + e * a.sb1e;
+              c0 += to_f32<T>(bias[(woven ? 2 * pv : pv) * a.sb1n]);
+              if (pairs) c1 += to_f32<T>(bias[(woven ? 2 * pv + 1 : a.F + pv) * a.sb1n]);
+            }
+            reinterpret_cast<T*>(p.hidden)[static_cast<int64_t>(slot) * a.F + pv] =
+                from_f32<T>(gate * hidden_fast(a.act_layout, a.act, a.alpha, a.limit, c0, c1));
+          }
         }
-        const int slot = plan->slots[beg + i];
-        float h = hidden_fast(a.act_layout, a.act, a.alpha, a.limit, c0, c1);
-        if (a.gates) h *= load_any(a.gates, (slot / a.k) * a.sgt + (slot % a.k) * a.sgk, a.gates_dtype);
-        reinterpret_cast<T*>(p.hidden)[static_cast<int64_t>(slot) * a.F + pv] = from_f32<T>(h);
       }
-      consumers_sync();
     } else {
-      // add the job's slots to their tokens; slots of one token (the same expert twice) stand together and go to one thread
-      const int row = tid % RT;
-      for (int i = tid / RT; i < n; i += CONSUMERS * 32 / RT) {
-        const int t = token[beg + i];
-        if (i > 0 && token[beg + i - 1] == t) continue;
-        if (row < r.count) {
-          float v = total_of(i, row);
-          for (int m = i + 1; m < n && token[beg + m] == t; ++m) v += total_of(m, row);
-          oacc[t * OP + row] += v;
+      // add the job's slots to this warp's token sums. Slots of one token (the same expert twice) stand together and may sit in
+      // neighbouring lanes: then the lanes take turns
+      float* own = sums + warp * a.T * pitch;
+      const bool twice = __any_sync(0xffffffffu, lane > 0 && lane < n && token[beg + min(lane, n - 1)] == token[beg + min(lane, n - 1) - (lane > 0)]);
+      for (int turn = 0; turn < (twice ? 4 : 1); ++turn) {
+        if (!twice || (lane & 3) == turn) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (g >= groups) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
+              if (i >= n) continue;
+              float* to = own + token[beg + i] * pitch + row;
+              if (row < count) to[0] += acc[0][g][q];
+              if (use1 && 16 + row < count) to[16] += acc[1][g][q];
+            }
+          }
         }
+        if (twice) __syncwarp();
       }
-      consumers_sync();
       if (r.last) {
+        consumers_sync();
         bool write = true;
+        auto total_of = [&](int t, int col) {
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < CONSUMERS; ++w) v += sums[(w * a.T + t) * pitch + col];
+          return v;
+        };
+        int64_t first = 0, stop = 0, tile_beg = 0, total = 1;
+        const int64_t g = gridDim.x;
+        auto begin_of = [&](int64_t b) { return total * b / g; };
+        bool split = false;
         if (!KMAJOR) {
-          // does this block hold the whole tile, or only a part of its pieces?
-          const int64_t g = gridDim.x, tile_beg = static_cast<int64_t>(r.tile) * walk.units, tile_end = tile_beg + walk.units;
-          const int64_t total = static_cast<int64_t>(walk.units) * ((a.d_out + 2 * BOX - 1) / (2 * BOX));
-          auto begin_of = [&](int64_t b) { return total * b / g; };
+          // does this block hold the whole tile, or only a part of its steps?
+          tile_beg = static_cast<int64_t>(r.tile) * walk.units;
+          const int64_t tile_end = tile_beg + walk.units;
+          total = static_cast<int64_t>(walk.units) * ((a.d_out + TILE - 1) / TILE);
           const int64_t mine0 = begin_of(blockIdx.x), mine1 = begin_of(blockIdx.x + 1);
-          if (mine0 > tile_beg || mine1 < tile_end) {
-            float* part = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (mine0 > tile_beg ? 0 : 1)) * a.T * RT;
-            for (int i = tid; i < a.T * RT; i += CONSUMERS * 32) part[i] = oacc[(i / RT) * OP + i % RT];
+          split = mine0 > tile_beg || mine1 < tile_end;
+          if (split) {
+            float* part = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (mine0 > tile_beg ? 0 : 1)) * a.T * TILE;
+            for (int i = tid; i < a.T * r.count; i += CONSUMERS * 32) part[(i / r.count) * TILE + i % r.count] = total_of(i / r.count, i % r.count);
             __threadfence();
             consumers_sync();
-            int64_t first = tile_beg * g / total, stop = first;
+            first = tile_beg * g / total;
             while (first > 0 && begin_of(first) > tile_beg) --first;
             while (begin_of(first + 1) <= tile_beg) ++first;
             int parts = 0;
             for (stop = first; stop < g && begin_of(stop) < tile_end; ++stop) parts += begin_of(stop + 1) > begin_of(stop);
             if (tid == 0) *joined = atomicAdd(p.counters + r.tile, 1) == parts - 1;
             consumers_sync();
-            write = *joined != 0;
-            if (write) {        // the last block of the tile adds the parts up, always in the same order
-              __threadfence();
-              for (int i = tid; i < a.T * RT; i += CONSUMERS * 32) {
-                float v = 0.f;
-                for (int64_t b = first; b < stop; ++b)
-                  if (begin_of(b + 1) > begin_of(b))
-                    v += __ldcg(p.partial + (b * 2 + (begin_of(b) > tile_beg ? 0 : 1)) * a.T * RT + i);
-                oacc[(i / RT) * OP + i % RT] = v;
-              }
-            }
-            consumers_sync();
+            write = *joined != 0;      // the last block of the tile adds the parts up, always in the same order
+            if (write) __threadfence();
           }
         }
         if (write)
           for (int idx = tid; idx < a.T * r.count; idx += CONSUMERS * 32) {
             const int t = idx / r.count, col = idx - t * r.count;
-            float v = oacc[t * OP + col];
+            float v = 0.f;
+            if (split) {
+              for (int64_t b = first; b < stop; ++b)
+                if (begin_of(b + 1) > begin_of(b))
+                  v += __ldcg(p.partial + ((b * 2 + (begin_of(b) > tile_beg ? 0 : 1)) * a.T + t) * TILE + col);
+            } else {
+              v = total_of(t, col);
+            }
             if (a.B2)
               for (int j = 0; j < a.k; ++j) {
                 const int64_t ex = a.ids[t * a.sit + j * a.sik];
@@ -545,10 +547,9 @@ constexpr size_t HIDDEN_ALIGN = 256;
 static size_t hidden_bytes(int64_t T, int k, int F) {
   return (static_cast<size_t>(T) * k * F * 2 + HIDDEN_ALIGN - 1) / HIDDEN_ALIGN * HIDDEN_ALIGN;
 }
-static int column_tiles(int d_out) { return cdiv(d_out, 2 * BOX); }
+static int column_tiles(int d_out) { return cdiv(d_out, TILE); }
 size_t stream_workspace_bytes(int64_t T, int k, int F, int d_out) {
-  return hidden_bytes(T, k, F) + static_cast<size_t>(column_tiles(d_out)) * 4 + 16 +
-         static_cast<size_t>(MAX_CTAS) * 2 * T * 2 * BOX * 4;
+  return hidden_bytes(T, k, F) + static_cast<size_t>(column_tiles(d_out)) * 4 + 16 + static_cast<size_t>(MAX_CTAS) * 2 * T * TILE * 4;
 }
 
 struct Order { bool k_major, n_major; };
@@ -557,62 +558,60 @@ static Order weight_order(const void* W, int64_t se, int64_t sk, int64_t sn, int
   return {sk == 1 && sn % 8 == 0 && sn >= K, sn == 1 && sk % 8 == 0 && sk >= N && N % 8 == 0};
 }
 
-// Pieces of K: multiples of 64, at most `most`, all but the last alike.
-static int piece_of(int K, int most) {
-  const int blocks = cdiv(K, 64), n = cdiv(blocks, most / 64);
-  return cdiv(blocks, n) * 64;
-}
-
-// K-major boxes: 64 of K x `rows` x `halves` (the two columns of a hidden value; 1 without a gate) of one expert.
-static bool encode_k_major(CUtensorMap* map, bool bf16, const void* W, int K, int rows_total, int64_t row_stride, int halves,
-                           int64_t half_stride, int E, int64_t se, int box_rows) {
-  const uint64_t dim[4] = {static_cast<uint64_t>(K), static_cast<uint64_t>(rows_total), static_cast<uint64_t>(halves),
-                           static_cast<uint64_t>(E)};
+// Boxes of one expert, 128-byte swizzle: 64 of K x `rows` x `halves` (the two columns of a hidden value; 1 without a gate).
+static bool encode_k_major(CUtensorMap* map, bool bf16, const void* W, int K, int values, int64_t value_stride, int halves,
+                           int64_t half_stride, int E, int64_t se, int rows) {
+  const uint64_t dim[4] = {static_cast<uint64_t>(K), static_cast<uint64_t>(values), static_cast<uint64_t>(halves), static_cast<uint64_t>(E)};
   // the stride of an axis of one element is never used, but has to be valid
-  const uint64_t stride[3] = {static_cast<uint64_t>(row_stride) * 2, static_cast<uint64_t>(halves > 1 ? half_stride : row_stride) * 2,
-                              static_cast<uint64_t>(E > 1 ? se : row_stride) * 2};
-  const uint32_t box[4] = {64, static_cast<uint32_t>(box_rows), static_cast<uint32_t>(halves), 1};
+  const uint64_t stride[3] = {static_cast<uint64_t>(value_stride) * 2, static_cast<uint64_t>(halves > 1 ? half_stride : value_stride) * 2,
+                              static_cast<uint64_t>(E > 1 ? se : value_stride) * 2};
+  const uint32_t box[4] = {BLOCK_K, static_cast<uint32_t>(rows), static_cast<uint32_t>(halves), 1};
   return encode_tensor_map(map, bf16, W, 4, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-static bool encode_n_major(CUtensorMap* map, bool bf16, const void* W, int N, int K, int64_t row_stride, int E, int64_t se, int box_k) {
-  const uint64_t dim[3] = {static_cast<uint64_t>(N), static_cast<uint64_t>(K), static_cast<uint64_t>(E)};
-  const uint64_t stride[2] = {static_cast<uint64_t>(row_stride) * 2, static_cast<uint64_t>(E > 1 ? se : row_stride) * 2};
-  const uint32_t box[3] = {BOX, static_cast<uint32_t>(box_k), 1};
-  return encode_tensor_map(map, bf16, W, 3, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_64B);
+// Boxes of one expert: 32 columns x 64 of K, 64-byte swizzle; where the two columns of a hidden value are a half apart, 16 columns of one
+// half x 64 of K, 32-byte swizzle.
+static bool encode_n_major(CUtensorMap* map, bool bf16, const void* W, int N, int K, int64_t row_stride, int halves, int E, int64_t se) {
+  const uint64_t dim[4] = {static_cast<uint64_t>(N / halves), static_cast<uint64_t>(halves), static_cast<uint64_t>(K), static_cast<uint64_t>(E)};
+  const uint64_t stride[3] = {static_cast<uint64_t>(halves > 1 ? N / 2 : row_stride) * 2, static_cast<uint64_t>(row_stride) * 2,
+                              static_cast<uint64_t>(E > 1 ? se : row_stride) * 2};
+  const uint32_t box[4] = {static_cast<uint32_t>(TILE / halves), 1, BLOCK_K, 1};
+  return encode_tensor_map(map, bf16, W, 4, dim, stride, box, halves > 1 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
-// rows of a K-major box: the hidden values of a tile, or the output columns of a block (at most 32)
-static int down_rows(int d_out, int grid) { return cdiv(d_out, grid) < 32 ? cdiv(d_out, grid) : 32; }
+// rows of a K-major box of the down-projection: the output columns of a block, at most a tile
+static int down_rows(int d_out, int grid) { return cdiv(d_out, grid) < TILE ? cdiv(d_out, grid) : TILE; }
 
 template <typename T, bool UP, bool KMAJOR>
 static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& di, int grid) {
   const Args& a = p.a;
+  p.rows = UP ? 0 : (KMAJOR ? down_rows(a.d_out, grid) : TILE);
   // shared memory that is not the ring
-  const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 + 8 * p.NT * RED_PITCH * 4 +
-                    (UP ? 0 : a.T * ((KMAJOR ? 32 : 2 * BOX) + 1) * 4) + 1024 + 64;
+  const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 +
+                    (UP ? 0 : CONSUMERS * a.T * (p.rows + 1) * 4) + 1024 + 64;
   const int budget = (di.max_smem_optin < 232448 ? di.max_smem_optin : 232448) - fixed;
-  if (KMAJOR) {
-    const int rows = UP ? 32 : down_rows(a.d_out, grid);
-    p.load_bytes = rows * 128;
-    p.box_bytes = cdiv(rows, 8) * 1024;                    // boxes start on the swizzle's period
-    // Stages of up to 32 KB of weights where the ring then still holds four, else 16 KB: enough of them that the stream never stops,
-    // few enough that a stage is worth its waits (16 KB stages with one slot per job were bound by the warps' loop overhead).
-    const int block = p.box_bytes + p.NT * 128;            // bytes of 64 of K: weights and slots
-    p.KC = piece_of(p.K, 64 * (32768 / p.box_bytes));
-    if ((budget - 2048) / (p.KC / 64 * block) < 4) p.KC = piece_of(p.K, 64 * (16384 / p.box_bytes));
-    p.x_offset = p.KC / 64 * p.box_bytes;
+  const int rows = UP || !KMAJOR ? TILE : p.rows;
+  p.load_bytes = rows * BLOCK_K * 2;
+  p.box_bytes = cdiv(rows, 8) * 1024;                      // boxes start on the swizzle's period
+  p.blocks = cdiv(p.K, BLOCK_K);
+  const int slack = 2048;      // ldmatrix reads whole 16-row blocks: past a box of fewer rows (never used, but inside the ring)
+  if (UP) {
+    // a stage is up to 8 boxes (32 KB): one step of K of 8 tiles, or more steps of fewer tiles
+    p.slots = CONSUMERS;
+    p.x_slots = 64 / p.NT;                                 // at most 8 KB of the slots' rows
+    p.x_offset = p.slots * p.box_bytes;
+    p.stage_bytes = p.x_offset + p.x_slots * p.NT * 128;
   } else {
-    p.load_bytes = p.box_bytes = 0;
-    p.KC = piece_of(p.K, 256);                             // as the tensor map's boxes
-    p.x_offset = 2 * p.KC * BOX * 2;
+    // steps of K: up to 32 KB of weights where the ring then still holds four stages, else half of that
+    int most = 32768 / p.box_bytes;
+    if ((budget - slack) / (most * (p.box_bytes + p.NT * 128)) < 4) most /= 2;
+    p.slots = p.x_slots = cdiv(p.blocks, cdiv(p.blocks, most));
+    p.x_offset = p.slots * p.box_bytes;
+    p.stage_bytes = p.x_offset + p.slots * p.NT * 128;
   }
-  p.n_chunks = cdiv(p.K, p.KC);
-  p.stage_bytes = p.x_offset + p.KC / 64 * p.NT * 128;
-  p.stages = (budget - (KMAJOR ? 2048 : 0)) / p.stage_bytes;
+  p.stages = (budget - slack) / p.stage_bytes;
   if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
   if (p.stages < 2) return SMOE_ERR_UNSUPPORTED;
-  // ldmatrix reads whole 16-row blocks: up to 8 rows past a box of fewer rows (never used, but inside the ring)
-  p.ring_bytes = p.stages * p.stage_bytes + (KMAJOR ? 2048 : 0);
+  p.ring_bytes = p.stages * p.stage_bytes + slack;
   const int scratch = (plan_scratch_bytes(a.E) + 15) / 16 * 16;      // the plan sorts in the ring before the first copy
   if (scratch > budget) return SMOE_ERR_UNSUPPORTED;
   if (p.ring_bytes < scratch) p.ring_bytes = scratch;
@@ -661,10 +660,10 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
   memset(&m2, 0, sizeof(m2));
   const bool pairs = a.act_layout != LAYOUT_PLAIN, woven = a.act_layout == LAYOUT_GPT_OSS;
   const bool ok1 = o1.k_major ? encode_k_major(&m1, bf16, a.W1, a.d, a.F, woven ? 2 * a.s1n : a.s1n, pairs ? 2 : 1,
-                                               woven ? a.s1n : a.s1n * a.F, a.E, a.s1e, pairs ? 16 : 32)
-                              : encode_n_major(&m1, bf16, a.W1, n_up_cols, a.d, a.s1k, a.E, a.s1e, piece_of(a.d, 256));
+                                               woven ? a.s1n : a.s1n * a.F, a.E, a.s1e, pairs ? TILE / 2 : TILE)
+                              : encode_n_major(&m1, bf16, a.W1, n_up_cols, a.d, a.s1k, pairs && !woven ? 2 : 1, a.E, a.s1e);
   const bool ok2 = o2.k_major ? encode_k_major(&m2, bf16, a.W2, a.F, a.d_out, a.s2n, 1, 0, a.E, a.s2e, down_rows(a.d_out, grid))
-                              : encode_n_major(&m2, bf16, a.W2, a.d_out, a.F, a.s2k, a.E, a.s2e, piece_of(a.F, 256));
+                              : encode_n_major(&m2, bf16, a.W2, a.d_out, a.F, a.s2k, 1, a.E, a.s2e);
   if (!ok1 || !ok2) return SMOE_ERR_UNSUPPORTED;
   p.K = a.d;
   if (int rc = o1.k_major ? launch_one<T, true, true>(p, m1, di, grid) : launch_one<T, true, false>(p, m1, di, grid)) return rc;

@@ -5,6 +5,8 @@
 // Bound by the weights of the experts that occur, read once per job of up to 8 slots. Weights with contiguous inputs: a warp
 // owns 4 weight rows and its lanes stride over K (4 x 8 partial sums per lane, one transposing reduction at the end).
 // Any other strides: a lane owns a weight column, the warps of a block split K.
+#include <cooperative_groups.h>
+
 #include "act_math.cuh"
 #include "few_token.cuh"
 
@@ -309,9 +311,11 @@ int launch_simt(const Args& a) {
 }
 
 // ---- router --------------------------------------------------------------------------------------------
-// One block per token: logits z_e = <x, Wr[e]> + br[e] in fp32 (a warp per expert), then the k largest and their gates by the first
-// warp. Order: larger logit first, equal logits by lower expert id, a NaN counts as the largest.
+// A cluster of up to 8 blocks per token: logits z_e = <x, Wr[e]> + br[e] in fp32, a warp per expert, gathered in the first block's shared
+// memory; its first warp picks the k largest and makes the gates. Order: larger logit first, equal logits by lower expert
+// id, a NaN counts as the largest. Bound by latency: one block per token read the router's 0.5 MB (128 experts of 2048) in 25 us.
 constexpr int ROUTE_THREADS = 512;
+constexpr int ROUTE_CLUSTER = 8;
 
 struct RouteParams {
   const void* X; int64_t sxm;
@@ -333,11 +337,17 @@ template <typename T, int V>
 __global__ void __launch_bounds__(ROUTE_THREADS)
 ft_route_kernel(const RouteParams p) {
   __shared__ float z[MAX_E];
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the layer's kernels may take their places
+  cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+  const int parts = static_cast<int>(cluster.num_blocks()), part = static_cast<int>(cluster.block_rank());
+  const int t = blockIdx.x / parts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float* z0 = cluster.map_shared_rank(z, 0);
   const T* x = static_cast<const T*>(p.X) + static_cast<int64_t>(t) * p.sxm;
-  for (int e = warp; e < p.E; e += ROUTE_THREADS / 32) {
+  cluster.sync();            // the first block runs before its memory is written
+  for (int e = part * (ROUTE_THREADS / 32) + warp; e < p.E; e += parts * (ROUTE_THREADS / 32)) {
     const T* w = static_cast<const T*>(p.Wr) + static_cast<int64_t>(e) * p.swm;
     float acc = 0.f;
+#pragma unroll 4
     for (int kk = lane * V; kk < p.d; kk += 32 * V) {
       float a[V], b[V];
       load_v<T, V>(x + kk, a);
@@ -347,10 +357,10 @@ ft_route_kernel(const RouteParams p) {
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0) z[e] = acc + (p.br ? to_f32<T>(static_cast<const T*>(p.br)[e * p.sbn]) : 0.f);
+    if (lane == 0) z0[e] = acc + (p.br ? to_f32<T>(static_cast<const T*>(p.br)[e * p.sbn]) : 0.f);
   }
-  __syncthreads();
-  if (warp != 0) return;
+  cluster.sync();
+  if (part != 0 || warp != 0) return;
   float total = 0.f, top = 0.f, mine = 0.f;
   int my_id = 0;
   if (p.mode == 0 && !p.renorm) {          // softmax over all experts
@@ -397,9 +407,19 @@ template <typename T>
 static int launch_route(const RouteParams& p, int T_, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   const bool vec = p.d % V == 0 && p.sxm % V == 0 && p.swm % V == 0 && al16(p.X) && al16(p.Wr);
-  if (vec) ft_route_kernel<T, V><<<T_, ROUTE_THREADS, 0, stream>>>(p);
-  else ft_route_kernel<T, 1><<<T_, ROUTE_THREADS, 0, stream>>>(p);
-  SMOE_LAUNCH_CHECK();
+  int parts = 1;
+  while (parts < ROUTE_CLUSTER && parts * (ROUTE_THREADS / 32) < p.E) parts *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(T_ * parts));
+  cfg.blockDim = dim3(ROUTE_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {static_cast<unsigned>(parts), 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (vec) SMOE_CUDA(cudaLaunchKernelEx(&cfg, ft_route_kernel<T, V>, p));
+  else SMOE_CUDA(cudaLaunchKernelEx(&cfg, ft_route_kernel<T, 1>, p));
   return SMOE_OK;
 }
 
@@ -420,7 +440,7 @@ extern "C" int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm,
                                     const void* br, int64_t stride_bn, int32_t E, int32_t d, int32_t k, int32_t mode,
                                     int32_t renormalize, int64_t* expert_idxs, float* gates, int32_t dtype, void* stream) {
   SMOE_CHECK_ARG(dtype == SMOE_F32 || dtype == SMOE_BF16 || dtype == SMOE_F16, "few_token_route: unknown dtype %d", dtype);
-  SMOE_CHECK_ARG(T >= 0 && T < (int64_t(1) << 31), "few_token_route: T=%lld out of range", (long long)T);
+  SMOE_CHECK_ARG(T >= 0 && T < (int64_t(1) << 27), "few_token_route: T=%lld out of range", (long long)T);
   SMOE_CHECK_ARG(E >= 1 && E <= ft::MAX_E && d >= 0, "few_token_route: E=%d out of range [1, %d] or d=%d negative", E, ft::MAX_E, d);
   SMOE_CHECK_ARG(k >= 1 && k <= E && k <= 32, "few_token_route: k=%d out of range [1, min(E, 32)]", k);
   SMOE_CHECK_ARG(mode == 0 || mode == 1, "few_token_route: unknown mode %d", mode);
