@@ -12,13 +12,16 @@
 //   up    A round is up to 8 tiles of one job, a tile 32 weight rows: 16 hidden values with their two columns, or 32 without a gate. Each
 //         warp owns a tile over the whole of K and makes its hidden values in registers: no exchange between warps, no barrier; the
 //         slots' rows are fetched once per round.
-//   down  The block's output columns are one tile. The warps split every piece of K and add each job's result to
-//         token sums of their own in shared memory; the eight are joined, in order, once at the end.
+//   down  The block's output columns are one tile. Pairs of warps take the stages in turn, so that four jobs are under way at once, and
+//         add their part of a job to token sums of their own in shared memory, joined in order once at the end. The two warps of a pair
+//         hold 16 columns each, or half of K each where the tile has no more than 16.
 //
 // A first version gave the warps parts of K in both kernels and joined them after every tile and job: with many small jobs the
 // joins cost as much as the stream (24 tokens on 128 experts of 9.4 MB: 126 + 127 us against 97 + 49 of reading).
-// Issuing is what limits such a stream, not depth: one thread issues a box every 70-150 ns, so one thread moved 3.7 TB/s of 4 KB boxes
-// (2.5 of 1.8 KB ones) with 25 to 190 KB in flight alike, two 5.4, four 5.4-5.7 (3.7-6.5). One bulk copy per weight row: 1.2-3 TB/s.
+// Issuing is what limits such a stream, not depth: one thread issues a box every 70-150 ns and spends 0.25 us more on a stage, so one
+// thread moved 3.7 TB/s of 4 KB boxes (2.5 of 1.8 KB ones) with 25 to 190 KB in flight alike, two 5.4, four 5.4-5.7 (3.7-6.5), in stages of
+// 32 KB; stages of 8 KB 2.2-4.2. Hence few, large stages, and as many steps of K in one as the job's slots leave room for.
+// One bulk copy per weight row: 1.2-3 TB/s.
 //
 // Weights with contiguous inputs ("K-major", nn.Linear storage) are read through ldmatrix and may start at any row, so that a range may
 // begin anywhere (rows that two blocks load come from L2); weights with contiguous outputs ("N-major") through the transposing
@@ -46,8 +49,12 @@ using namespace ptx;
 
 constexpr int CONSUMERS = 8;                       // warps that multiply
 constexpr int LOADERS = 4;                         // warps whose first thread loads weights, each every fourth box of a stage
-constexpr int GATHERERS = 2;                       // warps that fetch the slots' rows
+constexpr int GATHERERS = 4;                       // warps that fetch the slots' rows: two pairs that take the stages in turn
+constexpr int GATHER_TURNS = 2;
+constexpr int GATHER_THREADS = GATHERERS * 32 / GATHER_TURNS;
+constexpr int DOWN_TURNS = 4;                      // down: pairs of multiplying warps that take the stages in turn
 constexpr int THREADS = (CONSUMERS + LOADERS + GATHERERS) * 32;
+// The number of stages is a multiple of the turns: every stage then always belongs to the same warps, which wait for each of its passes.
 constexpr int MAX_STAGES = 16;
 constexpr int TILE = 32;                           // weight rows (output columns) of a tile
 constexpr int BLOCK_K = 64;                        // K of a box: one 128-byte line of 16-bit values
@@ -63,9 +70,8 @@ struct StreamParams {
   int NT;                     // slots of a job
   int K, blocks;              // K and its boxes
   int box_bytes, load_bytes;  // bytes a box takes in the ring, and bytes it loads
-  int slots;                  // boxes of a stage (up: at most one per warp and step of K; down: steps of K)
-  int x_slots;                // steps of K of the slots' rows a stage can hold
-  int stages, stage_bytes, x_offset, ring_bytes;
+  int steps_of[4];            // steps of K of a stage for a job of 1-8, 9-16, 17-24, 25-32 slots (up: with one tile)
+  int stages, stage_bytes, ring_bytes;
   int rows;                   // down: rows of a tile's token sums (the tile's columns)
 };
 
@@ -122,20 +128,18 @@ struct RingPos {
 // ---- the list of runs of a block --------------------------------------------------------------------------
 // A run is a stretch of K of one job: up, a round of `tiles` tiles over the whole of K, `nb` steps of K per stage; down, (part
 // of) the K of the block's tile. The runs of a tile follow each other; `last` closes the tile (for this block).
-struct Run { int job, b0, b1, nb, p0, count, tiles, tile; bool first, last; };
+struct Run { int job, b0, b1, nb, p0, count, tiles, tile, groups, x_offset; bool first, last; };
 
 template <bool UP, bool KMAJOR>
 struct Walker {
-  int lo, hi, units, jobs, blocks, width, per_tile, job, slots, x_slots;
+  int lo, hi, units, jobs, blocks, width, per_tile, job, tile, step;
 
   // up, K-major: [lo, hi) is this block's part of all jobs' hidden values; N-major: of all jobs' tiles (boxes start on a multiple).
-  // down, K-major: [lo, hi) are this block's output columns; N-major: its part of the flat list of steps of K.
+  // down, K-major: [lo, hi) are this block's output columns; N-major: its part of the flat list of steps of K, (tile, job, step).
   __device__ void init(const StreamParams& p, int n_jobs) {
     jobs = n_jobs;
     blocks = p.blocks;
-    slots = p.slots;
-    x_slots = p.x_slots;
-    job = 0;
+    job = -1;
     const int64_t b = blockIdx.x, g = gridDim.x;
     int64_t total;
     if (UP) {
@@ -155,7 +159,7 @@ struct Walker {
     if (lo >= hi) return false;
     r.b0 = 0;
     r.b1 = blocks;
-    r.first = r.last = true;
+    r.tiles = 1;
     if (UP) {
       r.job = lo / units;
       const int in = lo - r.job * units;
@@ -170,34 +174,46 @@ struct Walker {
         r.p0 = in * per_tile;
         r.count = min(r.tiles * per_tile, width - r.p0);
       }
-      r.nb = min(x_slots, slots / r.tiles);
-      return true;
-    }
-    r.tiles = 1;
-    r.nb = slots;
-    if (KMAJOR) {
+    } else if (KMAJOR) {
+      r.first = ++job == 0;
       r.job = job;
       r.p0 = lo;
       r.count = min(TILE, hi - lo);
-      r.first = job == 0;
-      r.last = ++job == jobs;
-      if (r.last) { job = 0; lo += r.count; }
-      return true;
+      r.last = job + 1 == jobs;
+      if (r.last) { job = -1; lo += r.count; }
+    } else {
+      if (job < 0) {                       // the block's first run
+        tile = lo / units;
+        step = lo - tile * units;
+        job = step / blocks;
+        step -= job * blocks;
+        r.first = true;
+      } else {
+        step = 0;
+        if (++job == jobs) { job = 0; ++tile; }
+        r.first = job == 0;
+      }
+      r.tile = tile;
+      r.job = job;
+      r.b0 = step;
+      r.b1 = min(blocks, step + (hi - lo));
+      r.p0 = tile * TILE;
+      r.count = min(TILE, width - r.p0);
+      lo += r.b1 - r.b0;
+      r.last = lo >= hi || job + 1 == jobs;
     }
-    r.tile = lo / units;
-    const int in = lo - r.tile * units;
-    r.job = in / blocks;
-    r.b0 = in - r.job * blocks;
-    r.b1 = min(blocks, r.b0 + (hi - lo));
-    r.p0 = r.tile * TILE;
-    r.count = min(TILE, width - r.p0);
-    r.first = job == 0 || in == 0;     // `job` only marks "not the first run of the block" here
-    job = 1;
-    lo += r.b1 - r.b0;
-    r.last = lo >= hi || lo % units == 0;
     return true;
   }
 };
+
+// Steps of K in a stage of this run, and where its slots' rows start (after the weights; `groups` x 8 rows of 128 bytes per step).
+template <bool UP>
+__device__ __forceinline__ void shape_of(const StreamParams& p, Run& r, int n) {
+  r.groups = (n + 7) >> 3;
+  r.nb = p.steps_of[r.groups - 1];
+  if (UP && r.tiles > 1) r.nb = min(r.nb, r.tiles == 2 ? 4 : (r.tiles <= 4 ? 2 : 1));
+  r.x_offset = r.tiles * r.nb * p.box_bytes;
+}
 
 // hidden value from the up-projection's one or two columns (act_math.cuh has the layouts)
 __device__ __forceinline__ float hidden_fast(int layout, int act, float alpha, float limit, float c0, float c1) {
@@ -224,7 +240,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   uint64_t* bars = reinterpret_cast<uint64_t*>(token + MAX_R);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * MAX_STAGES);
   int* joined = reinterpret_cast<int*>(bars + 2 * MAX_STAGES) + 1;
-  float* sums = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // down: [warp][T][rows + 1]
+  float* sums = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // down: [warp][T][rows + 1]; up: the listed slots' gates
   const int pitch = p.rows + 1;
   const Args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -234,8 +250,8 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 
   if (tid == 0) {
     for (int s = 0; s < p.stages; ++s) {
-      mbar_init(full_bar(s), LOADERS + GATHERERS * 32);      // the weights (expect_tx) and the gatherers' threads
-      mbar_init(empty_bar(s), CONSUMERS);
+      mbar_init(full_bar(s), LOADERS + GATHER_THREADS);      // the weights (expect_tx) and the gatherers' threads
+      mbar_init(empty_bar(s), UP ? CONSUMERS : CONSUMERS / DOWN_TURNS);
     }
     *abort_flag = 0;
     fence_mbar_init();
@@ -250,7 +266,11 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   // ids are older than the up-projection, so the down-projection plans before it waits
   make_plan(plan, ring, a.ids, a.sit, a.sik, a.T, a.k, a.E, p.NT);
   const int listed = plan->jobs ? plan->job_begin[plan->jobs - 1] + plan->job_count[plan->jobs - 1] : 0;
-  for (int i = tid; i < listed; i += THREADS) token[i] = static_cast<uint8_t>(plan->slots[i] / a.k);
+  for (int i = tid; i < listed; i += THREADS) {
+    const int slot = plan->slots[i], t = slot / a.k;
+    token[i] = static_cast<uint8_t>(t);
+    if (UP) sums[i] = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
+  }
   fence_proxy_async_smem();            // the plan's scratch in the ring was written with ordinary stores
   __syncthreads();
 
@@ -277,20 +297,22 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     bool ok = true;
     while (walk.next(r) && ok) {
       const int e = plan->job_expert[r.job];
+      shape_of<UP>(p, r, plan->job_count[r.job]);
       for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
-        const int s = at.stage, steps = min(r.nb, r.b1 - b), total = r.tiles * steps;
+        const int s = at.stage, steps = min(r.nb, r.b1 - b);
         if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
-        const uint32_t dst = ring0 + s * p.stage_bytes;
-        mbar_arrive_expect_tx(full_bar(s), (total - mine + LOADERS - 1) / LOADERS * p.load_bytes);
-        for (int q = mine; q < total; q += LOADERS) {
-          const int t = UP ? q / steps : 0, i = q - t * steps;
-          const uint32_t to = dst + (t * r.nb + i) * p.box_bytes;
-          const int kk = (b + i) * BLOCK_K, v = r.p0 + t * walk.per_tile;
-          // K-major: (K, value, column of the value, expert). N-major: (column, half, K, expert).
-          if (KMAJOR) tma_load_4d(to, &tmap, full_bar(s), kk, UP ? v : r.p0, 0, e);
-          else tma_load_4d(to, &tmap, full_bar(s), UP ? (woven ? 2 * v : v) : r.p0, 0, kk, e);
-          if (halves) tma_load_4d(to + 2048, &tmap, full_bar(s), v, 1, kk, e);
-        }
+        mbar_arrive_expect_tx(full_bar(s), ((UP ? r.tiles * steps : steps) - mine + LOADERS - 1) / LOADERS * p.load_bytes);
+        uint32_t to = ring0 + s * p.stage_bytes;
+        int v = r.p0, i = mine;
+        for (int t = 0; t < r.tiles; ++t, i -= steps, to += r.nb * p.box_bytes, v += UP ? walk.per_tile : 0)
+          for (; i < steps; i += LOADERS) {
+            const uint32_t dst = to + i * p.box_bytes;
+            const int kk = (b + i) * BLOCK_K;
+            // K-major: (K, value, column of the value, expert). N-major: (column, half, K, expert).
+            if (KMAJOR) tma_load_4d(dst, &tmap, full_bar(s), kk, v, 0, e);
+            else tma_load_4d(dst, &tmap, full_bar(s), woven ? 2 * v : v, 0, kk, e);
+            if (halves) tma_load_4d(dst + 2048, &tmap, full_bar(s), v, 1, kk, e);
+          }
       }
     }
     if (!ok)      // give copies already in flight time to land before the block goes away
@@ -300,29 +322,43 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   if (warp >= CONSUMERS + LOADERS) {
     // ---------------- the slots' rows: 16 bytes per thread, zeros beyond K ---------------------------------------------
     if (!UP) wait_for_previous_kernel();
-    const int g = tid - (CONSUMERS + LOADERS) * 32, chunk = g & 7, row0 = g >> 3;      // rows row0, row0 + 8, ...
+    const int g = tid - (CONSUMERS + LOADERS) * 32, turn = g / GATHER_THREADS;
+    const int chunk = g & 7, row0 = (g % GATHER_THREADS) >> 3;                          // rows row0, row0 + 8, ...
+    static_assert(GATHER_THREADS == 64, "eight rows at a time");
     const uint32_t mine = row0 * 128 + static_cast<uint32_t>((chunk ^ row0) << 4);      // row & 7 == row0
     Run r;
     RingPos at;
     bool ok = true;
     while (walk.next(r) && ok) {
       const int n = plan->job_count[r.job], beg = plan->job_begin[r.job];
+      shape_of<UP>(p, r, n);
+      const int x_block = r.groups * 1024;
       const uint8_t* src[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = beg + min(row0 + 8 * i, n - 1);
-        src[i] = UP ? static_cast<const uint8_t*>(a.X) + static_cast<int64_t>(token[j]) * a.sxm * 2
-                    : p.hidden + static_cast<int64_t>(plan->slots[j]) * a.F * 2;
-      }
+      bool have = false;
       for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
         const int s = at.stage, steps = min(r.nb, r.b1 - b);
-        if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 23)) { ok = false; break; }
-        uint32_t dst = ring0 + s * p.stage_bytes + p.x_offset + mine;
-        int kk = b * BLOCK_K + chunk * 8;
-        for (int st = 0; st < steps; ++st, kk += BLOCK_K, dst += p.NT * 128)
+        if ((s & (GATHER_TURNS - 1)) != turn) continue;
+        if (!have) {
+          have = true;
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (row0 + 8 * i < n) cp_async16(dst + i * 1024, src[i] + (kk < p.K ? kk * 2 : 0), kk < p.K ? 16 : 0);
+            if (row0 + 8 * i < n) {
+              const int j = beg + row0 + 8 * i;
+              src[i] = UP ? static_cast<const uint8_t*>(a.X) + static_cast<int64_t>(token[j]) * a.sxm * 2
+                          : p.hidden + static_cast<int64_t>(plan->slots[j]) * a.F * 2;
+            }
+        }
+        if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 23)) { ok = false; break; }
+        const uint32_t dst = ring0 + s * p.stage_bytes + r.x_offset + mine;
+        const int k0 = b * BLOCK_K + chunk * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (row0 + 8 * i < n) {
+            uint32_t to = dst + i * 1024;
+            int kk = k0;
+            for (int st = 0; st < steps; ++st, kk += BLOCK_K, to += x_block)
+              cp_async16(to, src[i] + (kk < p.K ? kk * 2 : 0), kk < p.K ? 16 : 0);
+          }
         cp_async_arrive(full_bar(s));
       }
     }
@@ -336,84 +372,115 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   bool ok = true;
   RingPos at;
   Run r;
+  // down: the warp's 16 columns of the tile, or (no more than 16 in all) its half of every box's K
+  const bool by_columns = !UP && p.rows > 16;
+  const int m0 = by_columns ? (warp & 1) * 16 : 0;
+  const int copies = by_columns ? CONSUMERS / 2 : CONSUMERS, copy = by_columns ? warp >> 1 : warp;
   // ldmatrix addresses of this lane inside a box and inside a step of the slots' rows; 16 of K further: see `step`
   uint32_t w_lane, x1_lane, x4_lane;
   {
     const int row = (lane & 7) + ((lane >> 3) & 1) * 8, xrow = (lane & 7) + (lane >> 4) * 8;
     const int krow = (lane & 7) + (lane >> 4) * 8;
-    if (KMAJOR) w_lane = row * 128 + (((lane >> 4) ^ (row & 7)) << 4);
+    if (KMAJOR) w_lane = (row + m0) * 128 + (((lane >> 4) ^ (row & 7)) << 4);
     else if (halves) w_lane = krow * 32 + ((((lane >> 3) & 1) ^ ((krow >> 2) & 1)) << 4);      // 32-byte rows
-    else w_lane = krow * 64 + ((((lane >> 3) & 1) ^ ((krow >> 1) & 3)) << 4);
+    else w_lane = krow * 64 + (((((lane >> 3) & 1) + (m0 >> 3)) ^ ((krow >> 1) & 3)) << 4);
     x1_lane = (lane & 7) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
     x4_lane = xrow * 128 + ((((lane >> 3) & 1) ^ (xrow & 7)) << 4);
   }
-  const int x_block = p.NT * 128, w_step = halves ? 512 : 1024;
+  const int w_step = halves ? 512 : 1024;
   while (walk.next(r)) {
     const int n = plan->job_count[r.job], beg = plan->job_begin[r.job], e = plan->job_expert[r.job];
-    const int groups = (n + 7) >> 3;
-    // the warp's weight rows: up, tile `warp` of the round; down, the one tile
+    shape_of<UP>(p, r, n);
+    const int groups = r.groups, x_block = groups * 1024;
+    // the warp's weight rows: up, tile `warp` of the round; down, its part of the one tile
     const int v0 = UP ? r.p0 + warp * walk.per_tile : r.p0;
     const int count = UP ? min(walk.per_tile, r.count - warp * walk.per_tile) : r.count;
-    const bool use0 = count > 0, use1 = pairs ? (woven && !KMAJOR ? count > 8 : use0) : count > 16;
-    if (!UP && r.first)
-      for (int i = lane; i < a.T * pitch; i += 32) sums[warp * a.T * pitch + i] = 0.f;
-    float acc[2][4][4];
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][g][q] = 0.f;
+    const bool use0 = count > m0, use1 = UP && (pairs ? (woven && !KMAJOR ? count > 8 : use0) : count > 16);
+    if (!UP && r.first && (!by_columns || !(warp & 1))) {
+      for (int i = lane; i < a.T * pitch; i += 32) sums[copy * a.T * pitch + i] = 0.f;
+    }
+    if (!UP && r.first && by_columns) consumers_sync();        // a pair shares its sums
+    constexpr int M = UP ? 2 : 1;                              // 16-row halves a warp multiplies
+    float acc[M][4][4];
+    bool mine = false;                                         // this warp has a part of the run
     auto stream = [&](auto G_) {
       constexpr int G = decltype(G_)::value;           // groups of 8 slots, rounded up to 1, 2 or 4
+      // independent accumulators for neighbouring steps: a chain of dependent products would leave the warp waiting
+      constexpr int S = G == 1 ? 4 : (G == 2 ? 2 : 1);
+      float part[S][M][G][4];
+#pragma unroll
+      for (int c = 0; c < S; ++c)
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[c][m][g][q] = 0.f;
       for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
         const int s = at.stage;
+        if (!UP && (s & (DOWN_TURNS - 1)) != (warp >> 1)) continue;
+        mine = true;
         if (ok) ok = mbar_wait_warp(full_bar(s), at.phase, abort_flag, p.status, 22);
         if (ok && use0) {
           const int steps = min(r.nb, r.b1 - b);
-          const uint32_t wst = ring0 + s * p.stage_bytes + (UP ? warp * r.nb * p.box_bytes : 0), xst = ring0 + s * p.stage_bytes + p.x_offset;
-          auto step = [&](uint32_t w, uint32_t x, int i) {       // the i-th 16 of K of a box
-            uint32_t a0[4], a1[4] = {0, 0, 0, 0}, bx[G][2];
+          uint32_t w = ring0 + s * p.stage_bytes + (UP ? warp * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
+          auto step = [&](int i, float (&to)[M][G][4]) {       // the i-th 16 of K of a box
+            uint32_t a0[4], a1[4], bx[G][2];
             if (KMAJOR) {
               ldsm4(a0, w + (w_lane ^ (i << 5)));
-              if (use1) ldsm4(a1, w + (w_lane ^ (i << 5)) + 16 * 128);
+              if (UP && use1) ldsm4(a1, w + (w_lane ^ (i << 5)) + 16 * 128);
             } else {
               ldsm4_trans(a0, w + w_lane + i * w_step);
-              if (use1) ldsm4_trans(a1, w + (halves ? w_lane + 2048 : w_lane ^ 32) + i * w_step);
+              if (UP && use1) ldsm4_trans(a1, w + (halves ? w_lane + 2048 : w_lane ^ 32) + i * w_step);
             }
             if (G == 1) {
               ldsm2(bx[0][0], bx[0][1], x + (x1_lane ^ (i << 5)));
             } else {
 #pragma unroll
               for (int g = 0; g < G; g += 2) {
-                uint32_t t[4];
-                ldsm4(t, x + (x4_lane ^ (i << 5)) + g * 1024);
+                uint32_t t[4] = {0, 0, 0, 0};
+                if (g < groups) ldsm4(t, x + (x4_lane ^ (i << 5)) + g * 1024);
                 bx[g][0] = t[0]; bx[g][1] = t[1]; bx[g + 1][0] = t[2]; bx[g + 1][1] = t[3];
               }
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-              Mma<T>::run(acc[0][g], a0, bx[g][0], bx[g][1]);
-              if (use1) Mma<T>::run(acc[1][g], a1, bx[g][0], bx[g][1]);
+              Mma<T>::run(to[0][g], a0, bx[g][0], bx[g][1]);
+              if (UP && use1) Mma<T>::run(to[M - 1][g], a1, bx[g][0], bx[g][1]);
             }
           };
-          if (UP) {
-            for (int i = 0; i < steps; ++i) {
+          if (UP || by_columns) {
+            for (int i = 0; i < steps; ++i, w += p.box_bytes, x += x_block) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) step(wst + i * p.box_bytes, xst + i * x_block, q);
+              for (int q = 0; q < 4; ++q) step(q, part[q % S]);
             }
           } else {
-            // half a box per warp and turn
-            for (int i = warp >> 1; i < steps; i += CONSUMERS / 2) {
-              const uint32_t w = wst + i * p.box_bytes, x = xst + i * x_block;
-              step(w, x, (warp & 1) * 2);
-              step(w, x, (warp & 1) * 2 + 1);
+            for (int i = 0; i < steps; i += 2) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (i + h < steps) {
+                  step((warp & 1) * 2, part[(h * 2) % S]);
+                  step((warp & 1) * 2 + 1, part[(h * 2 + 1) % S]);
+                  w += p.box_bytes;
+                  x += x_block;
+                }
             }
           }
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty_bar(s));
       }
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v = part[0][m][g][q];
+#pragma unroll
+            for (int c = 1; c < S; ++c) v += part[c][m][g][q];
+            acc[m][g][q] = v;
+          }
     };
     if (groups == 1) stream(std::integral_constant<int, 1>{});
     else if (groups == 2) stream(std::integral_constant<int, 2>{});
@@ -427,7 +494,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
-          float c[2][2] = {{acc[0][g][q], acc[1][g][q]}, {0.f, 0.f}};       // (first, second column) of up to two values
+          float c[2][2] = {{acc[0][g][q], acc[M - 1][g][q]}, {0.f, 0.f}};       // (first, second column) of up to two values
           int v[2] = {row, -1};
           if (!pairs) {
             c[1][0] = c[0][1];
@@ -440,7 +507,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           }
           if (i >= n) continue;
           const int slot = plan->slots[beg + i];
-          const float gate = a.gates ? load_any(a.gates, token[beg + i] * a.sgt + (slot - token[beg + i] * a.k) * a.sgk, a.gates_dtype) : 1.f;
+          const float gate = sums[beg + i];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (v[h] < 0 || v[h] >= count) continue;
@@ -459,32 +526,46 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     } else {
       // add the job's slots to this warp's token sums. Slots of one token (the same expert twice) stand together and may sit in
       // neighbouring lanes: then the lanes take turns
-      float* own = sums + warp * a.T * pitch;
-      const bool twice = __any_sync(0xffffffffu, lane > 0 && lane < n && token[beg + min(lane, n - 1)] == token[beg + min(lane, n - 1) - (lane > 0)]);
-      for (int turn = 0; turn < (twice ? 4 : 1); ++turn) {
-        if (!twice || (lane & 3) == turn) {
+      if (mine && use0) {
+        float* own = sums + copy * a.T * pitch + m0;
+        const bool twice = __any_sync(0xffffffffu, lane > 0 && lane < n && token[beg + min(lane, n - 1)] == token[beg + min(lane, n - 1) - (lane > 0)]);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (g >= groups) continue;
+        for (int g = 0; g < 4; ++g) {
+          if (g >= groups) continue;
+          float* to[4];
+          bool in[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
-              if (i >= n) continue;
-              float* to = own + token[beg + i] * pitch + row;
-              if (row < count) to[0] += acc[0][g][q];
-              if (use1 && 16 + row < count) to[16] += acc[1][g][q];
+          for (int q = 0; q < 4; ++q) {
+            const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
+            to[q] = own + token[beg + min(i, n - 1)] * pitch + row;
+            in[q] = i < n && m0 + row < count;
+          }
+          if (!twice) {      // all different: read, add, write
+            float v[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = in[q] ? *to[q] : 0.f;
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (in[q]) *to[q] = v[q] + acc[0][g][q];
+          } else {
+            for (int turn = 0; turn < 4; ++turn) {
+              if ((lane & 3) == turn) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  if (in[q]) *to[q] += acc[0][g][q];
+              }
+              __syncwarp();
             }
           }
         }
-        if (twice) __syncwarp();
+        __syncwarp();
       }
       if (r.last) {
         consumers_sync();
         bool write = true;
         auto total_of = [&](int t, int col) {
           float v = 0.f;
-#pragma unroll
-          for (int w = 0; w < CONSUMERS; ++w) v += sums[(w * a.T + t) * pitch + col];
+          for (int w = 0; w < copies; ++w) v += sums[(w * a.T + t) * pitch + col];
           return v;
         };
         int64_t first = 0, stop = 0, tile_beg = 0, total = 1;
@@ -587,30 +668,26 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   p.rows = UP ? 0 : (KMAJOR ? down_rows(a.d_out, grid) : TILE);
   // shared memory that is not the ring
   const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 +
-                    (UP ? 0 : CONSUMERS * a.T * (p.rows + 1) * 4) + 1024 + 64;
+                    (UP ? MAX_R * 4 : (p.rows > 16 ? CONSUMERS / 2 : CONSUMERS) * a.T * (p.rows + 1) * 4) + 1024 + 64;
   const int budget = (di.max_smem_optin < 232448 ? di.max_smem_optin : 232448) - fixed;
   const int rows = UP || !KMAJOR ? TILE : p.rows;
   p.load_bytes = rows * BLOCK_K * 2;
   p.box_bytes = cdiv(rows, 8) * 1024;                      // boxes start on the swizzle's period
   p.blocks = cdiv(p.K, BLOCK_K);
   const int slack = 2048;      // ldmatrix reads whole 16-row blocks: past a box of fewer rows (never used, but inside the ring)
-  if (UP) {
-    // a stage is up to 8 boxes (32 KB): one step of K of 8 tiles, or more steps of fewer tiles
-    p.slots = CONSUMERS;
-    p.x_slots = 64 / p.NT;                                 // at most 8 KB of the slots' rows
-    p.x_offset = p.slots * p.box_bytes;
-    p.stage_bytes = p.x_offset + p.x_slots * p.NT * 128;
-  } else {
-    // steps of K: up to 32 KB of weights where the ring then still holds four stages, else half of that
-    int most = 32768 / p.box_bytes;
-    if ((budget - slack) / (most * (p.box_bytes + p.NT * 128)) < 4) most /= 2;
-    p.slots = p.x_slots = cdiv(p.blocks, cdiv(p.blocks, most));
-    p.x_offset = p.slots * p.box_bytes;
-    p.stage_bytes = p.x_offset + p.slots * p.NT * 128;
+  // Four stages (a multiple of the turns) of up to 48 KB: weights and, beside them, the rows of the job's slots.
+  constexpr int TURNS = UP ? GATHER_TURNS : DOWN_TURNS;
+  static_assert(4 % TURNS == 0, "every stage belongs to the same warps in every pass");
+  p.stages = 4;
+  p.stage_bytes = (budget - slack) / 4 / 1024 * 1024;
+  if (p.stage_bytes > 48 * 1024) p.stage_bytes = 48 * 1024;
+  for (int g = 0; g < 4; ++g) {
+    int steps = p.stage_bytes / (p.box_bytes + (g + 1) * 1024);
+    if (UP && steps > CONSUMERS) steps = CONSUMERS;      // more tiles: fewer steps, never more boxes than one tile would have
+    if (steps < 1) return SMOE_ERR_UNSUPPORTED;
+    p.steps_of[g] = cdiv(p.blocks, cdiv(p.blocks, steps));
   }
-  p.stages = (budget - slack) / p.stage_bytes;
-  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  if (p.stages < 2) return SMOE_ERR_UNSUPPORTED;
+  if (UP && p.stage_bytes < CONSUMERS * p.box_bytes + 4 * 1024) return SMOE_ERR_UNSUPPORTED;      // 8 tiles, one step, 32 slots
   p.ring_bytes = p.stages * p.stage_bytes + slack;
   const int scratch = (plan_scratch_bytes(a.E) + 15) / 16 * 16;      // the plan sorts in the ring before the first copy
   if (scratch > budget) return SMOE_ERR_UNSUPPORTED;
@@ -653,7 +730,7 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
   p.counters = reinterpret_cast<int*>(after);
   p.partial = reinterpret_cast<float*>(after + (static_cast<size_t>(p.n_counters) * 4 + 15) / 16 * 16);
   p.status = a.status;
-  p.NT = a.T <= 8 ? 8 : (a.T <= 16 ? 16 : 32);
+  p.NT = 32;
   const int grid = di.sm_count < MAX_CTAS ? di.sm_count : MAX_CTAS;
   CUtensorMap m1, m2;
   memset(&m1, 0, sizeof(m1));

@@ -63,6 +63,41 @@ __device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* __
   uint32_t* packed = reinterpret_cast<uint32_t*>(scratch);                    // [E] count | jobs << 16, then their prefixes
   uint16_t* hist = reinterpret_cast<uint16_t*>(scratch + ((E * 4 + 15) & ~15));   // [PLAN_WARPS][E]
   const int R = T * k;
+  if (R <= 32) {      // one warp sorts them in registers: position = slots of a lower expert + earlier slots of the same
+    if (warp == 0) {
+      int e = MAX_E + 1;
+      if (lane < R) {
+        const int64_t id = ids[static_cast<int64_t>(lane / k) * sit + static_cast<int64_t>(lane % k) * sik];
+        if (id >= 0 && id < E) e = static_cast<int>(id);
+      }
+      const bool live = e < E;
+      int lower = 0, same = 0, total = 0, jobs_before = 0;
+      for (int o = 0; o < R; ++o) {
+        const int oe = __shfl_sync(0xffffffffu, e, o);
+        lower += oe < e;
+        total += oe == e;
+        same += oe == e && o < lane;
+      }
+      const bool leads = live && same == 0;
+      const int my_jobs = leads ? (total + NT - 1) / NT : 0;
+      int all_jobs = 0;
+      for (int o = 0; o < R; ++o) {
+        const int oe = __shfl_sync(0xffffffffu, e, o), oj = __shfl_sync(0xffffffffu, my_jobs, o);
+        jobs_before += oe < e ? oj : 0;
+        all_jobs += oj;
+      }
+      if (live) plan->slots[lower + same] = static_cast<uint16_t>(lane);
+      if (leads)
+        for (int c = 0, job = jobs_before; c < total; c += NT, ++job) {
+          plan->job_expert[job] = static_cast<uint16_t>(e);
+          plan->job_begin[job] = static_cast<uint16_t>(lower + c);
+          plan->job_count[job] = static_cast<uint16_t>(min(NT, total - c));
+        }
+      if (lane == 0) plan->jobs = all_jobs;
+    }
+    __syncthreads();
+    return;
+  }
   constexpr int STEPS = MAX_R / (PLAN_WARPS * 32);
   const int steps = (R + PLAN_WARPS * 32 - 1) / (PLAN_WARPS * 32);
   for (int i = tid; i < PLAN_WARPS * E; i += nthreads) hist[i] = 0;
