@@ -25,7 +25,7 @@
 //
 // Weights with contiguous inputs ("K-major", nn.Linear storage) are read through ldmatrix and may start at any row, so that a range may
 // begin anywhere (rows that two blocks load come from L2); weights with contiguous outputs ("N-major") through the transposing
-// form. N-major columns are too few to give every SM its own, so there the down-projection's list (column tile, job, piece of K)
+// form, in boxes of 64 columns that two warps share (128-byte rows; with 64-byte rows the stream reached 60 %). N-major columns are too few to give every SM its own, so there the down-projection's list (column tile, job, piece of K)
 // is cut into equal parts and partial sums are joined in a fixed order by the last block of a tile.
 //
 // The down-projection starts (programmatic launch) while the up-projection drains: it plans and fills its ring with weights, which do not
@@ -56,14 +56,14 @@ constexpr int DOWN_TURNS = 4;                      // down: pairs of multiplying
 constexpr int THREADS = (CONSUMERS + LOADERS + GATHERERS) * 32;
 // The number of stages is a multiple of the turns: every stage then always belongs to the same warps, which wait for each of its passes.
 constexpr int MAX_STAGES = 16;
-constexpr int TILE = 32;                           // weight rows (output columns) of a tile
+constexpr int TILE = 32;                           // weight rows (output columns) of a warp's tile
 constexpr int BLOCK_K = 64;                        // K of a box: one 128-byte line of 16-bit values
 constexpr int MAX_CTAS = 160;
 
 struct StreamParams {
   Args a;
   uint8_t* hidden;            // (R, F), storage type of the tokens
-  float* partial;             // N-major down-projection: [block][2][T][TILE]
+  float* partial;             // N-major down-projection: [block][2][T][2 * TILE]
   int* counters;              // one per column tile of it, zeroed by the up-projection
   int n_counters;
   int32_t* status;
@@ -128,10 +128,11 @@ struct RingPos {
 // ---- the list of runs of a block --------------------------------------------------------------------------
 // A run is a stretch of K of one job: up, a round of `tiles` tiles over the whole of K, `nb` steps of K per stage; down, (part
 // of) the K of the block's tile. The runs of a tile follow each other; `last` closes the tile (for this block).
-struct Run { int job, b0, b1, nb, p0, count, tiles, tile, groups, x_offset; bool first, last; };
+struct Run { int job, b0, b1, nb, p0, count, tiles, tile, groups, boxes, x_offset; bool first, last; };
 
 template <bool UP, bool KMAJOR>
 struct Walker {
+  static constexpr int DOWN_TILE = KMAJOR ? TILE : 2 * TILE;      // output columns of a tile of the down-projection
   int lo, hi, units, jobs, blocks, width, per_tile, job, tile, step;
 
   // up, K-major: [lo, hi) is this block's part of all jobs' hidden values; N-major: of all jobs' tiles (boxes start on a multiple).
@@ -150,7 +151,7 @@ struct Walker {
     } else {
       width = p.a.d_out;
       units = jobs * blocks;      // steps of K of one column tile
-      total = KMAJOR ? width : static_cast<int64_t>(units) * ((width + TILE - 1) / TILE);
+      total = KMAJOR ? width : static_cast<int64_t>(units) * ((width + DOWN_TILE - 1) / DOWN_TILE);
     }
     lo = static_cast<int>(total * b / g);
     hi = static_cast<int>(total * (b + 1) / g);
@@ -197,8 +198,8 @@ struct Walker {
       r.job = job;
       r.b0 = step;
       r.b1 = min(blocks, step + (hi - lo));
-      r.p0 = tile * TILE;
-      r.count = min(TILE, width - r.p0);
+      r.p0 = tile * DOWN_TILE;
+      r.count = min(DOWN_TILE, width - r.p0);
       lo += r.b1 - r.b0;
       r.last = lo >= hi || job + 1 == jobs;
     }
@@ -207,12 +208,14 @@ struct Walker {
 };
 
 // Steps of K in a stage of this run, and where its slots' rows start (after the weights; `groups` x 8 rows of 128 bytes per step).
-template <bool UP>
+// An N-major box holds two tiles.
+template <bool UP, bool KMAJOR>
 __device__ __forceinline__ void shape_of(const StreamParams& p, Run& r, int n) {
   r.groups = (n + 7) >> 3;
   r.nb = p.steps_of[r.groups - 1];
   if (UP && r.tiles > 1) r.nb = min(r.nb, r.tiles == 2 ? 4 : (r.tiles <= 4 ? 2 : 1));
-  r.x_offset = r.tiles * r.nb * p.box_bytes;
+  r.boxes = KMAJOR ? r.tiles : (r.tiles + 1) >> 1;
+  r.x_offset = r.boxes * r.nb * p.box_bytes;
 }
 
 // hidden value from the up-projection's one or two columns (act_math.cuh has the layouts)
@@ -269,7 +272,6 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   for (int i = tid; i < listed; i += THREADS) {
     const int slot = plan->slots[i], t = slot / a.k;
     token[i] = static_cast<uint8_t>(t);
-    if (UP) sums[i] = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
   }
   fence_proxy_async_smem();            // the plan's scratch in the ring was written with ordinary stores
   __syncthreads();
@@ -286,7 +288,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   walk.init(p, plan->jobs);
   const bool pairs = UP && a.act_layout != LAYOUT_PLAIN;
   const bool woven = pairs && a.act_layout == LAYOUT_GPT_OSS;
-  const bool halves = !KMAJOR && pairs && !woven;      // N-major: a box is 16 columns of one half and 16 of the other
+  const bool halves = !KMAJOR && pairs && !woven;      // N-major: a box is 32 columns of one half and 32 of the other
 
   if (warp >= CONSUMERS && warp < CONSUMERS + LOADERS) {
     // ---------------- weights: they depend on no kernel before, so nothing is waited for -----------------------------
@@ -297,21 +299,21 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     bool ok = true;
     while (walk.next(r) && ok) {
       const int e = plan->job_expert[r.job];
-      shape_of<UP>(p, r, plan->job_count[r.job]);
+      shape_of<UP, KMAJOR>(p, r, plan->job_count[r.job]);
       for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
         const int s = at.stage, steps = min(r.nb, r.b1 - b);
         if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
-        mbar_arrive_expect_tx(full_bar(s), ((UP ? r.tiles * steps : steps) - mine + LOADERS - 1) / LOADERS * p.load_bytes);
+        mbar_arrive_expect_tx(full_bar(s), ((UP ? r.boxes * steps : steps) - mine + LOADERS - 1) / LOADERS * p.load_bytes);
         uint32_t to = ring0 + s * p.stage_bytes;
         int v = r.p0, i = mine;
-        for (int t = 0; t < r.tiles; ++t, i -= steps, to += r.nb * p.box_bytes, v += UP ? walk.per_tile : 0)
+        for (int t = 0; t < r.boxes; ++t, i -= steps, to += r.nb * p.box_bytes, v += UP ? (KMAJOR ? 1 : 2) * walk.per_tile : 0)
           for (; i < steps; i += LOADERS) {
             const uint32_t dst = to + i * p.box_bytes;
             const int kk = (b + i) * BLOCK_K;
             // K-major: (K, value, column of the value, expert). N-major: (column, half, K, expert).
             if (KMAJOR) tma_load_4d(dst, &tmap, full_bar(s), kk, v, 0, e);
             else tma_load_4d(dst, &tmap, full_bar(s), woven ? 2 * v : v, 0, kk, e);
-            if (halves) tma_load_4d(dst + 2048, &tmap, full_bar(s), v, 1, kk, e);
+            if (halves) tma_load_4d(dst + 4096, &tmap, full_bar(s), v, 1, kk, e);
           }
       }
     }
@@ -331,7 +333,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     bool ok = true;
     while (walk.next(r) && ok) {
       const int n = plan->job_count[r.job], beg = plan->job_begin[r.job];
-      shape_of<UP>(p, r, n);
+      shape_of<UP, KMAJOR>(p, r, n);
       const int x_block = r.groups * 1024;
       const uint8_t* src[4];
       bool have = false;
@@ -368,39 +370,54 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 
   // ---------------- products -----------------------------------------------------------------------------------
   // a wait that runs out does not leave the loops: the barriers below stay matched, the results are reported as invalid
-  if (!UP) wait_for_previous_kernel();
+  if (UP) {
+    for (int i = tid; i < listed; i += CONSUMERS * 32) {
+      const int slot = plan->slots[i], t = token[i];
+      sums[i] = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
+    }
+    consumers_sync();
+  } else {
+    wait_for_previous_kernel();
+  }
   bool ok = true;
   RingPos at;
   Run r;
-  // down: the warp's 16 columns of the tile, or (no more than 16 in all) its half of every box's K
+  // down: the warp's half of the tile's columns, or (K-major, no more than 16 in all) its half of every box's K
   const bool by_columns = !UP && p.rows > 16;
-  const int m0 = by_columns ? (warp & 1) * 16 : 0;
+  const int m0 = by_columns ? (warp & 1) * (KMAJOR ? 16 : 32) : 0;
   const int copies = by_columns ? CONSUMERS / 2 : CONSUMERS, copy = by_columns ? warp >> 1 : warp;
   // ldmatrix addresses of this lane inside a box and inside a step of the slots' rows; 16 of K further: see `step`
-  uint32_t w_lane, x1_lane, x4_lane;
+  uint32_t w_lane, w_lane1 = 0, x1_lane, x4_lane;
   {
     const int row = (lane & 7) + ((lane >> 3) & 1) * 8, xrow = (lane & 7) + (lane >> 4) * 8;
-    const int krow = (lane & 7) + (lane >> 4) * 8;
-    if (KMAJOR) w_lane = (row + m0) * 128 + (((lane >> 4) ^ (row & 7)) << 4);
-    else if (halves) w_lane = krow * 32 + ((((lane >> 3) & 1) ^ ((krow >> 2) & 1)) << 4);      // 32-byte rows
-    else w_lane = krow * 64 + (((((lane >> 3) & 1) + (m0 >> 3)) ^ ((krow >> 1) & 3)) << 4);
+    const int krow = (lane & 7) + (lane >> 4) * 8, chunk = (lane >> 3) & 1;
+    if (KMAJOR) {
+      w_lane = (row + m0) * 128 + (((lane >> 4) ^ (row & 7)) << 4);
+      w_lane1 = w_lane + 16 * 128;
+    } else if (halves) {      // 64-byte rows, the warp's 16 columns of either half
+      w_lane = krow * 64 + (((chunk + (warp & 1) * 2) ^ ((krow >> 1) & 3)) << 4);
+      w_lane1 = w_lane + 4096;
+    } else {                  // 128-byte rows, the warp's 32 columns
+      w_lane = krow * 128 + (((chunk + (warp & 1) * 4) ^ (krow & 7)) << 4);
+      w_lane1 = w_lane ^ 32;
+    }
     x1_lane = (lane & 7) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
     x4_lane = xrow * 128 + ((((lane >> 3) & 1) ^ (xrow & 7)) << 4);
   }
-  const int w_step = halves ? 512 : 1024;
+  const int w_step = halves ? 1024 : 2048;
   while (walk.next(r)) {
     const int n = plan->job_count[r.job], beg = plan->job_begin[r.job], e = plan->job_expert[r.job];
-    shape_of<UP>(p, r, n);
+    shape_of<UP, KMAJOR>(p, r, n);
     const int groups = r.groups, x_block = groups * 1024;
     // the warp's weight rows: up, tile `warp` of the round; down, its part of the one tile
     const int v0 = UP ? r.p0 + warp * walk.per_tile : r.p0;
     const int count = UP ? min(walk.per_tile, r.count - warp * walk.per_tile) : r.count;
-    const bool use0 = count > m0, use1 = UP && (pairs ? (woven && !KMAJOR ? count > 8 : use0) : count > 16);
+    const bool use0 = count > m0, use1 = UP ? (pairs ? (woven && !KMAJOR ? count > 8 : use0) : count > 16) : count > m0 + 16;
     if (!UP && r.first && (!by_columns || !(warp & 1))) {
       for (int i = lane; i < a.T * pitch; i += 32) sums[copy * a.T * pitch + i] = 0.f;
     }
     if (!UP && r.first && by_columns) consumers_sync();        // a pair shares its sums
-    constexpr int M = UP ? 2 : 1;                              // 16-row halves a warp multiplies
+    constexpr int M = UP || !KMAJOR ? 2 : 1;                   // 16-row halves a warp multiplies
     float acc[M][4][4];
     bool mine = false;                                         // this warp has a part of the run
     auto stream = [&](auto G_) {
@@ -423,15 +440,15 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
         if (ok) ok = mbar_wait_warp(full_bar(s), at.phase, abort_flag, p.status, 22);
         if (ok && use0) {
           const int steps = min(r.nb, r.b1 - b);
-          uint32_t w = ring0 + s * p.stage_bytes + (UP ? warp * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
+          uint32_t w = ring0 + s * p.stage_bytes + (UP ? (KMAJOR ? warp : warp >> 1) * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
           auto step = [&](int i, float (&to)[M][G][4]) {       // the i-th 16 of K of a box
             uint32_t a0[4], a1[4], bx[G][2];
             if (KMAJOR) {
               ldsm4(a0, w + (w_lane ^ (i << 5)));
-              if (UP && use1) ldsm4(a1, w + (w_lane ^ (i << 5)) + 16 * 128);
+              if (M == 2 && use1) ldsm4(a1, w + (w_lane1 ^ (i << 5)));
             } else {
               ldsm4_trans(a0, w + w_lane + i * w_step);
-              if (UP && use1) ldsm4_trans(a1, w + (halves ? w_lane + 2048 : w_lane ^ 32) + i * w_step);
+              if (M == 2 && use1) ldsm4_trans(a1, w + w_lane1 + i * w_step);
             }
             if (G == 1) {
               ldsm2(bx[0][0], bx[0][1], x + (x1_lane ^ (i << 5)));
@@ -446,7 +463,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
               Mma<T>::run(to[0][g], a0, bx[g][0], bx[g][1]);
-              if (UP && use1) Mma<T>::run(to[M - 1][g], a1, bx[g][0], bx[g][1]);
+              if (M == 2 && use1) Mma<T>::run(to[M - 1][g], a1, bx[g][0], bx[g][1]);
             }
           };
           if (UP || by_columns) {
@@ -527,34 +544,37 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
       // add the job's slots to this warp's token sums. Slots of one token (the same expert twice) stand together and may sit in
       // neighbouring lanes: then the lanes take turns
       if (mine && use0) {
-        float* own = sums + copy * a.T * pitch + m0;
+        float* own = sums + copy * a.T * pitch + m0;       // the second 16 columns (N-major) follow 16 further
         const bool twice = __any_sync(0xffffffffu, lane > 0 && lane < n && token[beg + min(lane, n - 1)] == token[beg + min(lane, n - 1) - (lane > 0)]);
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           if (g >= groups) continue;
-          float* to[4];
-          bool in[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
-            to[q] = own + token[beg + min(i, n - 1)] * pitch + row;
-            in[q] = i < n && m0 + row < count;
-          }
-          if (!twice) {      // all different: read, add, write
-            float v[4];
+          for (int m = 0; m < M; ++m) {
+            float* to[4];
+            bool in[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = in[q] ? *to[q] : 0.f;
+            for (int q = 0; q < 4; ++q) {
+              const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = m * 16 + (lane >> 2) + (q >> 1) * 8;
+              to[q] = own + token[beg + min(i, n - 1)] * pitch + row;
+              in[q] = i < n && m0 + row < count;
+            }
+            if (!twice) {      // all different: read, add, write
+              float v[4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (in[q]) *to[q] = v[q] + acc[0][g][q];
-          } else {
-            for (int turn = 0; turn < 4; ++turn) {
-              if ((lane & 3) == turn) {
+              for (int q = 0; q < 4; ++q) v[q] = in[q] ? *to[q] : 0.f;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  if (in[q]) *to[q] += acc[0][g][q];
+              for (int q = 0; q < 4; ++q)
+                if (in[q]) *to[q] = v[q] + acc[m][g][q];
+            } else {
+              for (int turn = 0; turn < 4; ++turn) {
+                if ((lane & 3) == turn) {
+#pragma unroll
+                  for (int q = 0; q < 4; ++q)
+                    if (in[q]) *to[q] += acc[m][g][q];
+                }
+                __syncwarp();
               }
-              __syncwarp();
             }
           }
         }
@@ -562,6 +582,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
       }
       if (r.last) {
         consumers_sync();
+        constexpr int DT = Walker<UP, KMAJOR>::DOWN_TILE;
         bool write = true;
         auto total_of = [&](int t, int col) {
           float v = 0.f;
@@ -576,12 +597,12 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           // does this block hold the whole tile, or only a part of its steps?
           tile_beg = static_cast<int64_t>(r.tile) * walk.units;
           const int64_t tile_end = tile_beg + walk.units;
-          total = static_cast<int64_t>(walk.units) * ((a.d_out + TILE - 1) / TILE);
+          total = static_cast<int64_t>(walk.units) * ((a.d_out + DT - 1) / DT);
           const int64_t mine0 = begin_of(blockIdx.x), mine1 = begin_of(blockIdx.x + 1);
           split = mine0 > tile_beg || mine1 < tile_end;
           if (split) {
-            float* part = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (mine0 > tile_beg ? 0 : 1)) * a.T * TILE;
-            for (int i = tid; i < a.T * r.count; i += CONSUMERS * 32) part[(i / r.count) * TILE + i % r.count] = total_of(i / r.count, i % r.count);
+            float* part = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (mine0 > tile_beg ? 0 : 1)) * a.T * DT;
+            for (int i = tid; i < a.T * r.count; i += CONSUMERS * 32) part[(i / r.count) * DT + i % r.count] = total_of(i / r.count, i % r.count);
             __threadfence();
             consumers_sync();
             first = tile_beg * g / total;
@@ -602,7 +623,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
             if (split) {
               for (int64_t b = first; b < stop; ++b)
                 if (begin_of(b + 1) > begin_of(b))
-                  v += __ldcg(p.partial + ((b * 2 + (begin_of(b) > tile_beg ? 0 : 1)) * a.T + t) * TILE + col);
+                  v += __ldcg(p.partial + ((b * 2 + (begin_of(b) > tile_beg ? 0 : 1)) * a.T + t) * DT + col);
             } else {
               v = total_of(t, col);
             }
@@ -628,9 +649,9 @@ constexpr size_t HIDDEN_ALIGN = 256;
 static size_t hidden_bytes(int64_t T, int k, int F) {
   return (static_cast<size_t>(T) * k * F * 2 + HIDDEN_ALIGN - 1) / HIDDEN_ALIGN * HIDDEN_ALIGN;
 }
-static int column_tiles(int d_out) { return cdiv(d_out, TILE); }
+static int column_tiles(int d_out) { return cdiv(d_out, 2 * TILE); }
 size_t stream_workspace_bytes(int64_t T, int k, int F, int d_out) {
-  return hidden_bytes(T, k, F) + static_cast<size_t>(column_tiles(d_out)) * 4 + 16 + static_cast<size_t>(MAX_CTAS) * 2 * T * TILE * 4;
+  return hidden_bytes(T, k, F) + static_cast<size_t>(column_tiles(d_out)) * 4 + 16 + static_cast<size_t>(MAX_CTAS) * 2 * T * 2 * TILE * 4;
 }
 
 struct Order { bool k_major, n_major; };
@@ -649,14 +670,14 @@ static bool encode_k_major(CUtensorMap* map, bool bf16, const void* W, int K, in
   const uint32_t box[4] = {BLOCK_K, static_cast<uint32_t>(rows), static_cast<uint32_t>(halves), 1};
   return encode_tensor_map(map, bf16, W, 4, dim, stride, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
-// Boxes of one expert: 32 columns x 64 of K, 64-byte swizzle; where the two columns of a hidden value are a half apart, 16 columns of one
-// half x 64 of K, 32-byte swizzle.
+// Boxes of one expert: 64 columns x 64 of K, 128-byte swizzle; where the two columns of a hidden value are a half apart, 32 columns of one
+// half x 64 of K, 64-byte swizzle.
 static bool encode_n_major(CUtensorMap* map, bool bf16, const void* W, int N, int K, int64_t row_stride, int halves, int E, int64_t se) {
   const uint64_t dim[4] = {static_cast<uint64_t>(N / halves), static_cast<uint64_t>(halves), static_cast<uint64_t>(K), static_cast<uint64_t>(E)};
   const uint64_t stride[3] = {static_cast<uint64_t>(halves > 1 ? N / 2 : row_stride) * 2, static_cast<uint64_t>(row_stride) * 2,
                               static_cast<uint64_t>(E > 1 ? se : row_stride) * 2};
-  const uint32_t box[4] = {static_cast<uint32_t>(TILE / halves), 1, BLOCK_K, 1};
-  return encode_tensor_map(map, bf16, W, 4, dim, stride, box, halves > 1 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B);
+  const uint32_t box[4] = {static_cast<uint32_t>(2 * TILE / halves), 1, BLOCK_K, 1};
+  return encode_tensor_map(map, bf16, W, 4, dim, stride, box, halves > 1 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 // rows of a K-major box of the down-projection: the output columns of a block, at most a tile
@@ -665,12 +686,12 @@ static int down_rows(int d_out, int grid) { return cdiv(d_out, grid) < TILE ? cd
 template <typename T, bool UP, bool KMAJOR>
 static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& di, int grid) {
   const Args& a = p.a;
-  p.rows = UP ? 0 : (KMAJOR ? down_rows(a.d_out, grid) : TILE);
+  p.rows = UP ? 0 : (KMAJOR ? down_rows(a.d_out, grid) : 2 * TILE);
   // shared memory that is not the ring
   const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 +
                     (UP ? MAX_R * 4 : (p.rows > 16 ? CONSUMERS / 2 : CONSUMERS) * a.T * (p.rows + 1) * 4) + 1024 + 64;
   const int budget = (di.max_smem_optin < 232448 ? di.max_smem_optin : 232448) - fixed;
-  const int rows = UP || !KMAJOR ? TILE : p.rows;
+  const int rows = KMAJOR ? (UP ? TILE : p.rows) : 2 * TILE;
   p.load_bytes = rows * BLOCK_K * 2;
   p.box_bytes = cdiv(rows, 8) * 1024;                      // boxes start on the swizzle's period
   p.blocks = cdiv(p.K, BLOCK_K);
@@ -683,11 +704,11 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   if (p.stage_bytes > 48 * 1024) p.stage_bytes = 48 * 1024;
   for (int g = 0; g < 4; ++g) {
     int steps = p.stage_bytes / (p.box_bytes + (g + 1) * 1024);
-    if (UP && steps > CONSUMERS) steps = CONSUMERS;      // more tiles: fewer steps, never more boxes than one tile would have
+    if (UP && steps > 32768 / p.box_bytes) steps = 32768 / p.box_bytes;      // more tiles: fewer steps, never more than 32 KB of weights
     if (steps < 1) return SMOE_ERR_UNSUPPORTED;
     p.steps_of[g] = cdiv(p.blocks, cdiv(p.blocks, steps));
   }
-  if (UP && p.stage_bytes < CONSUMERS * p.box_bytes + 4 * 1024) return SMOE_ERR_UNSUPPORTED;      // 8 tiles, one step, 32 slots
+  if (UP && p.stage_bytes < 48 * 1024) return SMOE_ERR_UNSUPPORTED;      // two tiles, four steps, 32 slots
   p.ring_bytes = p.stages * p.stage_bytes + slack;
   const int scratch = (plan_scratch_bytes(a.E) + 15) / 16 * 16;      // the plan sorts in the ring before the first copy
   if (scratch > budget) return SMOE_ERR_UNSUPPORTED;

@@ -312,7 +312,7 @@ int launch_simt(const Args& a) {
 
 // ---- router --------------------------------------------------------------------------------------------
 // A cluster of up to 8 blocks per token: logits z_e = <x, Wr[e]> + br[e] in fp32, a warp per expert, gathered in the first block's shared
-// memory; its first warp picks the k largest and makes the gates. Order: larger logit first, equal logits by lower expert
+// memory, which ranks them and makes the gates. Order: larger logit first, equal logits by lower expert
 // id, a NaN counts as the largest. Bound by latency: one block per token read the router's 0.5 MB (128 experts of 2048) in 25 us.
 constexpr int ROUTE_THREADS = 512;
 constexpr int ROUTE_CLUSTER = 8;
@@ -325,8 +325,8 @@ struct RouteParams {
   int E, d, k, mode, renorm;
 };
 
+// whether logit v of expert i goes before logit `best` of expert bi
 __device__ __forceinline__ bool beats(float v, int i, float best, int bi) {
-  if (bi < 0) return true;
   const bool vn = v != v, bn = best != best;
   if (vn != bn) return vn;
   if (vn || v == best) return i < bi;
@@ -360,45 +360,32 @@ ft_route_kernel(const RouteParams p) {
     if (lane == 0) z0[e] = acc + (p.br ? to_f32<T>(static_cast<const T*>(p.br)[e * p.sbn]) : 0.f);
   }
   cluster.sync();
-  if (part != 0 || warp != 0) return;
-  float total = 0.f, top = 0.f, mine = 0.f;
-  int my_id = 0;
-  if (p.mode == 0 && !p.renorm) {          // softmax over all experts
-    float m = -INFINITY;
-    for (int e = lane; e < p.E; e += 32) m = fmaxf(m, z[e]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    for (int e = lane; e < p.E; e += 32) total += expf(z[e] - m);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    top = m;
+  if (part != 0) return;
+  // An expert's place is the number of experts that beat it: every thread counts for its own, all at once (k rounds of a
+  // maximum over one warp took 2 us).
+  __shared__ float chosen[32];
+  __shared__ int chosen_id[32];
+  for (int e = threadIdx.x; e < p.E; e += ROUTE_THREADS) {
+    const float mine = z[e];
+    int place = 0;
+    for (int o = 0; o < p.E; ++o) place += beats(z[o], o, mine, e) && o != e;
+    if (place < p.k) { chosen[place] = mine; chosen_id[place] = e; }
   }
-  unsigned taken = 0;                       // bit i: this lane's expert lane + 32 i is selected
-  for (int j = 0; j < p.k; ++j) {
-    float best = 0.f;
-    int bi = -1;
-    for (int e = lane, i = 0; e < p.E; e += 32, ++i)
-      if (!(taken >> i & 1u) && beats(z[e], e, best, bi)) { best = z[e]; bi = e; }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, best, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (oi >= 0 && beats(ov, oi, best, bi)) { best = ov; bi = oi; }
-    }
-    if (lane == j) { mine = best; my_id = bi; }
-    if ((bi & 31) == lane) taken |= 1u << (bi >> 5);
-  }
+  __syncthreads();
+  if (warp != 0) return;
   const bool sel = lane < p.k;
-  const bool over_selected = p.mode == 1 || p.renorm;
-  if (over_selected) top = __shfl_sync(0xffffffffu, mine, 0);
+  const float mine = sel ? chosen[lane] : 0.f, top = chosen[0];       // the largest of all logits
   const float g = sel ? expf(mine - top) : 0.f;
-  if (over_selected) {
+  float total = 0.f;
+  if (p.mode == 0 && !p.renorm) {          // softmax over all experts
+    for (int e = lane; e < p.E; e += 32) total += expf(z[e] - top);
+  } else {
     total = g;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (sel) {
-    p.ids[static_cast<int64_t>(t) * p.k + lane] = my_id;
+    p.ids[static_cast<int64_t>(t) * p.k + lane] = chosen_id[lane];
     p.gates[static_cast<int64_t>(t) * p.k + lane] = g / total;
   }
 }
