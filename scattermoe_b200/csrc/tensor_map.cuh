@@ -26,7 +26,8 @@ inline TensorMapEncodeFn tensor_map_encoder() {
 
 // Axis 0 is contiguous; `stride[i]` of axis i + 1 in bytes (multiples of 16). Elements outside the axes read as zero.
 inline bool encode_tensor_map(CUtensorMap* map, bool bf16, const void* base, int rank, const uint64_t* dim, const uint64_t* stride,
-                              const uint32_t* box, CUtensorMapSwizzle swizzle) {
+                              const uint32_t* box, CUtensorMapSwizzle swizzle,
+                              CUtensorMapL2promotion promotion = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   TensorMapEncodeFn fn = tensor_map_encoder();
   if (!fn) return false;
   cuuint64_t dims[5], strides[4];
@@ -39,7 +40,7 @@ inline bool encode_tensor_map(CUtensorMap* map, bool bf16, const void* base, int
   }
   return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, static_cast<cuuint32_t>(rank),
             const_cast<void*>(base), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            promotion, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace smoe
