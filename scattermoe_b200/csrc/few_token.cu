@@ -23,8 +23,7 @@
 // 32 KB; stages of 8 KB 2.2-4.2. Hence few, large stages, and as many steps of K in one as the job's slots leave room for.
 // One bulk copy per weight row: 1.2-3 TB/s.
 //
-// Weights with contiguous inputs ("K-major", nn.Linear storage) are read through ldmatrix and may start at any row, so that a range may
-// begin anywhere (rows that two blocks load come from L2); weights with contiguous outputs ("N-major") through the transposing
+// Weights with contiguous inputs ("K-major", nn.Linear storage) are read through ldmatrix; weights with contiguous outputs ("N-major") through the transposing
 // form, in boxes of 64 columns that two warps share (128-byte rows; with 64-byte rows the stream reached 60 %). N-major columns are too few to give every SM its own, so there the down-projection's list (column tile, job, piece of K)
 // is cut into equal parts and partial sums are joined in a fixed order by the last block of a tile.
 //
@@ -66,6 +65,7 @@ struct StreamParams {
   float* partial;             // N-major down-projection: [block][2][T][2 * TILE]
   int* counters;              // one per column tile of it, zeroed by the up-projection
   int n_counters;
+  uint32_t part_step;         // 2^32 / blocks of the grid, rounded up
   int32_t* status;
   int NT;                     // slots of a job
   int K, blocks;              // K and its boxes
@@ -125,6 +125,14 @@ struct RingPos {
   }
 };
 
+// First of the units of block b when `total` units are dealt out evenly: the same for every caller, without a division.
+// part_step is 2^32 / blocks, rounded up; total < 2^30.
+__device__ __forceinline__ int part_begin(int total, int b, uint32_t part_step) {
+  const uint64_t share = static_cast<uint64_t>(static_cast<uint32_t>(b)) * part_step;        // of 2^32
+  const uint64_t at = share >= (1ull << 32) ? static_cast<uint64_t>(total) : (static_cast<uint64_t>(static_cast<uint32_t>(total)) * share) >> 32;
+  return static_cast<int>(at);
+}
+
 // ---- the list of runs of a block --------------------------------------------------------------------------
 // A run is a stretch of K of one job: up, a round of `tiles` tiles over the whole of K, `nb` steps of K per stage; down, (part
 // of) the K of the block's tile. The runs of a tile follow each other; `last` closes the tile (for this block).
@@ -135,26 +143,25 @@ struct Walker {
   static constexpr int DOWN_TILE = KMAJOR ? TILE : 2 * TILE;      // output columns of a tile of the down-projection
   int lo, hi, units, jobs, blocks, width, per_tile, job, tile, step;
 
-  // up, K-major: [lo, hi) is this block's part of all jobs' hidden values; N-major: of all jobs' tiles (boxes start on a multiple).
+  // up: [lo, hi) is this block's part of all jobs' tiles.
   // down, K-major: [lo, hi) are this block's output columns; N-major: its part of the flat list of steps of K, (tile, job, step).
   __device__ void init(const StreamParams& p, int n_jobs) {
     jobs = n_jobs;
     blocks = p.blocks;
     job = -1;
-    const int64_t b = blockIdx.x, g = gridDim.x;
-    int64_t total;
+    int total;
     if (UP) {
       width = p.a.F;
       per_tile = p.a.act_layout != LAYOUT_PLAIN ? TILE / 2 : TILE;
-      units = KMAJOR ? width : (width + per_tile - 1) / per_tile;
-      total = static_cast<int64_t>(units) * jobs;
+      units = (width + per_tile - 1) / per_tile;
+      total = units * jobs;
     } else {
       width = p.a.d_out;
       units = jobs * blocks;      // steps of K of one column tile
-      total = KMAJOR ? width : static_cast<int64_t>(units) * ((width + DOWN_TILE - 1) / DOWN_TILE);
+      total = KMAJOR ? width : units * ((width + DOWN_TILE - 1) / DOWN_TILE);
     }
-    lo = static_cast<int>(total * b / g);
-    hi = static_cast<int>(total * (b + 1) / g);
+    lo = part_begin(total, blockIdx.x, p.part_step);
+    hi = part_begin(total, blockIdx.x + 1, p.part_step);
   }
   __device__ bool next(Run& r) {
     if (lo >= hi) return false;
@@ -164,17 +171,12 @@ struct Walker {
     if (UP) {
       r.job = lo / units;
       const int in = lo - r.job * units;
-      if (KMAJOR) {
-        r.p0 = in;
-        r.count = min(min(CONSUMERS * per_tile, units - in), hi - lo);
-        lo += r.count;
-        r.tiles = (r.count + per_tile - 1) / per_tile;
-      } else {
-        r.tiles = min(min(CONSUMERS, units - in), hi - lo);
-        lo += r.tiles;
-        r.p0 = in * per_tile;
-        r.count = min(r.tiles * per_tile, width - r.p0);
-      }
+      // what is left of the job, in equal rounds: a last round of one tile would keep one warp busy and seven waiting
+      const int left = min(units - in, hi - lo), rounds = (left + CONSUMERS - 1) / CONSUMERS;
+      r.tiles = (left + rounds - 1) / rounds;
+      lo += r.tiles;
+      r.p0 = in * per_tile;
+      r.count = min(r.tiles * per_tile, width - r.p0);
     } else if (KMAJOR) {
       r.first = ++job == 0;
       r.job = job;
@@ -421,9 +423,9 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     float acc[M][4][4];
     bool mine = false;                                         // this warp has a part of the run
     auto stream = [&](auto G_) {
-      constexpr int G = decltype(G_)::value;           // groups of 8 slots, rounded up to 1, 2 or 4
+      constexpr int G = decltype(G_)::value;           // groups of 8 slots
       // independent accumulators for neighbouring steps: a chain of dependent products would leave the warp waiting
-      constexpr int S = G == 1 ? 4 : (G == 2 ? 2 : 1);
+      constexpr int S = !UP && !KMAJOR ? (G == 1 ? 2 : 1) : (G == 1 ? 4 : (G == 2 ? 2 : 1));      // (registers)
       float part[S][M][G][4];
 #pragma unroll
       for (int c = 0; c < S; ++c)
@@ -442,7 +444,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           const int steps = min(r.nb, r.b1 - b);
           uint32_t w = ring0 + s * p.stage_bytes + (UP ? (KMAJOR ? warp : warp >> 1) * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
           auto step = [&](int i, float (&to)[M][G][4]) {       // the i-th 16 of K of a box
-            uint32_t a0[4], a1[4], bx[G][2];
+            uint32_t a0[4], a1[4], bx[G + 1][2];
             if (KMAJOR) {
               ldsm4(a0, w + (w_lane ^ (i << 5)));
               if (M == 2 && use1) ldsm4(a1, w + (w_lane1 ^ (i << 5)));
@@ -455,8 +457,8 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
             } else {
 #pragma unroll
               for (int g = 0; g < G; g += 2) {
-                uint32_t t[4] = {0, 0, 0, 0};
-                if (g < groups) ldsm4(t, x + (x4_lane ^ (i << 5)) + g * 1024);
+                uint32_t t[4];
+                ldsm4(t, x + (x4_lane ^ (i << 5)) + g * 1024);
                 bx[g][0] = t[0]; bx[g][1] = t[1]; bx[g + 1][0] = t[2]; bx[g + 1][1] = t[3];
               }
             }
@@ -501,6 +503,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     };
     if (groups == 1) stream(std::integral_constant<int, 1>{});
     else if (groups == 2) stream(std::integral_constant<int, 2>{});
+    else if (groups == 3) stream(std::integral_constant<int, 3>{});
     else stream(std::integral_constant<int, 4>{});
 
     if (UP) {
@@ -589,23 +592,23 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           for (int w = 0; w < copies; ++w) v += sums[(w * a.T + t) * pitch + col];
           return v;
         };
-        int64_t first = 0, stop = 0, tile_beg = 0, total = 1;
-        const int64_t g = gridDim.x;
-        auto begin_of = [&](int64_t b) { return total * b / g; };
+        int first = 0, stop = 0, tile_beg = 0, total = 1;
+        const int g = static_cast<int>(gridDim.x);
+        auto begin_of = [&](int b) { return part_begin(total, b, p.part_step); };
         bool split = false;
         if (!KMAJOR) {
           // does this block hold the whole tile, or only a part of its steps?
-          tile_beg = static_cast<int64_t>(r.tile) * walk.units;
-          const int64_t tile_end = tile_beg + walk.units;
-          total = static_cast<int64_t>(walk.units) * ((a.d_out + DT - 1) / DT);
-          const int64_t mine0 = begin_of(blockIdx.x), mine1 = begin_of(blockIdx.x + 1);
+          tile_beg = r.tile * walk.units;
+          const int tile_end = tile_beg + walk.units;
+          total = walk.units * ((a.d_out + DT - 1) / DT);
+          const int mine0 = begin_of(blockIdx.x), mine1 = begin_of(blockIdx.x + 1);
           split = mine0 > tile_beg || mine1 < tile_end;
           if (split) {
             float* part = p.partial + (static_cast<int64_t>(blockIdx.x) * 2 + (mine0 > tile_beg ? 0 : 1)) * a.T * DT;
             for (int i = tid; i < a.T * r.count; i += CONSUMERS * 32) part[(i / r.count) * DT + i % r.count] = total_of(i / r.count, i % r.count);
             __threadfence();
             consumers_sync();
-            first = tile_beg * g / total;
+            first = static_cast<int>(static_cast<int64_t>(tile_beg) * g / total);
             while (first > 0 && begin_of(first) > tile_beg) --first;
             while (begin_of(first + 1) <= tile_beg) ++first;
             int parts = 0;
@@ -621,9 +624,9 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
             const int t = idx / r.count, col = idx - t * r.count;
             float v = 0.f;
             if (split) {
-              for (int64_t b = first; b < stop; ++b)
+              for (int b = first; b < stop; ++b)
                 if (begin_of(b + 1) > begin_of(b))
-                  v += __ldcg(p.partial + ((b * 2 + (begin_of(b) > tile_beg ? 0 : 1)) * a.T + t) * DT + col);
+                  v += __ldcg(p.partial + ((static_cast<int64_t>(b) * 2 + (begin_of(b) > tile_beg ? 0 : 1)) * a.T + t) * DT + col);
             } else {
               v = total_of(t, col);
             }
@@ -699,16 +702,25 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   p.box_bytes = cdiv(rows, 8) * 1024;                      // boxes start on the swizzle's period
   p.blocks = cdiv(p.K, BLOCK_K);
   const int slack = 2048;      // ldmatrix reads whole 16-row blocks: past a box of fewer rows (never used, but inside the ring)
-  // Four stages (a multiple of the turns) of up to 48 KB: weights and, beside them, the rows of the job's slots.
+  // Stages of up to 48 KB, weights and beside them the rows of the job's slots: four, or as many more (a multiple of the turns) as the
+  // ring holds where the whole of K needs less.
   constexpr int TURNS = UP ? GATHER_TURNS : DOWN_TURNS;
   static_assert(4 % TURNS == 0, "every stage belongs to the same warps in every pass");
-  p.stages = 4;
+  const int most_groups = a.T < 32 ? cdiv(a.T, 8) : 4;
   p.stage_bytes = (budget - slack) / 4 / 1024 * 1024;
   if (p.stage_bytes > 48 * 1024) p.stage_bytes = 48 * 1024;
+  const int whole = p.blocks * (p.box_bytes + most_groups * 1024);
+  if (!UP && whole < p.stage_bytes) p.stage_bytes = whole;
+  p.stages = (budget - slack) / p.stage_bytes;
+  p.stages = (p.stages > MAX_STAGES ? MAX_STAGES : p.stages) / TURNS * TURNS;
+  if (p.stages < TURNS) return SMOE_ERR_UNSUPPORTED;
   for (int g = 0; g < 4; ++g) {
     int steps = p.stage_bytes / (p.box_bytes + (g + 1) * 1024);
     if (UP && steps > 32768 / p.box_bytes) steps = 32768 / p.box_bytes;      // more tiles: fewer steps, never more than 32 KB of weights
-    if (steps < 1) return SMOE_ERR_UNSUPPORTED;
+    if (steps < 1) {
+      if (g < most_groups) return SMOE_ERR_UNSUPPORTED;
+      steps = 1;
+    }
     p.steps_of[g] = cdiv(p.blocks, cdiv(p.blocks, steps));
   }
   if (UP && p.stage_bytes < 48 * 1024) return SMOE_ERR_UNSUPPORTED;      // two tiles, four steps, 32 slots
@@ -756,6 +768,7 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
   p.status = a.status;
   p.NT = 32;
   const int grid = di.sm_count < MAX_CTAS ? di.sm_count : MAX_CTAS;
+  p.part_step = static_cast<uint32_t>(((1ull << 32) + grid - 1) / grid);
   CUtensorMap m1, m2;
   memset(&m1, 0, sizeof(m1));
   memset(&m2, 0, sizeof(m2));
@@ -775,7 +788,10 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
 int launch_stream(const Args& a) {
   if (a.dtype != SMOE_BF16 && a.dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
   if (a.d % 8 || a.F % 8 || a.sxm % 8 || !al16(a.X)) return SMOE_ERR_UNSUPPORTED;
-  if (a.d > (1 << 20) || a.F > (1 << 20) || a.d_out > (1 << 20)) return SMOE_ERR_UNSUPPORTED;     // 32-bit unit counts
+  {      // the lists of tiles and of steps of K are counted in 32 bits
+    const int64_t jobs = static_cast<int64_t>(a.T) * a.k, most = int64_t(1) << 30;
+    if (jobs * cdiv(a.F, TILE / 2) >= most || jobs * cdiv(a.F, BLOCK_K) * cdiv(a.d_out, TILE) >= most) return SMOE_ERR_UNSUPPORTED;
+  }
   DeviceInfo di;
   if (int rc = get_device_info(&di)) return rc;
   if (di.cc_major != 10) return SMOE_ERR_UNSUPPORTED;
