@@ -260,23 +260,26 @@ int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void
 
 /* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference) ---------------------
  * Each row names its adapter a = adapter_idxs[t]; ids outside [0, n) mean none. Three products make both directions:
- * smoe_adapter_shrink:  H[t, j] = s_a sum_c X[t, c] M[a][j, c]     fp32 (T, r), zero rows without an adapter;
- *     s_a = scaling[a], or `scale` where `scaling` is null. M: lora_a forward, lora_b seen as (n, r, out) backward.
+ * smoe_adapter_shrink:  H[t, j] = s_a sum_c X[t, c] M[a][j, c]     zero rows without an adapter;
+ *     s_a = scaling[a], or `scale` where `scaling` is null. M: lora_a forward, lora_b seen as (n, r, out) backward. H is
+ *     (T, R) contiguous in `dtype`, R = r rounded up to a multiple of 8, the padding written as zeros.
  * smoe_adapter_linear:  Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum_j H[t, j] M[a][j, o]      (bias nullable, contiguous)
- * smoe_adapter_grad:    D[a][j, c] = sum over the rows t of adapter a of U[t, j] V[t, c], U fp32 (T, r), rows listed by
+ * smoe_adapter_grad:    D[a][j, c] = sum over the rows t of adapter a of U[t, j] V[t, c], U as H above, rows listed by
  *     smoe_sort_count of adapter_idxs (sorted_scattered_idxs, expert_offsets); every element of D is written.
  * smoe_column_sum:      out[c] = sum_t V[t, c]   (the bias's gradient). Fixed summation order everywhere.
- * X, Y, V rows have inner stride 1; W, M, D in element strides. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31. */
+ * X, Y, V rows have inner stride 1; W, M, D in element strides. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31. Workspaces (16-byte
+ * aligned, sized by the queries) belong to the call until its work has finished. */
 int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma, int64_t stride_mj,
-                        int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling, float scale, float* H, int32_t n,
+                        int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling, float scale, void* H, int32_t n,
                         int32_t C, int32_t r, int32_t dtype, void* stream);
 int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk, int64_t stride_wn,
-                        const void* bias, const float* H, const void* M, int64_t stride_ma, int64_t stride_mj,
+                        const void* bias, const void* H, const void* M, int64_t stride_ma, int64_t stride_mj,
                         int64_t stride_mo, const int64_t* adapter_idxs, void* Y, int64_t stride_ym, int32_t n, int32_t C,
                         int32_t O, int32_t r, int32_t dtype, int32_t* status, void* stream);
-int smoe_adapter_grad(const float* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
+size_t smoe_adapter_grad_workspace_bytes(int64_t T, int32_t C, int32_t r);
+int smoe_adapter_grad(const void* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
                       const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc, int32_t n,
-                      int32_t C, int32_t r, int32_t dtype, void* stream);
+                      int32_t C, int32_t r, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
 size_t smoe_column_sum_workspace_bytes(int64_t T, int32_t C);
 int smoe_column_sum(const void* V, int64_t T, int64_t stride_vm, int32_t C, void* out, int32_t dtype, void* workspace,
                     size_t workspace_bytes, void* stream);

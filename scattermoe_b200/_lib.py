@@ -104,7 +104,8 @@ SIGNATURES = {
     "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P], c_int32),
     "smoe_adapter_linear": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32,
                              _I32, _P, _P], c_int32),
-    "smoe_adapter_grad": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P], c_int32),
+    "smoe_adapter_grad_workspace_bytes": ([_I64, _I32, _I32], c_size_t),
+    "smoe_adapter_grad": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, c_size_t, _P], c_int32),
     "smoe_column_sum_workspace_bytes": ([_I64, _I32], c_size_t),
     "smoe_column_sum": ([_P, _I64, _I64, _I32, _P, _I32, _P, c_size_t, _P], c_int32),
 }

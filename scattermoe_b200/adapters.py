@@ -6,7 +6,7 @@
 batch mixes the tokens of many requests, each with an adapter of its own or none (an id outside [0, n): y = W x + b).
 The ids may be in any order; tokens of one request usually stand together, which the kernels use and do not need.
 
-Two launches forward: the shrink into the rank (h = s A x, fp32 rows) and the shared product, whose accumulators take up
+Two launches forward: the shrink into the rank (h = s A x; in 16 bits rounded once, as the tensor cores take it) and the shared product, whose accumulators take up
 B h before they are rounded once: the adapted output is never read back. Backward mirrors it (g = s B^T dy, then
 dx = W^T dy + A^T g in one launch) and sums the outer products dA_a = sum g x^T, dB_a = sum dy h^T per adapter in a fixed
 order. Gradients nobody asked for are not computed; adapters without rows get zeros; `scaling` is a constant.
@@ -27,11 +27,15 @@ MAX_RANK = 256
 MAX_ADAPTERS = 4096
 
 
+def _padded(r: int) -> int:
+    return (r + 7) // 8 * 8
+
+
 def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float) -> torch.Tensor:
-    """h[t, j] = s sum_c x[t, c] m[ids[t], j, c], fp32 (T, r); zero rows for ids outside [0, n)."""
+    """h[t, j] = s sum_c x[t, c] m[ids[t], j, c], (T, r padded to a multiple of 8); zero rows for ids outside [0, n)."""
     T = x.size(0)
     n, r, C = m.shape
-    h = torch.empty((T, r), dtype=torch.float32, device=x.device)
+    h = torch.empty((T, _padded(r)), dtype=x.dtype, device=x.device)
     with torch.cuda.device(x.device):
         rc = _lib.load().smoe_adapter_shrink(
             x.data_ptr(), T, x.stride(0), m.data_ptr(), m.stride(0), m.stride(1), m.stride(2), ids.data_ptr(),
@@ -57,16 +61,20 @@ def _linear_impl(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     return y
 
 
-def _grad_impl(u: torch.Tensor, v: torch.Tensor, sorted_idx: torch.Tensor, offsets: torch.Tensor,
+def _grad_impl(u: torch.Tensor, v: torch.Tensor, r: int, sorted_idx: torch.Tensor, offsets: torch.Tensor,
                transposed: bool) -> torch.Tensor:
-    """d[a] = sum over the rows t of adapter a of u[t]^T v[t]: (n, r, C), or its transpose (n, C, r)."""
-    n, r, C = offsets.size(0), u.size(1), v.size(1)
+    """d[a] = sum over the rows t of adapter a of u[t, :r]^T v[t]: (n, r, C), or its transpose (n, C, r)."""
+    n, C = offsets.size(0), v.size(1)
+    lib = _lib.load()
+    ws_bytes = lib.smoe_adapter_grad_workspace_bytes(u.size(0), C, r)
+    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=v.device)
     d = torch.empty((n, C, r) if transposed else (n, r, C), dtype=v.dtype, device=v.device)
     view = d.transpose(1, 2) if transposed else d
     with torch.cuda.device(v.device):
-        rc = _lib.load().smoe_adapter_grad(
+        rc = lib.smoe_adapter_grad(
             u.data_ptr(), u.size(0), v.data_ptr(), v.stride(0), sorted_idx.data_ptr(), offsets.data_ptr(), d.data_ptr(),
-            view.stride(0), view.stride(1), view.stride(2), n, C, r, _lib.DTYPE_CODE[v.dtype], _lib.stream_ptr(v.device))
+            view.stride(0), view.stride(1), view.stride(2), n, C, r, _lib.DTYPE_CODE[v.dtype], ws.data_ptr(), ws_bytes,
+            _lib.stream_ptr(v.device))
     _lib.check(rc, "smoe_adapter_grad")
     return d
 
@@ -93,7 +101,7 @@ def shrink_compileable(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scal
 
 @shrink_compileable.register_fake
 def _(x, m, ids, scaling, scale):
-    return torch.empty((x.size(0), m.size(1)), dtype=torch.float32, device=x.device)
+    return torch.empty((x.size(0), _padded(m.size(1))), dtype=x.dtype, device=x.device)
 
 
 @torch.library.custom_op("scattermoe_b200::adapter_linear", mutates_args={})
@@ -108,14 +116,14 @@ def _(x, w, bias, h, m, ids):
 
 
 @torch.library.custom_op("scattermoe_b200::adapter_grad", mutates_args={})
-def grad_compileable(u: torch.Tensor, v: torch.Tensor, sorted_idx: torch.Tensor, offsets: torch.Tensor,
+def grad_compileable(u: torch.Tensor, v: torch.Tensor, r: int, sorted_idx: torch.Tensor, offsets: torch.Tensor,
                      transposed: bool) -> torch.Tensor:
-    return _grad_impl(u, v, sorted_idx, offsets, transposed)
+    return _grad_impl(u, v, r, sorted_idx, offsets, transposed)
 
 
 @grad_compileable.register_fake
-def _(u, v, sorted_idx, offsets, transposed):
-    n, r, C = offsets.size(0), u.size(1), v.size(1)
+def _(u, v, r, sorted_idx, offsets, transposed):
+    n, C = offsets.size(0), v.size(1)
     return torch.empty((n, C, r) if transposed else (n, r, C), dtype=v.dtype, device=v.device)
 
 
@@ -161,9 +169,9 @@ class AdapterLinear_(torch.autograd.Function):
             _, sorted_idx, offsets = flatten_sort_count(ids, lora_a.size(0))
             grad = _pick(grad_compileable, _grad_impl)
             if need_a:
-                d_a = grad(g, x, sorted_idx, offsets, False)
+                d_a = grad(g, x, lora_a.size(1), sorted_idx, offsets, False)
             if need_b:
-                d_b = grad(h, dy, sorted_idx, offsets, True)
+                d_b = grad(h, dy, lora_a.size(1), sorted_idx, offsets, True)
         if need_w:
             rows = torch.full((1,), x.size(0), dtype=torch.int64, device=x.device)
             d_w, db = kernels.ops.group_bwd_W(DY=dy, X=x, expert_offsets=rows, E=1, has_bias=need_bias)

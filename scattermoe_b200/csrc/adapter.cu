@@ -4,12 +4,25 @@
 namespace smoe {
 namespace ad {
 
-// ---- shrink: a warp per (token, 4 rank rows), lanes over the contracted axis -------------------------------
-template <typename T>
+// V consecutive values as floats: one 16-byte load, or one value
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T* p, float (&out)[V]) {
+  if (V == 1) {
+    out[0] = to_f32<T>(__ldg(p));
+  } else {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
+    const T* t = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = to_f32<T>(t[i]);
+  }
+}
+
+// ---- shrink: a warp per (token, 4 rank rows), lanes over the contracted axis, V values at a time -----------------
+template <typename T, int V>
 __global__ void __launch_bounds__(256)
 shrink_simt_kernel(const ShrinkArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int blocks = (a.r + 3) / 4;
+  const int blocks = static_cast<int>(rank_pitch(a.r) / 4);
   const int64_t total = a.T * blocks;
   for (int64_t it = static_cast<int64_t>(blockIdx.x) * 8 + warp; it < total; it += static_cast<int64_t>(gridDim.x) * 8) {
     const int64_t t = it / blocks;
@@ -21,19 +34,26 @@ shrink_simt_kernel(const ShrinkArgs a) {
       s = a.scaling ? a.scaling[id] : a.scale;
       const T* x = static_cast<const T*>(a.X) + t * a.sxm;
       const T* m = static_cast<const T*>(a.M) + id * a.sma;
-      for (int c = lane; c < a.C; c += 32) {
-        const float xv = to_f32<T>(__ldg(x + c));
+#pragma unroll 2
+      for (int c = lane * V; c < a.C; c += 32 * V) {       // V > 1: contiguous and aligned, C a multiple of V
+        float xv[V];
+        load_values<T, V>(x + c, xv);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (j0 + i < a.r) acc[i] = fmaf(xv, to_f32<T>(__ldg(m + (j0 + i) * a.smj + c * a.smc)), acc[i]);
+          if (j0 + i < a.r) {
+            float mv[V];
+            load_values<T, V>(m + (j0 + i) * a.smj + c * a.smc, mv);
+#pragma unroll
+            for (int v = 0; v < V; ++v) acc[i] = fmaf(xv[v], mv[v], acc[i]);
+          }
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-      // an adapter that is not there leaves a zero row, whatever the inputs hold
-      if (lane == 0 && j0 + i < a.r) a.H[t * a.r + j0 + i] = (id >= 0 && id < a.n) ? acc[i] * s : 0.f;
+      // an adapter that is not there leaves a zero row, whatever the inputs hold; so does the padding
+      if (lane == 0) static_cast<T*>(a.H)[t * rank_pitch(a.r) + j0 + i] = from_f32<T>((id >= 0 && id < a.n && j0 + i < a.r) ? acc[i] * s : 0.f);
     }
   }
 }
@@ -89,9 +109,9 @@ linear_simt_kernel(const LinearArgs a) {
     const int64_t id = a.ids[t];
     if (id >= 0 && id < a.n) {
       const T* m = static_cast<const T*>(a.M) + id * a.sma;
-      const float* h = a.H + t * a.r;
+      const T* h = static_cast<const T*>(a.H) + t * rank_pitch(a.r);
       for (int jj = 0; jj < a.r; ++jj) {
-        const float hv = h[jj];
+        const float hv = to_f32<T>(h[jj]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int o = o0 + tx * 4 + j;
@@ -126,7 +146,7 @@ grad_simt_kernel(const GradArgs a) {
     __syncthreads();
     for (int i = tid; i < 32 * 16; i += 256) {
       const int m = i >> 4, j = i & 15;
-      us[m][j] = (m < cnt && j0 + j < a.r) ? a.U[rows[m] * a.r + j0 + j] : 0.f;
+      us[m][j] = (m < cnt && j0 + j < a.r) ? to_f32<T>(static_cast<const T*>(a.U)[rows[m] * rank_pitch(a.r) + j0 + j]) : 0.f;
     }
     for (int i = tid; i < 32 * 64; i += 256) {
       const int m = i >> 6, c = i & 63;
@@ -156,9 +176,13 @@ grad_simt_kernel(const GradArgs a) {
   }
 
 int launch_shrink_simt(const ShrinkArgs& a) {
-  const int64_t warps = a.T * cdiv(a.r, 4);
+  const int64_t warps = a.T * (rank_pitch(a.r) / 4);
   const int grid = static_cast<int>(min(cdiv64(warps, 8), static_cast<int64_t>(148 * 32)));
-  SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_><<<grid, 256, 0, a.stream>>>(a);)
+  const int v = 16 / dtype_size(a.dtype);
+  auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
+  const bool vec = a.smc == 1 && a.C % v == 0 && a.sxm % v == 0 && a.smj % v == 0 && a.sma % v == 0 && al16(a.X) && al16(a.M);
+  if (vec) SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 16 / sizeof(T_)><<<grid, 256, 0, a.stream>>>(a);)
+  else SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 1><<<grid, 256, 0, a.stream>>>(a);)
   SMOE_LAUNCH_CHECK();
   return SMOE_OK;
 }
@@ -171,7 +195,7 @@ int launch_linear_simt(const LinearArgs& a) {
     const int es = dtype_size(a.dtype);
     b.X = static_cast<const uint8_t*>(a.X) + t0 * a.sxm * es;
     b.Y = static_cast<uint8_t*>(a.Y) + t0 * a.sym * es;
-    b.H = a.H + t0 * a.r;
+    b.H = static_cast<const uint8_t*>(a.H) + t0 * rank_pitch(a.r) * es;
     b.ids = a.ids + t0;
     b.T = a.T - t0 < slice ? a.T - t0 : slice;
     dim3 grid(static_cast<unsigned>(cdiv(a.O, TN)), static_cast<unsigned>(cdiv64(b.T, TM)));
@@ -204,17 +228,18 @@ using namespace smoe;
 
 extern "C" int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma,
                                    int64_t stride_mj, int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling,
-                                   float scale, float* H, int32_t n, int32_t C, int32_t r, int32_t dtype, void* stream) {
+                                   float scale, void* H, int32_t n, int32_t C, int32_t r, int32_t dtype, void* stream) {
   if (int rc = ad::check_common("adapter_shrink", T, n, C, r, dtype)) return rc;
   if (T == 0) return SMOE_OK;
   SMOE_CHECK_ARG(X && M && adapter_idxs && H, "adapter_shrink: null pointer");
   ad::ShrinkArgs a{X, T, stride_xm, M, stride_ma, stride_mj, stride_mc, adapter_idxs, scaling, scale, H, n, C, r, dtype,
                    static_cast<cudaStream_t>(stream)};
-  return ad::launch_shrink_simt(a);
+  const int rc = ad::launch_shrink_tc(a);
+  return rc != SMOE_ERR_UNSUPPORTED ? rc : ad::launch_shrink_simt(a);
 }
 
 extern "C" int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk,
-                                   int64_t stride_wn, const void* bias, const float* H, const void* M, int64_t stride_ma,
+                                   int64_t stride_wn, const void* bias, const void* H, const void* M, int64_t stride_ma,
                                    int64_t stride_mj, int64_t stride_mo, const int64_t* adapter_idxs, void* Y,
                                    int64_t stride_ym, int32_t n, int32_t C, int32_t O, int32_t r, int32_t dtype,
                                    int32_t* status, void* stream) {
@@ -224,17 +249,34 @@ extern "C" int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, 
   SMOE_CHECK_ARG(X && W && H && M && adapter_idxs && Y, "adapter_linear: null pointer");
   ad::LinearArgs a{X, T, stride_xm, W, stride_wk, stride_wn, bias, H, M, stride_ma, stride_mj, stride_mo, adapter_idxs, Y,
                    stride_ym, n, C, O, r, dtype, status, static_cast<cudaStream_t>(stream)};
+  const int rc = ad::launch_linear_tc(a);
+  if (rc != SMOE_ERR_UNSUPPORTED) {
+    if (rc == SMOE_OK) set_last_path(1);
+    return rc;
+  }
+  set_last_path(0);
   return ad::launch_linear_simt(a);
 }
 
-extern "C" int smoe_adapter_grad(const float* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
+extern "C" size_t smoe_adapter_grad_workspace_bytes(int64_t T, int32_t C, int32_t r) {
+  if (T < 0 || C < 1 || r < 1) return 0;
+  return ad::grad_workspace_bytes(T, C, r);
+}
+
+extern "C" int smoe_adapter_grad(const void* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
                                  const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc,
-                                 int32_t n, int32_t C, int32_t r, int32_t dtype, void* stream) {
+                                 int32_t n, int32_t C, int32_t r, int32_t dtype, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
   if (int rc = ad::check_common("adapter_grad", T, n, C, r, dtype)) return rc;
   SMOE_CHECK_ARG(D && offsets && (T == 0 || (U && V && sorted_idx)), "adapter_grad: null pointer");
+  if (workspace == nullptr || workspace_bytes < smoe_adapter_grad_workspace_bytes(T, C, r)) {
+    set_error("adapter_grad: workspace of %zu bytes needed, %zu given", smoe_adapter_grad_workspace_bytes(T, C, r), workspace_bytes);
+    return SMOE_ERR_WORKSPACE;
+  }
   ad::GradArgs a{U, T, V, stride_vm, sorted_idx, offsets, D, stride_da, stride_dj, stride_dc, n, C, r, dtype,
-                 static_cast<cudaStream_t>(stream)};
-  return ad::launch_grad_simt(a);
+                 workspace, workspace_bytes, static_cast<cudaStream_t>(stream)};
+  const int rc = ad::launch_grad_tc(a);
+  return rc != SMOE_ERR_UNSUPPORTED ? rc : ad::launch_grad_simt(a);
 }
 
 // ---- column sums (the shared bias's gradient): fp32 partial sums over slices of the rows, added up in order ----

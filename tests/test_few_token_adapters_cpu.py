@@ -50,13 +50,17 @@ def test_adapter_entry_points_refuse(bad, word):
     linear = dict(X=256, T=4, sxm=64, W=256, swk=1, swn=64, bias=None, H=256, M=256, sma=512, smj=1, smo=8, ids=256, Y=256, sym=64,
                   n=2, C=64, O=64, r=8, dtype=1, status=None, stream=None)
     assert lib.smoe_adapter_linear(*{**linear, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
-    grad = dict(U=256, T=4, V=256, svm=64, idx=256, off=256, D=256, sda=512, sdj=64, sdc=1, n=2, C=64, r=8, dtype=1, stream=None)
+    grad = dict(U=256, T=4, V=256, svm=64, idx=256, off=256, D=256, sda=512, sdj=64, sdc=1, n=2, C=64, r=8, dtype=1, ws=256, ws_bytes=1 << 24, stream=None)
     bad = {("V" if k == "X" else k): v for k, v in bad.items()}
     assert lib.smoe_adapter_grad(*{**grad, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
 
 
-def test_column_sum_refuses():
+def test_column_sum_and_gradient_workspaces():
     lib = _lib.load()
+    need = lib.smoe_adapter_grad_workspace_bytes(100, 64, 8)
+    assert need > 0
+    assert lib.smoe_adapter_grad(256, 100, 256, 64, 256, 256, 256, 512, 64, 1, 2, 64, 8, 1, 256, need - 1, None) == 4
+    assert "workspace" in _lib.last_error()
     need = lib.smoe_column_sum_workspace_bytes(100, 64)
     assert need >= 64 * 4
     assert lib.smoe_column_sum(256, 100, 64, 64, 256, 1, 256, need - 1, None) == 4
