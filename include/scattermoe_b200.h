@@ -42,8 +42,10 @@ enum smoe_flags {
   SMOE_FLAG_FORCE_SIMT = 2,   /* take the CUDA-core kernel even where a tensor-core kernel exists */
   SMOE_FLAG_FORCE_TC = 4,     /* fail with SMOE_ERR_UNSUPPORTED instead of taking the CUDA-core kernel */
   SMOE_FLAG_GATHER_ROWS = 8,  /* feed grouped inputs through the row-gather path too (testing / comparison) */
-  SMOE_FLAG_AFTER_ROUTER = 16 /* smoe_few_token_mlp: the call just before on this stream is the smoe_few_token_route that
+  SMOE_FLAG_AFTER_ROUTER = 16, /* smoe_few_token_mlp: the call just before on this stream is the smoe_few_token_route that
                                  writes expert_idxs and gates; the kernels may be scheduled while it still runs */
+  SMOE_FLAG_AFTER_SHRINK = 32 /* smoe_adapter_linear: the call just before on this stream is the smoe_adapter_shrink that
+                                 writes H, and only H comes from it: the kernel may read the rest while it still runs */
 };
 
 int smoe_version(void);
@@ -275,7 +277,7 @@ int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void*
 int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk, int64_t stride_wn,
                         const void* bias, const void* H, const void* M, int64_t stride_ma, int64_t stride_mj,
                         int64_t stride_mo, const int64_t* adapter_idxs, void* Y, int64_t stride_ym, int32_t n, int32_t C,
-                        int32_t O, int32_t r, int32_t dtype, int32_t* status, void* stream);
+                        int32_t O, int32_t r, int32_t dtype, int32_t flags, int32_t* status, void* stream);
 size_t smoe_adapter_grad_workspace_bytes(int64_t T, int32_t C, int32_t r);
 int smoe_adapter_grad(const void* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
                       const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc, int32_t n,

@@ -28,6 +28,7 @@ FLAG_FORCE_SIMT = 2
 FLAG_FORCE_TC = 4
 FLAG_GATHER_ROWS = 8
 FLAG_AFTER_ROUTER = 16
+FLAG_AFTER_SHRINK = 32
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -103,7 +104,7 @@ SIGNATURES = {
     "smoe_few_token_route": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _I32, _P], c_int32),
     "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P], c_int32),
     "smoe_adapter_linear": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32,
-                             _I32, _P, _P], c_int32),
+                             _I32, _I32, _P, _P], c_int32),
     "smoe_adapter_grad_workspace_bytes": ([_I64, _I32, _I32], c_size_t),
     "smoe_adapter_grad": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, c_size_t, _P], c_int32),
     "smoe_column_sum_workspace_bytes": ([_I64, _I32], c_size_t),
@@ -182,6 +183,29 @@ def require_cuda(t: torch.Tensor, name: str):
 
 def stream_ptr(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def path_flags() -> int:
+    """Flags of kernels.ops.FORCE_PATH (a testing hook) for the entry points that choose between two kinds of kernels."""
+    from .kernels import ops
+    return {None: 0, "simt": FLAG_FORCE_SIMT, "tc": FLAG_FORCE_TC}[ops.FORCE_PATH]
+
+
+class on_device_of:
+    """`with torch.cuda.device(t.device)` that does nothing, quickly, where that device is current already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device: torch.device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
 
 
 _status_words = {}

@@ -36,7 +36,7 @@ def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: O
     T = x.size(0)
     n, r, C = m.shape
     h = torch.empty((T, _padded(r)), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device_of(x.device):
         rc = _lib.load().smoe_adapter_shrink(
             x.data_ptr(), T, x.stride(0), m.data_ptr(), m.stride(0), m.stride(1), m.stride(2), ids.data_ptr(),
             scaling.data_ptr() if scaling is not None else None, scale, h.data_ptr(), n, C, r, _lib.DTYPE_CODE[x.dtype],
@@ -46,17 +46,18 @@ def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: O
 
 
 def _linear_impl(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], h: torch.Tensor, m: torch.Tensor,
-                 ids: torch.Tensor) -> torch.Tensor:
+                 ids: torch.Tensor, after_shrink: bool = False) -> torch.Tensor:
     """y = x w + bias + h m[ids]; w is (C, O), m is (n, r, O), any strides."""
     T, C = x.shape
     O = w.size(1)
     n, r, _ = m.shape
     y = torch.empty((T, O), dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device_of(x.device):
         rc = _lib.load().smoe_adapter_linear(
             x.data_ptr(), T, x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), bias.data_ptr() if bias is not None else None,
             h.data_ptr(), m.data_ptr(), m.stride(0), m.stride(1), m.stride(2), ids.data_ptr(), y.data_ptr(), y.stride(0),
-            n, C, O, r, _lib.DTYPE_CODE[x.dtype], _lib.status_word(x.device).data_ptr(), _lib.stream_ptr(x.device))
+            n, C, O, r, _lib.DTYPE_CODE[x.dtype], _lib.path_flags() | (_lib.FLAG_AFTER_SHRINK if after_shrink else 0),
+            _lib.status_word(x.device).data_ptr(), _lib.stream_ptr(x.device))
     _lib.check(rc, "smoe_adapter_linear")
     return y
 
@@ -70,7 +71,7 @@ def _grad_impl(u: torch.Tensor, v: torch.Tensor, r: int, sorted_idx: torch.Tenso
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=v.device)
     d = torch.empty((n, C, r) if transposed else (n, r, C), dtype=v.dtype, device=v.device)
     view = d.transpose(1, 2) if transposed else d
-    with torch.cuda.device(v.device):
+    with _lib.on_device_of(v.device):
         rc = lib.smoe_adapter_grad(
             u.data_ptr(), u.size(0), v.data_ptr(), v.stride(0), sorted_idx.data_ptr(), offsets.data_ptr(), d.data_ptr(),
             view.stride(0), view.stride(1), view.stride(2), n, C, r, _lib.DTYPE_CODE[v.dtype], ws.data_ptr(), ws_bytes,
@@ -85,7 +86,7 @@ def _column_sum_impl(v: torch.Tensor) -> torch.Tensor:
     out = torch.empty((C,), dtype=v.dtype, device=v.device)
     ws_bytes = lib.smoe_column_sum_workspace_bytes(T, C)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=v.device)
-    with torch.cuda.device(v.device):
+    with _lib.on_device_of(v.device):
         rc = lib.smoe_column_sum(v.data_ptr(), T, v.stride(0), C, out.data_ptr(), _lib.DTYPE_CODE[v.dtype], ws.data_ptr(), ws_bytes,
                                  _lib.stream_ptr(v.device))
     _lib.check(rc, "smoe_column_sum")
@@ -141,12 +142,16 @@ def _pick(compiled, direct):
     return compiled if torch.compiler.is_compiling() else direct
 
 
+def _linear(*args, after_shrink):
+    return linear_compileable(*args) if torch.compiler.is_compiling() else _linear_impl(*args, after_shrink=after_shrink)
+
+
 class AdapterLinear_(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, lora_a, lora_b, ids, scaling, scale, bias):
         x = _rowmajor(x)
         h = _pick(shrink_compileable, _shrink_impl)(x, lora_a, ids, scaling, scale)
-        y = _pick(linear_compileable, _linear_impl)(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids)
+        y = _linear(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids, after_shrink=True)
         ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scaling, h)
         ctx.scale = scale
         return y
@@ -164,7 +169,7 @@ class AdapterLinear_(torch.autograd.Function):
         if need_x or need_a:
             g = _pick(shrink_compileable, _shrink_impl)(dy, lora_b.transpose(1, 2), ids, scaling, ctx.scale)
         if need_x:
-            d_x = _pick(linear_compileable, _linear_impl)(dy, weight, None, g, lora_a, ids)
+            d_x = _linear(dy, weight, None, g, lora_a, ids, after_shrink=True)
         if need_a or need_b:
             _, sorted_idx, offsets = flatten_sort_count(ids, lora_a.size(0))
             grad = _pick(grad_compileable, _grad_impl)

@@ -1,6 +1,9 @@
 // Low-rank adapters on CUDA cores (fp32, and 16-bit operands the tensor-core kernels cannot address), and the C entry points.
 #include "adapter.cuh"
 
+#include "act_math.cuh"
+#include "few_token.cuh"
+
 namespace smoe {
 namespace ad {
 
@@ -21,6 +24,7 @@ __device__ __forceinline__ void load_values(const T* p, float (&out)[V]) {
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
 shrink_simt_kernel(const ShrinkArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the linear may start its stream of W
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = static_cast<int>(rank_pitch(a.r) / 4);
   const int64_t total = a.T * blocks;
@@ -212,6 +216,25 @@ int launch_grad_simt(const GradArgs& a) {
   return SMOE_OK;
 }
 
+// Few tokens: the product is a read of W, see few_token.cu.
+static int launch_linear_few(const LinearArgs& a) {
+  if (a.T > FEW_TOKENS || a.sym != a.O) return SMOE_ERR_UNSUPPORTED;
+  ft::Args f = {};
+  f.X = a.X; f.sxm = a.sxm;
+  f.W1 = a.W; f.s1k = a.swk; f.s1n = a.swn;
+  f.B1 = a.bias; f.sb1n = 1;
+  f.T = static_cast<int>(a.T); f.k = 1; f.d = a.C; f.F = a.O; f.d_out = a.O; f.E = 1;
+  f.act_layout = LAYOUT_PLAIN; f.act = ACT_IDENTITY; f.dtype = a.dtype;
+  f.ws = a.Y;
+  f.status = a.status;
+  f.after_router = 0;
+  f.stream = a.stream;
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.M) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.H) & 15) == 0;
+  ft::Extension x{a.H, rank_pitch(a.r), a.M, a.sma, a.smj, a.smo, a.ids, a.n, a.r,
+                  a.smj == 1 && a.smo % 8 == 0 && a.sma % 8 == 0 && a.r % 8 == 0 && aligned ? 1 : 0, a.after_shrink};
+  return ft::launch_linear(f, x);
+}
+
 static int check_common(const char* who, int64_t T, int n, int C, int r, int dtype) {
   SMOE_CHECK_ARG(dtype == SMOE_F32 || dtype == SMOE_BF16 || dtype == SMOE_F16, "%s: unknown dtype %d", who, dtype);
   SMOE_CHECK_ARG(T >= 0 && T < (int64_t(1) << 31), "%s: T=%lld out of range [0, 2^31)", who, (long long)T);
@@ -242,17 +265,24 @@ extern "C" int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, 
                                    int64_t stride_wn, const void* bias, const void* H, const void* M, int64_t stride_ma,
                                    int64_t stride_mj, int64_t stride_mo, const int64_t* adapter_idxs, void* Y,
                                    int64_t stride_ym, int32_t n, int32_t C, int32_t O, int32_t r, int32_t dtype,
-                                   int32_t* status, void* stream) {
+                                   int32_t flags, int32_t* status, void* stream) {
   if (int rc = ad::check_common("adapter_linear", T, n, C, r, dtype)) return rc;
   SMOE_CHECK_ARG(O >= 1 && O < (1 << 28), "adapter_linear: bad width %d", O);
   if (T == 0) return SMOE_OK;
   SMOE_CHECK_ARG(X && W && H && M && adapter_idxs && Y, "adapter_linear: null pointer");
   ad::LinearArgs a{X, T, stride_xm, W, stride_wk, stride_wn, bias, H, M, stride_ma, stride_mj, stride_mo, adapter_idxs, Y,
-                   stride_ym, n, C, O, r, dtype, status, static_cast<cudaStream_t>(stream)};
-  const int rc = ad::launch_linear_tc(a);
-  if (rc != SMOE_ERR_UNSUPPORTED) {
-    if (rc == SMOE_OK) set_last_path(1);
-    return rc;
+                   stride_ym, n, C, O, r, dtype, (flags & SMOE_FLAG_AFTER_SHRINK) ? 1 : 0, status, static_cast<cudaStream_t>(stream)};
+  if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
+    int rc = ad::launch_linear_few(a);
+    if (rc == SMOE_ERR_UNSUPPORTED) rc = ad::launch_linear_tc(a);
+    if (rc != SMOE_ERR_UNSUPPORTED) {
+      if (rc == SMOE_OK) set_last_path(1);
+      return rc;
+    }
+    if (flags & SMOE_FLAG_FORCE_TC) {
+      set_error("adapter_linear: no tensor-core kernel for this dtype/alignment (dtype=%d in=%d out=%d)", dtype, C, O);
+      return rc;
+    }
   }
   set_last_path(0);
   return ad::launch_linear_simt(a);

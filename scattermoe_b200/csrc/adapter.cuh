@@ -15,6 +15,7 @@ namespace smoe {
 namespace ad {
 
 constexpr int MAX_RANK = 256;
+constexpr int FEW_TOKENS = 128;      // up to here the product is a read of W (few_token.cu)
 constexpr int64_t rank_pitch(int r) { return (r + 7) / 8 * 8; }
 
 struct ShrinkArgs {           // H[t, j] = s_a sum_c X[t, c] M[a][j, c]
@@ -36,6 +37,7 @@ struct LinearArgs {           // Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum
   const int64_t* ids;
   void* Y; int64_t sym;
   int n, C, O, r, dtype;
+  int after_shrink;         // the launch before on this stream is the shrink that writes H
   int32_t* status;
   cudaStream_t stream;
 };

@@ -11,7 +11,8 @@
 //
 //   up    A round is up to 8 tiles of one job, a tile 32 weight rows: 16 hidden values with their two columns, or 32 without a gate. Each
 //         warp owns a tile over the whole of K and makes its hidden values in registers: no exchange between warps, no barrier; the
-//         slots' rows are fetched once per round.
+//         slots' rows are fetched once per round. A round of few tiles gives each tile 2, 4 or 8 warps, which split the steps of K
+//         and are joined through shared memory.
 //   down  The block's output columns are one tile. Pairs of warps take the stages in turn, so that four jobs are under way at once, and
 //         add their part of a job to token sums of their own in shared memory, joined in order once at the end. The two warps of a pair
 //         hold 16 columns each, or half of K each where the tile has no more than 16.
@@ -70,7 +71,8 @@ struct StreamParams {
   int NT;                     // slots of a job
   int K, blocks;              // K and its boxes
   int box_bytes, load_bytes;  // bytes a box takes in the ring, and bytes it loads
-  int steps_of[4];            // steps of K of a stage for a job of 1-8, 9-16, 17-24, 25-32 slots (up: with one tile)
+  int steps_of[4][4];         // steps of K of a stage: 1, 2, 3-4, 5-8 boxes wide x a job of 1-8, 9-16, 17-24, 25-32 slots
+  Extension ext;              // up: added to the values before they are rounded (adapter_linear)
   int stages, stage_bytes, ring_bytes;
   int rows;                   // down: rows of a tile's token sums (the tile's columns)
 };
@@ -214,9 +216,8 @@ struct Walker {
 template <bool UP, bool KMAJOR>
 __device__ __forceinline__ void shape_of(const StreamParams& p, Run& r, int n) {
   r.groups = (n + 7) >> 3;
-  r.nb = p.steps_of[r.groups - 1];
-  if (UP && r.tiles > 1) r.nb = min(r.nb, r.tiles == 2 ? 4 : (r.tiles <= 4 ? 2 : 1));
   r.boxes = KMAJOR ? r.tiles : (r.tiles + 1) >> 1;
+  r.nb = p.steps_of[r.boxes <= 2 ? r.boxes - 1 : (r.boxes <= 4 ? 2 : 3)][r.groups - 1];
   r.x_offset = r.boxes * r.nb * p.box_bytes;
 }
 
@@ -231,6 +232,28 @@ __device__ __forceinline__ float hidden_fast(int layout, int act, float alpha, f
   float r;
   SMOE_ACT_SWITCH(act, r = act_fwd<ACT_, true>(gate);)
   return r * lin;
+}
+
+// What row t's adapter adds to column o.
+template <typename T>
+__device__ __forceinline__ float extension_term(const Extension& x, int t, int o) {
+  const int64_t id = x.ids[t];
+  if (id < 0 || id >= x.n) return 0.f;
+  const T* h = static_cast<const T*>(x.h) + t * x.h_pitch;
+  const T* m = static_cast<const T*>(x.m) + id * x.sma + o * x.smo;
+  float sum = 0.f;
+  if (x.m_vec) {
+#pragma unroll 2
+    for (int j = 0; j < x.r; j += 8) {
+      const uint4 hv = __ldg(reinterpret_cast<const uint4*>(h + j)), mv = __ldg(reinterpret_cast<const uint4*>(m + j));
+      const T *ht = reinterpret_cast<const T*>(&hv), *mt = reinterpret_cast<const T*>(&mv);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(to_f32<T>(ht[i]), to_f32<T>(mt[i]), sum);
+    }
+  } else {
+    for (int j = 0; j < x.r; ++j) sum = fmaf(to_f32<T>(h[j]), to_f32<T>(__ldg(m + j * x.smj)), sum);
+  }
+  return sum;
 }
 
 template <typename T, bool UP, bool KMAJOR>
@@ -263,7 +286,8 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     tma_prefetch_desc(&tmap);
   }
   if (UP) {
-    wait_for_previous_kernel();        // ids, gates (and everything else) come from it when it is the router
+    // ids and gates come from the kernel before when it is the router; an adapter's shrink only from there on (see below)
+    if (!p.ext.ids) wait_for_previous_kernel();
     let_next_kernel_start();
     if (blockIdx.x == 0)
       for (int i = tid; i < p.n_counters; i += THREADS) p.counters[i] = 0;
@@ -397,10 +421,10 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
       w_lane = (row + m0) * 128 + (((lane >> 4) ^ (row & 7)) << 4);
       w_lane1 = w_lane + 16 * 128;
     } else if (halves) {      // 64-byte rows, the warp's 16 columns of either half
-      w_lane = krow * 64 + (((chunk + (warp & 1) * 2) ^ ((krow >> 1) & 3)) << 4);
+      w_lane = krow * 64 + ((chunk ^ ((krow >> 1) & 3)) << 4);
       w_lane1 = w_lane + 4096;
     } else {                  // 128-byte rows, the warp's 32 columns
-      w_lane = krow * 128 + (((chunk + (warp & 1) * 4) ^ (krow & 7)) << 4);
+      w_lane = krow * 128 + (((chunk + (UP ? 0 : (warp & 1) * 4)) ^ (krow & 7)) << 4);
       w_lane1 = w_lane ^ 32;
     }
     x1_lane = (lane & 7) * 128 + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
@@ -411,9 +435,12 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     const int n = plan->job_count[r.job], beg = plan->job_begin[r.job], e = plan->job_expert[r.job];
     shape_of<UP, KMAJOR>(p, r, n);
     const int groups = r.groups, x_block = groups * 1024;
-    // the warp's weight rows: up, tile `warp` of the round; down, its part of the one tile
-    const int v0 = UP ? r.p0 + warp * walk.per_tile : r.p0;
-    const int count = UP ? min(walk.per_tile, r.count - warp * walk.per_tile) : r.count;
+    // the warp's weight rows: up, a tile of the round (shared by `team` warps); down, its part of the one tile
+    const int team = UP ? (r.tiles == 1 ? 8 : (r.tiles == 2 ? 4 : (r.tiles <= 4 ? 2 : 1))) : 1;
+    const int tl = UP ? warp / team : 0, sub = UP ? warp - tl * team : 0;
+    const int v0 = UP ? r.p0 + tl * walk.per_tile : r.p0;
+    const int count = UP ? min(walk.per_tile, r.count - tl * walk.per_tile) : r.count;
+    const uint32_t second_tile = UP && !KMAJOR ? (tl & 1) << (halves ? 5 : 6) : 0;       // N-major: which half of the box
     const bool use0 = count > m0, use1 = UP ? (pairs ? (woven && !KMAJOR ? count > 8 : use0) : count > 16) : count > m0 + 16;
     if (!UP && r.first && (!by_columns || !(warp & 1))) {
       for (int i = lane; i < a.T * pitch; i += 32) sums[copy * a.T * pitch + i] = 0.f;
@@ -442,15 +469,15 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
         if (ok) ok = mbar_wait_warp(full_bar(s), at.phase, abort_flag, p.status, 22);
         if (ok && use0) {
           const int steps = min(r.nb, r.b1 - b);
-          uint32_t w = ring0 + s * p.stage_bytes + (UP ? (KMAJOR ? warp : warp >> 1) * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
+          uint32_t w = ring0 + s * p.stage_bytes + (UP ? (KMAJOR ? tl : tl >> 1) * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
           auto step = [&](int i, float (&to)[M][G][4]) {       // the i-th 16 of K of a box
             uint32_t a0[4], a1[4], bx[G + 1][2];
             if (KMAJOR) {
               ldsm4(a0, w + (w_lane ^ (i << 5)));
               if (M == 2 && use1) ldsm4(a1, w + (w_lane1 ^ (i << 5)));
             } else {
-              ldsm4_trans(a0, w + w_lane + i * w_step);
-              if (M == 2 && use1) ldsm4_trans(a1, w + w_lane1 + i * w_step);
+              ldsm4_trans(a0, w + (w_lane ^ second_tile) + i * w_step);
+              if (M == 2 && use1) ldsm4_trans(a1, w + (w_lane1 ^ second_tile) + i * w_step);
             }
             if (G == 1) {
               ldsm2(bx[0][0], bx[0][1], x + (x1_lane ^ (i << 5)));
@@ -469,7 +496,9 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
             }
           };
           if (UP || by_columns) {
-            for (int i = 0; i < steps; ++i, w += p.box_bytes, x += x_block) {
+            w += sub * p.box_bytes;
+            x += sub * x_block;
+            for (int i = sub; i < steps; i += team, w += team * p.box_bytes, x += team * x_block) {
 #pragma unroll
               for (int q = 0; q < 4; ++q) step(q, part[q % S]);
             }
@@ -506,13 +535,41 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     else if (groups == 3) stream(std::integral_constant<int, 3>{});
     else stream(std::integral_constant<int, 4>{});
 
+    if (UP && team > 1) {
+      // the warps of a tile put their parts side by side; each then takes every team-th value of all
+      float* red = sums + MAX_R;
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (g < groups) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) red[(warp * 32 + (m * 4 + g) * 4 + q) * 32 + lane] = acc[m][g][q];
+          }
+      consumers_sync();
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (g < groups && (g * 4 + q) % team == sub) {
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+              float v = 0.f;
+              for (int w = 0; w < team; ++w) v += red[((tl * team + w) * 32 + (m * 4 + g) * 4 + q) * 32 + lane];
+              acc[m][g][q] = v;
+            }
+          }
+      consumers_sync();
+    }
     if (UP) {
+      if (p.ext.ids) wait_for_previous_kernel();      // the rank rows of the extension
       // accumulator q of group g: slot g*8 + 2*(lane & 3) + (q & 1), weight row (lane >> 2) + 8*(q >> 1) of each 16-row half
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         if (g >= groups || !use0) continue;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+          if (team > 1 && (g * 4 + q) % team != sub) continue;
           const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
           float c[2][2] = {{acc[0][g][q], acc[M - 1][g][q]}, {0.f, 0.f}};       // (first, second column) of up to two values
           int v[2] = {row, -1};
@@ -538,6 +595,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
               c0 += to_f32<T>(bias[(woven ? 2 * pv : pv) * a.sb1n]);
               if (pairs) c1 += to_f32<T>(bias[(woven ? 2 * pv + 1 : a.F + pv) * a.sb1n]);
             }
+            if (p.ext.ids) c0 += extension_term<T>(p.ext, slot, pv);
             reinterpret_cast<T*>(p.hidden)[static_cast<int64_t>(slot) * a.F + pv] =
                 from_f32<T>(gate * hidden_fast(a.act_layout, a.act, a.alpha, a.limit, c0, c1));
           }
@@ -695,7 +753,7 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   p.rows = UP ? 0 : (KMAJOR ? down_rows(a.d_out, grid) : 2 * TILE);
   // shared memory that is not the ring
   const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 +
-                    (UP ? MAX_R * 4 : (p.rows > 16 ? CONSUMERS / 2 : CONSUMERS) * a.T * (p.rows + 1) * 4) + 1024 + 64;
+                    (UP ? MAX_R * 4 + CONSUMERS * 32 * 32 * 4 : (p.rows > 16 ? CONSUMERS / 2 : CONSUMERS) * a.T * (p.rows + 1) * 4) + 1024 + 64;
   const int budget = (di.max_smem_optin < 232448 ? di.max_smem_optin : 232448) - fixed;
   const int rows = KMAJOR ? (UP ? TILE : p.rows) : 2 * TILE;
   p.load_bytes = rows * BLOCK_K * 2;
@@ -714,16 +772,17 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   p.stages = (budget - slack) / p.stage_bytes;
   p.stages = (p.stages > MAX_STAGES ? MAX_STAGES : p.stages) / TURNS * TURNS;
   if (p.stages < TURNS) return SMOE_ERR_UNSUPPORTED;
-  for (int g = 0; g < 4; ++g) {
-    int steps = p.stage_bytes / (p.box_bytes + (g + 1) * 1024);
-    if (UP && steps > 32768 / p.box_bytes) steps = 32768 / p.box_bytes;      // more tiles: fewer steps, never more than 32 KB of weights
-    if (steps < 1) {
-      if (g < most_groups) return SMOE_ERR_UNSUPPORTED;
-      steps = 1;
+  for (int c = 0; c < 4; ++c)
+    for (int g = 0; g < 4; ++g) {
+      const int boxes = 1 << c;      // the most of their class; never more than 32 KB of weights in the up-projection's rounds
+      int steps = p.stage_bytes / (boxes * p.box_bytes + (g + 1) * 1024);
+      if (UP && steps > 32768 / (boxes * p.box_bytes)) steps = 32768 / (boxes * p.box_bytes);
+      if (steps < 1) {
+        if (g < most_groups && boxes * p.box_bytes <= (UP ? 32768 : p.box_bytes)) return SMOE_ERR_UNSUPPORTED;
+        steps = 1;                   // never asked for
+      }
+      p.steps_of[c][g] = cdiv(p.blocks, cdiv(p.blocks, steps));
     }
-    p.steps_of[g] = cdiv(p.blocks, cdiv(p.blocks, steps));
-  }
-  if (UP && p.stage_bytes < 48 * 1024) return SMOE_ERR_UNSUPPORTED;      // two tiles, four steps, 32 slots
   p.ring_bytes = p.stages * p.stage_bytes + slack;
   const int scratch = (plan_scratch_bytes(a.E) + 15) / 16 * 16;      // the plan sorts in the ring before the first copy
   if (scratch > budget) return SMOE_ERR_UNSUPPORTED;
@@ -747,7 +806,7 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (!UP || a.after_router) ? 1 : 0;
+  cfg.numAttrs = (!UP || a.after_router || p.ext.after_shrink) ? 1 : 0;
   SMOE_CUDA(cudaLaunchKernelEx(&cfg, ft_stream_kernel<T, UP, KMAJOR>, map, p));
   return SMOE_OK;
 }
@@ -760,6 +819,7 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
   const bool bf16 = a.dtype == SMOE_BF16;
   StreamParams p;
   p.a = a;
+  memset(&p.ext, 0, sizeof(p.ext));
   p.hidden = static_cast<uint8_t*>(a.ws);
   uint8_t* after = static_cast<uint8_t*>(a.ws) + hidden_bytes(a.T, a.k, a.F);
   p.n_counters = column_tiles(a.d_out);
@@ -783,6 +843,41 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
   if (int rc = o1.k_major ? launch_one<T, true, true>(p, m1, di, grid) : launch_one<T, true, false>(p, m1, di, grid)) return rc;
   p.K = a.F;
   return o2.k_major ? launch_one<T, false, true>(p, m2, di, grid) : launch_one<T, false, false>(p, m2, di, grid);
+}
+
+// The up-projection kernel as a linear of a few tokens (one expert, no activation) whose values take up an adapter's term. `ws` is the
+// result (T, F), contiguous.
+template <typename T>
+static int launch_linear_typed(const Args& a, const Extension& ext, const DeviceInfo& di) {
+  const Order o = weight_order(a.W1, 0, a.s1k, a.s1n, a.d, a.F);
+  if (!o.k_major && !o.n_major) return SMOE_ERR_UNSUPPORTED;
+  const bool bf16 = a.dtype == SMOE_BF16;
+  StreamParams p;
+  p.a = a;
+  p.ext = ext;
+  p.hidden = static_cast<uint8_t*>(a.ws);
+  p.partial = nullptr;
+  p.counters = nullptr;
+  p.n_counters = 0;
+  p.status = a.status;
+  p.NT = 32;
+  const int grid = di.sm_count < MAX_CTAS ? di.sm_count : MAX_CTAS;
+  p.part_step = static_cast<uint32_t>(((1ull << 32) + grid - 1) / grid);
+  p.K = a.d;
+  CUtensorMap map;
+  const bool ok = o.k_major ? encode_k_major(&map, bf16, a.W1, a.d, a.F, a.s1n, 1, 0, 1, 0, TILE)
+                            : encode_n_major(&map, bf16, a.W1, a.F, a.d, a.s1k, 1, 1, 0);
+  if (!ok) return SMOE_ERR_UNSUPPORTED;
+  return o.k_major ? launch_one<T, true, true>(p, map, di, grid) : launch_one<T, true, false>(p, map, di, grid);
+}
+
+int launch_linear(const Args& a, const Extension& ext) {
+  if ((a.dtype != SMOE_BF16 && a.dtype != SMOE_F16) || a.T > MAX_T) return SMOE_ERR_UNSUPPORTED;
+  if (a.d % 8 || a.sxm % 8 || !al16(a.X) || static_cast<int64_t>(a.T) * cdiv(a.F, TILE) >= (int64_t(1) << 30)) return SMOE_ERR_UNSUPPORTED;
+  DeviceInfo di;
+  if (int rc = get_device_info(&di)) return rc;
+  if (di.cc_major != 10) return SMOE_ERR_UNSUPPORTED;
+  return a.dtype == SMOE_BF16 ? launch_linear_typed<__nv_bfloat16>(a, ext, di) : launch_linear_typed<__half>(a, ext, di);
 }
 
 int launch_stream(const Args& a) {

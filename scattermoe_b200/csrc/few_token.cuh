@@ -34,6 +34,15 @@ struct Args {
   cudaStream_t stream;
 };
 
+// What an adapter adds to the values of a plain linear (adapter.cuh): sum over j of h[t, j] m[ids[t]][j, o].
+struct Extension {
+  const void* h; int64_t h_pitch;
+  const void* m; int64_t sma, smj, smo;
+  const int64_t* ids;      // null: nothing is added
+  int n, r, m_vec;
+  int after_shrink;        // the launch before on this stream writes h, and nothing else that is read here
+};
+
 inline int n_up(const Args& a) { return a.act_layout == 0 ? a.F : 2 * a.F; }
 
 // CUDA-core kernels: fp32, and 16-bit operands the streaming kernels cannot address (any strides, any sizes).
@@ -41,6 +50,7 @@ int launch_simt(const Args& a);
 size_t simt_workspace_bytes(int64_t T, int k, int F, int d_out);
 // Streaming tensor-core kernels; SMOE_ERR_UNSUPPORTED (no error text) when the operands do not fit them.
 int launch_stream(const Args& a);
+int launch_linear(const Args& a, const Extension& ext);
 size_t stream_workspace_bytes(int64_t T, int k, int F, int d_out);
 
 // ---- plan --------------------------------------------------------------------------------------------
@@ -56,7 +66,8 @@ struct alignas(16) Plan {
 // Bytes of scratch `make_plan` needs (dead afterwards): per-warp histograms and one packed prefix per expert.
 __host__ __device__ inline int plan_scratch_bytes(int E) { return PLAN_WARPS * E * 2 + E * 4 + 16; }
 
-// Whole-block call (at least PLAN_WARPS warps). Ids outside [0, E) belong to no job. Ends with a barrier.
+// Whole-block call (at least PLAN_WARPS warps). Ids outside [0, E) belong to no job; without `ids` every slot is expert 0's. Ends with a
+// barrier.
 __device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* __restrict__ ids, int64_t sit, int64_t sik, int T,
                                  int k, int E, int NT) {
   const int tid = threadIdx.x, nthreads = blockDim.x, warp = tid >> 5, lane = tid & 31;
@@ -67,7 +78,7 @@ __device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* __
     if (warp == 0) {
       int e = MAX_E + 1;
       if (lane < R) {
-        const int64_t id = ids[static_cast<int64_t>(lane / k) * sit + static_cast<int64_t>(lane % k) * sik];
+        const int64_t id = ids ? ids[static_cast<int64_t>(lane / k) * sit + static_cast<int64_t>(lane % k) * sik] : 0;
         if (id >= 0 && id < E) e = static_cast<int>(id);
       }
       const bool live = e < E;
@@ -111,7 +122,7 @@ __device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* __
       const int s = (warp * steps + i) * 32 + lane;
       int e = -1;
       if (s < R) {
-        const int64_t id = ids[static_cast<int64_t>(s / k) * sit + static_cast<int64_t>(s % k) * sik];
+        const int64_t id = ids ? ids[static_cast<int64_t>(s / k) * sit + static_cast<int64_t>(s % k) * sik] : 0;
         e = (id >= 0 && id < E) ? static_cast<int>(id) : -1;
       }
       const unsigned same = __match_any_sync(0xffffffffu, e);

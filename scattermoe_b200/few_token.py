@@ -58,7 +58,7 @@ def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Opti
     ws_bytes = lib.smoe_few_token_workspace_bytes(T, k, F, d_out)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
     null = (None, 0, 0)
-    with torch.cuda.device(dev):
+    with _lib.on_device_of(dev):
         rc = lib.smoe_few_token_mlp(
             x.data_ptr(), T, x.stride(0), up.data_ptr(), up.stride(0), up.stride(1), up.stride(2),
             *((up_b.data_ptr(), up_b.stride(0), up_b.stride(1)) if up_b is not None else null),
@@ -67,15 +67,10 @@ def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Opti
             *((gates.data_ptr(), gates.stride(0), gates.stride(1), _lib.DTYPE_CODE[gates.dtype]) if gates is not None
               else (None, 0, 0, 0)),
             ids.data_ptr(), ids.stride(0), ids.stride(1), y.data_ptr(), y.stride(0), k, d, F, d_out, E, act_layout, act,
-            alpha, limit, _lib.DTYPE_CODE[x.dtype], _path_flags() | (_lib.FLAG_AFTER_ROUTER if after_router else 0),
+            alpha, limit, _lib.DTYPE_CODE[x.dtype], _lib.path_flags() | (_lib.FLAG_AFTER_ROUTER if after_router else 0),
             ws.data_ptr(), ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_few_token_mlp")
     return y
-
-
-def _path_flags() -> int:
-    from .kernels import ops
-    return {None: 0, "simt": _lib.FLAG_FORCE_SIMT, "tc": _lib.FLAG_FORCE_TC}[ops.FORCE_PATH]
 
 
 @torch.library.custom_op("scattermoe_b200::few_token_mlp", mutates_args={})
@@ -158,7 +153,7 @@ def _route_impl(x: torch.Tensor, wr: torch.Tensor, br: Optional[torch.Tensor], k
     dev = x.device
     ids = torch.empty((T, k), dtype=torch.int64, device=dev)
     gates = torch.empty((T, k), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
+    with _lib.on_device_of(dev):
         rc = _lib.load().smoe_few_token_route(
             x.data_ptr(), T, x.stride(0), wr.data_ptr(), wr.stride(0), br.data_ptr() if br is not None else None,
             br.stride(0) if br is not None else 0, wr.size(0), d, k, mode, int(renormalize), ids.data_ptr(), gates.data_ptr(),

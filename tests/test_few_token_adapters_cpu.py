@@ -48,7 +48,7 @@ def test_adapter_entry_points_refuse(bad, word):
     shrink = dict(X=256, T=4, sxm=64, M=256, sma=512, smj=64, smc=1, ids=256, scaling=None, scale=1.0, H=256, n=2, C=64, r=8, dtype=1, stream=None)
     assert lib.smoe_adapter_shrink(*{**shrink, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
     linear = dict(X=256, T=4, sxm=64, W=256, swk=1, swn=64, bias=None, H=256, M=256, sma=512, smj=1, smo=8, ids=256, Y=256, sym=64,
-                  n=2, C=64, O=64, r=8, dtype=1, status=None, stream=None)
+                  n=2, C=64, O=64, r=8, dtype=1, flags=0, status=None, stream=None)
     assert lib.smoe_adapter_linear(*{**linear, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
     grad = dict(U=256, T=4, V=256, svm=64, idx=256, off=256, D=256, sda=512, sdj=64, sdc=1, n=2, C=64, r=8, dtype=1, ws=256, ws_bytes=1 << 24, stream=None)
     bad = {("V" if k == "X" else k): v for k, v in bad.items()}
