@@ -264,7 +264,9 @@ int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void
  * Each row names its adapter a = adapter_idxs[t]; ids outside [0, n) mean none. Three products make both directions:
  * smoe_adapter_shrink:  H[t, j] = s_a sum_c X[t, c] M[a][j, c]     zero rows without an adapter;
  *     s_a = scaling[a], or `scale` where `scaling` is null. M: lora_a forward, lora_b seen as (n, r, out) backward. H is
- *     (T, R) contiguous in `dtype`, R = r rounded up to a multiple of 8, the padding written as zeros.
+ *     (T, R) contiguous in `dtype`, R = r rounded up to a multiple of 8, the padding written as zeros. `sorted_idx` and
+ *     `offsets` (nullable, both or neither) are smoe_sort_count's of adapter_idxs: rows in no order then cost no more than
+ *     rows in runs.
  * smoe_adapter_linear:  Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum_j H[t, j] M[a][j, o]      (bias nullable, contiguous)
  * smoe_adapter_grad:    D[a][j, c] = sum over the rows t of adapter a of U[t, j] V[t, c], U as H above, rows listed by
  *     smoe_sort_count of adapter_idxs (sorted_scattered_idxs, expert_offsets); every element of D is written.
@@ -273,7 +275,7 @@ int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void
  * aligned, sized by the queries) belong to the call until its work has finished. */
 int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma, int64_t stride_mj,
                         int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling, float scale, void* H, int32_t n,
-                        int32_t C, int32_t r, int32_t dtype, void* stream);
+                        int32_t C, int32_t r, int32_t dtype, const int64_t* sorted_idx, const int64_t* offsets, void* stream);
 int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk, int64_t stride_wn,
                         const void* bias, const void* H, const void* M, int64_t stride_ma, int64_t stride_mj,
                         int64_t stride_mo, const int64_t* adapter_idxs, void* Y, int64_t stride_ym, int32_t n, int32_t C,

@@ -102,7 +102,8 @@ SIGNATURES = {
                             _I32, _I32, _I32, _I32, _I32,    # k d F d_out E
                             _I32, _I32, c_float, c_float, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
     "smoe_few_token_route": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _I32, _P], c_int32),
-    "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P], c_int32),
+    "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P, _P, _P],
+                            c_int32),
     "smoe_adapter_linear": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32,
                              _I32, _I32, _P, _P], c_int32),
     "smoe_adapter_grad_workspace_bytes": ([_I64, _I32, _I32], c_size_t),

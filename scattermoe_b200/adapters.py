@@ -31,7 +31,8 @@ def _padded(r: int) -> int:
     return (r + 7) // 8 * 8
 
 
-def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float) -> torch.Tensor:
+def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float,
+                 sorted_idx: Optional[torch.Tensor], offsets: Optional[torch.Tensor]) -> torch.Tensor:
     """h[t, j] = s sum_c x[t, c] m[ids[t], j, c], (T, r padded to a multiple of 8); zero rows for ids outside [0, n)."""
     T = x.size(0)
     n, r, C = m.shape
@@ -40,6 +41,7 @@ def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: O
         rc = _lib.load().smoe_adapter_shrink(
             x.data_ptr(), T, x.stride(0), m.data_ptr(), m.stride(0), m.stride(1), m.stride(2), ids.data_ptr(),
             scaling.data_ptr() if scaling is not None else None, scale, h.data_ptr(), n, C, r, _lib.DTYPE_CODE[x.dtype],
+            sorted_idx.data_ptr() if sorted_idx is not None else None, offsets.data_ptr() if offsets is not None else None,
             _lib.stream_ptr(x.device))
     _lib.check(rc, "smoe_adapter_shrink")
     return h
@@ -95,13 +97,13 @@ def _column_sum_impl(v: torch.Tensor) -> torch.Tensor:
 
 # The registered forms are used while torch.compile traces, as everywhere in this package.
 @torch.library.custom_op("scattermoe_b200::adapter_shrink", mutates_args={})
-def shrink_compileable(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor],
-                       scale: float) -> torch.Tensor:
-    return _shrink_impl(x, m, ids, scaling, scale)
+def shrink_compileable(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float,
+                       sorted_idx: Optional[torch.Tensor], offsets: Optional[torch.Tensor]) -> torch.Tensor:
+    return _shrink_impl(x, m, ids, scaling, scale, sorted_idx, offsets)
 
 
 @shrink_compileable.register_fake
-def _(x, m, ids, scaling, scale):
+def _(x, m, ids, scaling, scale, sorted_idx, offsets):
     return torch.empty((x.size(0), _padded(m.size(1))), dtype=x.dtype, device=x.device)
 
 
@@ -150,16 +152,20 @@ class AdapterLinear_(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, lora_a, lora_b, ids, scaling, scale, bias):
         x = _rowmajor(x)
-        h = _pick(shrink_compileable, _shrink_impl)(x, lora_a, ids, scaling, scale)
+        # the gradients of the adapters need the rows sorted by adapter; the shrinks of both directions profit from it
+        sorted_idx = offsets = None
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            _, sorted_idx, offsets = flatten_sort_count(ids, lora_a.size(0))
+        h = _pick(shrink_compileable, _shrink_impl)(x, lora_a, ids, scaling, scale, sorted_idx, offsets)
         y = _linear(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids, after_shrink=True)
-        ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scaling, h)
+        ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scaling, h, sorted_idx, offsets)
         ctx.scale = scale
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, lora_a, lora_b, ids, scaling, h = ctx.saved_tensors
+        x, weight, lora_a, lora_b, ids, scaling, h, sorted_idx, offsets = ctx.saved_tensors
         need_x, need_w, need_a, need_b = ctx.needs_input_grad[:4]
         need_bias = ctx.needs_input_grad[7]
         dy = _rowmajor(dy)
@@ -167,11 +173,10 @@ class AdapterLinear_(torch.autograd.Function):
             dy = dy.to(x.dtype)
         d_x = d_w = d_a = d_b = d_bias = None
         if need_x or need_a:
-            g = _pick(shrink_compileable, _shrink_impl)(dy, lora_b.transpose(1, 2), ids, scaling, ctx.scale)
+            g = _pick(shrink_compileable, _shrink_impl)(dy, lora_b.transpose(1, 2), ids, scaling, ctx.scale, sorted_idx, offsets)
         if need_x:
             d_x = _linear(dy, weight, None, g, lora_a, ids, after_shrink=True)
         if need_a or need_b:
-            _, sorted_idx, offsets = flatten_sort_count(ids, lora_a.size(0))
             grad = _pick(grad_compileable, _grad_impl)
             if need_a:
                 d_a = grad(g, x, lora_a.size(1), sorted_idx, offsets, False)

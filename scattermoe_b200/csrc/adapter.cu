@@ -20,30 +20,32 @@ __device__ __forceinline__ void load_values(const T* p, float (&out)[V]) {
   }
 }
 
-// ---- shrink: a warp per (token, 4 rank rows), lanes over the contracted axis, V values at a time -----------------
-template <typename T, int V>
+// ---- shrink: a warp per (token, RW rank rows), lanes over the contracted axis, V values at a time -----------------
+template <typename T, int V, int RW>
 __global__ void __launch_bounds__(256)
 shrink_simt_kernel(const ShrinkArgs a) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // the linear may start its stream of W
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int blocks = static_cast<int>(rank_pitch(a.r) / 4);
+  const int blocks = static_cast<int>(rank_pitch(a.r) / RW);
   const int64_t total = a.T * blocks;
   for (int64_t it = static_cast<int64_t>(blockIdx.x) * 8 + warp; it < total; it += static_cast<int64_t>(gridDim.x) * 8) {
     const int64_t t = it / blocks;
-    const int j0 = static_cast<int>(it % blocks) * 4;
+    const int j0 = static_cast<int>(it % blocks) * RW;
     const int64_t id = a.ids[t];
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float acc[RW];
+#pragma unroll
+    for (int i = 0; i < RW; ++i) acc[i] = 0.f;
     float s = 0.f;
     if (id >= 0 && id < a.n) {
       s = a.scaling ? a.scaling[id] : a.scale;
       const T* x = static_cast<const T*>(a.X) + t * a.sxm;
       const T* m = static_cast<const T*>(a.M) + id * a.sma;
-#pragma unroll 2
+#pragma unroll (RW == 1 ? 8 : 2)
       for (int c = lane * V; c < a.C; c += 32 * V) {       // V > 1: contiguous and aligned, C a multiple of V
         float xv[V];
         load_values<T, V>(x + c, xv);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < RW; ++i)
           if (j0 + i < a.r) {
             float mv[V];
             load_values<T, V>(m + (j0 + i) * a.smj + c * a.smc, mv);
@@ -53,7 +55,7 @@ shrink_simt_kernel(const ShrinkArgs a) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < RW; ++i) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
       // an adapter that is not there leaves a zero row, whatever the inputs hold; so does the padding
@@ -180,13 +182,16 @@ grad_simt_kernel(const GradArgs a) {
   }
 
 int launch_shrink_simt(const ShrinkArgs& a) {
-  const int64_t warps = a.T * (rank_pitch(a.r) / 4);
+  // four rank rows per warp read the token's row a quarter as often; one each where there are too few warps to fill the GPU
+  const bool single = a.T * (rank_pitch(a.r) / 4) < 148 * 16;
+  const int64_t warps = a.T * (rank_pitch(a.r) / (single ? 1 : 4));
   const int grid = static_cast<int>(min(cdiv64(warps, 8), static_cast<int64_t>(148 * 32)));
   const int v = 16 / dtype_size(a.dtype);
   auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = a.smc == 1 && a.C % v == 0 && a.sxm % v == 0 && a.smj % v == 0 && a.sma % v == 0 && al16(a.X) && al16(a.M);
-  if (vec) SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 16 / sizeof(T_)><<<grid, 256, 0, a.stream>>>(a);)
-  else SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 1><<<grid, 256, 0, a.stream>>>(a);)
+  if (vec && single) SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 16 / sizeof(T_), 1><<<grid, 256, 0, a.stream>>>(a);)
+  else if (vec) SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 16 / sizeof(T_), 4><<<grid, 256, 0, a.stream>>>(a);)
+  else SMOE_AD_DTYPE(a.dtype, shrink_simt_kernel<T_, 1, 4><<<grid, 256, 0, a.stream>>>(a);)
   SMOE_LAUNCH_CHECK();
   return SMOE_OK;
 }
@@ -251,12 +256,13 @@ using namespace smoe;
 
 extern "C" int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma,
                                    int64_t stride_mj, int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling,
-                                   float scale, void* H, int32_t n, int32_t C, int32_t r, int32_t dtype, void* stream) {
+                                   float scale, void* H, int32_t n, int32_t C, int32_t r, int32_t dtype,
+                                   const int64_t* sorted_idx, const int64_t* offsets, void* stream) {
   if (int rc = ad::check_common("adapter_shrink", T, n, C, r, dtype)) return rc;
   if (T == 0) return SMOE_OK;
   SMOE_CHECK_ARG(X && M && adapter_idxs && H, "adapter_shrink: null pointer");
   ad::ShrinkArgs a{X, T, stride_xm, M, stride_ma, stride_mj, stride_mc, adapter_idxs, scaling, scale, H, n, C, r, dtype,
-                   static_cast<cudaStream_t>(stream)};
+                   offsets ? sorted_idx : nullptr, offsets, static_cast<cudaStream_t>(stream)};
   const int rc = ad::launch_shrink_tc(a);
   return rc != SMOE_ERR_UNSUPPORTED ? rc : ad::launch_shrink_simt(a);
 }

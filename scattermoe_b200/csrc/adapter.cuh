@@ -25,6 +25,7 @@ struct ShrinkArgs {           // H[t, j] = s_a sum_c X[t, c] M[a][j, c]
   const float* scaling; float scale;
   void* H;
   int n, C, r, dtype;
+  const int64_t* sorted_idx; const int64_t* offsets;      // the rows sorted by adapter, where the caller has them (nullable)
   cudaStream_t stream;
 };
 

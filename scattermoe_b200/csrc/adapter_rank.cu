@@ -32,11 +32,13 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t addr) {
 static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // ---- shrink --------------------------------------------------------------------------------------------------------
-// A block owns 32 tokens. Its eight warps take 64 of the contracted axis each, in turn, every warp with a double buffer of its own
-// (cp.async), and are joined once at the end. A pass multiplies up to 64 columns: the rank rows of as many of the block's
-// adapters as fit (a block whose tokens share an adapter needs one pass). X comes from HBM in the first pass, from L2 in others.
+// A block owns 32 tokens: consecutive ones, or, where the caller has sorted the rows by adapter, consecutive sorted ones. Its eight warps
+// take 64 of the contracted axis each, in turn, every warp with a ring of its own (cp.async, two to four stages), and are joined
+// once at the end. A pass multiplies up to 64 columns: the rank rows of as many of the block's adapters as the ring holds (a
+// block whose tokens share an adapter needs one pass). X comes from HBM in the first pass, from L2 in others.
 constexpr int SH_MAX_SMEM = 226 * 1024;      // 1 KB less than a block can have: the static arrays
-constexpr int SH_TOKENS = 32, SH_COLS = 64, SH_K = 64, SH_STAGES = 2;
+constexpr int SH_TOKENS = 32, SH_COLS = 64, SH_K = 64;
+constexpr int SH_SMALL_RING = 13 * 1024;      // per warp: two blocks fit an SM
 
 struct ShrinkParams {
   ShrinkArgs a;
@@ -44,8 +46,7 @@ struct ShrinkParams {
   int m_vec;         // and 16-byte pieces of it can be copied
   int per_pass;      // adapters of a pass
   int width;         // columns an adapter takes in a pass (the rank, or a part of it, rounded up to 8)
-  int m_pitch;       // bytes of a row of M in shared memory
-  int stage_bytes;   // of one warp
+  int ring_bytes;    // of one warp
 };
 
 template <typename T>
@@ -56,7 +57,8 @@ shrink_tc_kernel(const ShrinkParams p) {
   const ShrinkArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t t0 = static_cast<int64_t>(blockIdx.x) * SH_TOKENS;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(SH_TOKENS), a.T - t0));
+  __shared__ int32_t token[SH_TOKENS];
+  int rows = static_cast<int>(min(static_cast<int64_t>(SH_TOKENS), a.T - t0));
   const int64_t pitch = rank_pitch(a.r);
   uint32_t id = 0xffffffffu;
   if (lane < rows) {
@@ -69,8 +71,17 @@ shrink_tc_kernel(const ShrinkParams p) {
     const int t = i / static_cast<int>(pitch), j = i % static_cast<int>(pitch);
     if ((bare >> t & 1u) || j >= a.r) H[(t0 + t) * pitch + j] = from_f32<T>(0.f);
   }
-  const uint32_t ring = smem_u32(smem) + warp * SH_STAGES * p.stage_bytes;
-  uint8_t* ring_ptr = smem + warp * SH_STAGES * p.stage_bytes;
+  if (a.sorted_idx) {        // from here on the block's rows are sorted ones
+    const int64_t live = min(a.offsets[a.n - 1], a.T);
+    rows = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(SH_TOKENS), live - t0)));
+    const int64_t t = lane < rows ? a.sorted_idx[t0 + lane] : 0;
+    id = lane < rows ? static_cast<uint32_t>(a.ids[t]) : 0xffffffffu;
+    if (warp == 0) token[lane] = static_cast<int32_t>(t);
+  } else if (warp == 0) {
+    token[lane] = static_cast<int32_t>(lane < rows ? t0 + lane : 0);
+  }
+  const uint32_t ring = smem_u32(smem) + warp * p.ring_bytes;
+  uint8_t* ring_ptr = smem + warp * p.ring_bytes;
   const uint8_t* X = static_cast<const uint8_t*>(a.X);
   const uint8_t* M = static_cast<const uint8_t*>(a.M);
   uint32_t from = 0;
@@ -87,6 +98,8 @@ shrink_tc_kernel(const ShrinkParams p) {
     __syncthreads();
     for (int j0 = 0; j0 < a.r; j0 += p.width) {
       const int cols = adapters * p.width, groups = cols >> 3;
+      const int m_pitch = cols * 2 + 16;         // M with the rank contiguous: bytes of a row in shared memory
+      const int stage_bytes = SH_TOKENS * 128 + (p.k_major ? (groups + 1) / 2 * 2048 : SH_K * m_pitch);
       float acc[2][8][4];
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -94,45 +107,61 @@ shrink_tc_kernel(const ShrinkParams p) {
         for (int g = 0; g < 8; ++g)
 #pragma unroll
           for (int q = 0; q < 4; ++q) acc[m][g][q] = 0.f;
+      // what a lane copies is fixed but for the step of the contracted axis: addresses are made once
+      const int chunk = lane & 7, pieces = cols >> 3;
+      const uint8_t* x_row[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = (lane >> 3) + i * 4;
+        x_row[i] = row < rows ? X + (static_cast<int64_t>(token[row]) * a.sxm + chunk * 8) * 2 : nullptr;
+      }
+      const uint8_t* m_base = M + (static_cast<int64_t>(chosen[0]) * a.sma + static_cast<int64_t>(j0) * a.smj) * 2;
+      const int piece0 = lane % pieces, c_first = lane / pieces, c_step = 32 / pieces, piece_step = 32 - c_step * pieces;
+      // column -> its adapter's place in `chosen` and its rank row
+      auto adapter_of = [&](int col) { return adapters == 1 ? 0 : col / p.width; };
       auto load = [&](int s, int k0) {
-        const uint32_t dst = ring + s * p.stage_bytes;
-        const int chunk = lane & 7;
+        const uint32_t dst = ring + s * stage_bytes;
         const bool in_k = k0 + chunk * 8 < a.C;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {          // 32 token rows of 128 bytes
           const int row = (lane >> 3) + i * 4;
-          const bool v = in_k && row < rows;
-          cp_async16(dst + row * 128 + ((chunk ^ (row & 7)) << 4), X + (v ? ((t0 + row) * a.sxm + k0 + chunk * 8) * 2 : 0), v ? 16 : 0);
+          const bool v = in_k && x_row[i] != nullptr;
+          cp_async16(dst + row * 128 + ((chunk ^ (row & 7)) << 4), v ? x_row[i] + k0 * 2 : X, v ? 16 : 0);
         }
         const uint32_t dm = dst + SH_TOKENS * 128;
-        uint8_t* dm_ptr = ring_ptr + s * p.stage_bytes + SH_TOKENS * 128;
+        uint8_t* dm_ptr = ring_ptr + s * stage_bytes + SH_TOKENS * 128;
         if (p.k_major) {                       // a row per column: 64 of the contracted axis
           for (int col = lane >> 3; col < cols; col += 4) {
-            const int ad = col / p.width, j = j0 + col - ad * p.width;
-            const uint8_t* src = M + (static_cast<int64_t>(chosen[ad]) * a.sma + static_cast<int64_t>(j) * a.smj + k0 + chunk * 8) * 2;
+            const int ad = adapter_of(col), in = col - ad * p.width;
+            const bool live = j0 + in < a.r;
+            const uint8_t* src = (ad == 0 ? m_base : M + (static_cast<int64_t>(chosen[ad]) * a.sma + static_cast<int64_t>(j0) * a.smj) * 2) +
+                                 (in * a.smj + k0 + chunk * 8) * 2;
             const uint32_t at = col * 128 + ((chunk ^ (col & 7)) << 4);
             if (p.m_vec) {
-              const bool v = in_k && j < a.r;
+              const bool v = in_k && live;
               cp_async16(dm + at, v ? src : M, v ? 16 : 0);
             } else {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
                 reinterpret_cast<uint16_t*>(dm_ptr + at)[i] =
-                    j < a.r && k0 + chunk * 8 + i < a.C ? __ldg(reinterpret_cast<const uint16_t*>(src) + i * a.smc) : 0;
+                    live && k0 + chunk * 8 + i < a.C ? __ldg(reinterpret_cast<const uint16_t*>(src) + i) : 0;
             }
           }
         } else if (p.m_vec) {                  // a row per step of the contracted axis: the adapters' pieces of the rank
-          const int pieces = cols >> 3;
-          for (int i = lane; i < SH_K * pieces; i += 32) {
-            const int c = i / pieces, col = (i - c * pieces) * 8, ad = col / p.width, j = j0 + col - ad * p.width;
-            const bool v = k0 + c < a.C && j < a.r;
-            cp_async16(dm + c * p.m_pitch + col * 2,
-                       v ? M + (static_cast<int64_t>(chosen[ad]) * a.sma + static_cast<int64_t>(k0 + c) * a.smc + j) * 2 : M, v ? 16 : 0);
+          int c = c_first, piece = piece0;
+          while (c < SH_K) {
+            const int col = piece * 8, ad = adapter_of(col), in = col - ad * p.width;
+            const bool v = k0 + c < a.C && j0 + in < a.r;
+            const uint8_t* src = ad == 0 ? m_base : M + (static_cast<int64_t>(chosen[ad]) * a.sma + j0) * 2;
+            cp_async16(dm + c * m_pitch + col * 2, v ? src + (static_cast<int64_t>(k0 + c) * a.smc + in) * 2 : M, v ? 16 : 0);
+            c += c_step;
+            piece += piece_step;
+            if (piece >= pieces) { piece -= pieces; ++c; }
           }
         } else {
           for (int i = lane; i < SH_K * cols; i += 32) {
-            const int c = i / cols, col = i - c * cols, ad = col / p.width, j = j0 + col - ad * p.width;
-            *reinterpret_cast<uint16_t*>(dm_ptr + c * p.m_pitch + col * 2) =
+            const int c = i / cols, col = i - c * cols, ad = adapter_of(col), j = j0 + col - ad * p.width;
+            *reinterpret_cast<uint16_t*>(dm_ptr + c * m_pitch + col * 2) =
                 k0 + c < a.C && j < a.r
                     ? __ldg(reinterpret_cast<const uint16_t*>(M) + static_cast<int64_t>(chosen[ad]) * a.sma +
                             static_cast<int64_t>(k0 + c) * a.smc + static_cast<int64_t>(j) * a.smj) : 0;
@@ -141,13 +170,17 @@ shrink_tc_kernel(const ShrinkParams p) {
         cp_async_commit();
       };
       constexpr int TURN = 8 * SH_K;
-      int k0 = warp * SH_K, s = 0;
-      if (k0 < a.C) load(0, k0); else cp_async_commit();
-      for (; k0 < a.C; k0 += TURN, s ^= 1) {
-        if (k0 + TURN < a.C) load(s ^ 1, k0 + TURN); else cp_async_commit();
-        cp_async_wait<1>();
+      auto run = [&](auto S_) {
+      constexpr int S = decltype(S_)::value;      // stages of the ring
+      int k0 = warp * SH_K, s = 0, ahead = k0;
+#pragma unroll
+      for (int i = 0; i < S - 1; ++i, ahead += TURN)
+        if (ahead < a.C) load(i, ahead); else cp_async_commit();
+      for (; k0 < a.C; k0 += TURN, ahead += TURN, s = s + 1 == S ? 0 : s + 1) {
+        if (ahead < a.C) load(s == 0 ? S - 1 : s - 1, ahead); else cp_async_commit();
+        cp_async_wait<S - 1>();
         __syncwarp();
-        const uint32_t x = ring + s * p.stage_bytes, m = x + SH_TOKENS * 128;
+        const uint32_t x = ring + s * stage_bytes, m = x + SH_TOKENS * 128;
 #pragma unroll
         for (int st = 0; st < SH_K / 16; ++st) {
           uint32_t af[2][4];
@@ -163,7 +196,7 @@ shrink_tc_kernel(const ShrinkParams p) {
                 const int col = (lane & 7) + (lane >> 4) * 8;
                 ldsm4(b, m + (g * 8 + col) * 128 + (((st * 2 + ((lane >> 3) & 1)) ^ (col & 7)) << 4));
               } else {
-                ldsm4_trans(b, m + (st * 16 + (lane & 15)) * p.m_pitch + (g * 8 + (lane >> 4) * 8) * 2);
+                ldsm4_trans(b, m + (st * 16 + (lane & 15)) * m_pitch + (g * 8 + (lane >> 4) * 8) * 2);
               }
 #pragma unroll
               for (int mt = 0; mt < 2; ++mt) {
@@ -174,6 +207,10 @@ shrink_tc_kernel(const ShrinkParams p) {
         }
         __syncwarp();
       }
+      };
+      if (4 * stage_bytes <= p.ring_bytes) run(std::integral_constant<int, 4>{});
+      else if (3 * stage_bytes <= p.ring_bytes) run(std::integral_constant<int, 3>{});
+      else run(std::integral_constant<int, 2>{});
       cp_async_wait<0>();
       __syncthreads();
       // join the warps: [warp][token][column]
@@ -191,11 +228,11 @@ shrink_tc_kernel(const ShrinkParams p) {
       __syncthreads();
       for (int i = tid; i < SH_TOKENS * cols; i += 256) {
         const int t = i / cols, col = i - t * cols, ad = col / p.width, j = j0 + col - ad * p.width;
-        if (t >= rows || j >= a.r || a.ids[t0 + t] != static_cast<int64_t>(chosen[ad])) continue;
+        if (t >= rows || j >= a.r || a.ids[token[t]] != static_cast<int64_t>(chosen[ad])) continue;
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < 8; ++w) v += red[(w * SH_TOKENS + t) * rp + col];
-        H[(t0 + t) * pitch + j] = from_f32<T>(v * (a.scaling ? a.scaling[chosen[ad]] : a.scale));
+        H[token[t] * pitch + j] = from_f32<T>(v * (a.scaling ? a.scaling[chosen[ad]] : a.scale));
       }
       __syncthreads();
     }
@@ -211,15 +248,19 @@ int launch_shrink_tc(const ShrinkArgs& a) {
   p.a = a;
   const int r8 = static_cast<int>(rank_pitch(a.r));
   p.width = r8 < SH_COLS ? r8 : SH_COLS;
-  p.per_pass = r8 <= SH_COLS ? SH_COLS / r8 : 1;
   p.k_major = a.smc == 1 ? 1 : 0;
   const bool aligned = al16(a.M) && a.sma % 8 == 0;
   p.m_vec = aligned && (p.k_major ? a.smj % 8 == 0 : a.smj == 1 && a.smc % 8 == 0 && a.r % 8 == 0) ? 1 : 0;
+  // Two stages of one adapter are the least. Where that is little the ring stays small enough for two blocks per SM, which is what
+  // tokens in runs want; rows in no order (and not sorted) want as many adapters in a pass as fit.
+  auto stage_of = [&](int cols) { return SH_TOKENS * 128 + (p.k_major ? cdiv(cols, 16) * 2048 : SH_K * (cols * 2 + 16)); };
+  const int one = 2 * stage_of(p.width);
+  p.ring_bytes = one <= SH_SMALL_RING ? SH_SMALL_RING : (one > 20 * 1024 ? one : 20 * 1024);
+  p.per_pass = 1;
+  while (p.per_pass < 8 && (p.per_pass + 1) * p.width <= SH_COLS && 2 * stage_of((p.per_pass + 1) * p.width) <= p.ring_bytes) ++p.per_pass;
+  p.ring_bytes = cdiv(p.ring_bytes, 128) * 128;
   const int cols = p.per_pass * p.width;
-  p.m_pitch = p.k_major ? 128 : cols * 2 + 16;
-  p.stage_bytes = SH_TOKENS * 128 + (p.k_major ? cdiv(cols, 16) * 16 * 128 : SH_K * p.m_pitch);
-  p.stage_bytes = cdiv(p.stage_bytes, 128) * 128;
-  const int ring = 8 * SH_STAGES * p.stage_bytes, red = 8 * SH_TOKENS * (cols + 1) * 4;
+  const int ring = 8 * p.ring_bytes, red = 8 * SH_TOKENS * (cols + 1) * 4;
   const int smem = (ring > red ? ring : red) + 64;      // the last ldmatrix of an odd group reads 16 bytes past its row
   DeviceInfo di;
   if (int rc = get_device_info(&di)) return rc;
@@ -261,7 +302,8 @@ size_t grad_workspace_bytes(int64_t T, int C, int r) { return static_cast<size_t
 struct GradParams {
   GradArgs a;
   int chunks;
-  float* parts;      // [chunk][first, last][r][C]
+  float* parts;      // [chunk][first, last], each in the order of D: (r, C), or (C, r) where D has the rank contiguous
+  int by_rank;       // the latter
 };
 
 template <typename T>
@@ -295,22 +337,32 @@ grad_tc_kernel(const GradParams p) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) acc[g][q] = 0.f;
     const int tiles = static_cast<int>((end - beg + GR_ROWS - 1) / GR_ROWS);
+    // the rows of the next tile to load: their numbers are fetched a tile early, or every copy would wait for them
+    int32_t next_row[GR_ROWS / 16];
+    auto fetch_rows = [&](int i) {
+#pragma unroll
+      for (int q = 0; q < GR_ROWS / 16; ++q) {
+        const int64_t m = beg + static_cast<int64_t>(i) * GR_ROWS + (tid >> 4) + q * 16;
+        next_row[q] = m < end ? static_cast<int32_t>(a.sorted_idx[m]) : -1;
+      }
+    };
     auto load = [&](int i) {
       const uint32_t dst = ring + (i % GR_STAGES) * GR_STAGE;
       const int chunk = tid & 15;
 #pragma unroll
       for (int q = 0; q < GR_ROWS / 16; ++q) {
         const int row = (tid >> 4) + q * 16;
-        const int64_t m = beg + static_cast<int64_t>(i) * GR_ROWS + row;
-        const bool in = m < end;
-        const int64_t t = in ? a.sorted_idx[m] : 0;
+        const bool in = next_row[q] >= 0;
+        const int64_t t = in ? next_row[q] : 0;
         const bool v = in && c0 + chunk * 8 < a.C;
         cp_async16(dst + row * GR_V_PITCH + chunk * 16, V + (v ? (t * a.svm + c0 + chunk * 8) * 2 : 0), v ? 16 : 0);
         if (chunk < groups)
           cp_async16(dst + GR_ROWS * GR_V_PITCH + row * GR_U_PITCH + chunk * 16, U + (in ? (t * u_pitch + j0 + chunk * 8) * 2 : 0), in ? 16 : 0);
       }
       cp_async_commit();
+      fetch_rows(i + 1);
     };
+    fetch_rows(0);
     for (int i = 0; i < GR_STAGES - 1; ++i)
       if (i < tiles) load(i); else cp_async_commit();
     for (int i = 0; i < tiles; ++i) {
@@ -344,7 +396,7 @@ grad_tc_kernel(const GradParams p) {
           const int c = c0 + warp * 16 + (lane >> 2) + (q >> 1) * 8, j = j0 + g * 8 + (lane & 3) * 2 + (q & 1);
           if (c >= a.C || j >= a.r) continue;
           if (whole) static_cast<T*>(a.D)[e * a.sda + j * a.sdj + c * a.sdc] = from_f32<T>(acc[g][q]);
-          else part[static_cast<int64_t>(j) * a.C + c] = acc[g][q];
+          else part[p.by_rank ? static_cast<int64_t>(c) * a.r + j : static_cast<int64_t>(j) * a.C + c] = acc[g][q];
         }
       }
     beg = end;
@@ -370,7 +422,9 @@ grad_join_kernel(const GradParams p) {
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
     float v = 0.f;
     for (int z = z0; z <= z1; ++z) v += p.parts[(static_cast<int64_t>(z) * 2 + (beg < z * per ? 0 : 1)) * total + i];
-    const int64_t j = i / a.C, c = i - j * a.C;
+    const int64_t inner = p.by_rank ? a.r : a.C;
+    const int64_t outer_i = total < (int64_t(1) << 31) ? static_cast<uint32_t>(i) / static_cast<uint32_t>(inner) : i / inner;
+    const int64_t inner_i = i - outer_i * inner, j = p.by_rank ? inner_i : outer_i, c = p.by_rank ? outer_i : inner_i;
     static_cast<T*>(a.D)[e * a.sda + j * a.sdj + c * a.sdc] = from_f32<T>(v);
   }
 }
@@ -385,6 +439,7 @@ int launch_grad_tc(const GradArgs& a) {
   p.a = a;
   p.chunks = grad_chunks(a.T, a.C, a.r);
   p.parts = static_cast<float*>(a.ws);
+  p.by_rank = a.sdj == 1 && a.sdc != 1 ? 1 : 0;
   static std::mutex mu;
   static bool configured[64] = {false};
   {
@@ -403,7 +458,7 @@ int launch_grad_tc(const GradArgs& a) {
     SMOE_LAUNCH_CHECK();
   }
   const int64_t values = static_cast<int64_t>(a.r) * a.C;
-  dim3 grid(static_cast<unsigned>(cdiv64(values, 1024) < 256 ? cdiv64(values, 1024) : 256), 1, static_cast<unsigned>(a.n));
+  dim3 grid(static_cast<unsigned>(cdiv64(values, 256) < 256 ? cdiv64(values, 256) : 256), 1, static_cast<unsigned>(a.n));
   if (bf16) grad_join_kernel<__nv_bfloat16><<<grid, 256, 0, a.stream>>>(p);
   else grad_join_kernel<__half><<<grid, 256, 0, a.stream>>>(p);
   SMOE_LAUNCH_CHECK();

@@ -234,26 +234,32 @@ __device__ __forceinline__ float hidden_fast(int layout, int act, float alpha, f
   return r * lin;
 }
 
-// What row t's adapter adds to column o.
+// What adapter `id` adds to columns o and o + 16 of row t (second: whether the latter is wanted).
 template <typename T>
-__device__ __forceinline__ float extension_term(const Extension& x, int t, int o) {
-  const int64_t id = x.ids[t];
-  if (id < 0 || id >= x.n) return 0.f;
+__device__ __forceinline__ void extension_terms(const Extension& x, int t, int id, int o, bool second, float (&sum)[2]) {
+  sum[0] = sum[1] = 0.f;
+  if (id < 0) return;
   const T* h = static_cast<const T*>(x.h) + t * x.h_pitch;
   const T* m = static_cast<const T*>(x.m) + id * x.sma + o * x.smo;
-  float sum = 0.f;
+  const int64_t next = second ? 16 * x.smo : 0;
   if (x.m_vec) {
-#pragma unroll 2
+#pragma unroll 4
     for (int j = 0; j < x.r; j += 8) {
-      const uint4 hv = __ldg(reinterpret_cast<const uint4*>(h + j)), mv = __ldg(reinterpret_cast<const uint4*>(m + j));
-      const T *ht = reinterpret_cast<const T*>(&hv), *mt = reinterpret_cast<const T*>(&mv);
+      const uint4 hv = __ldg(reinterpret_cast<const uint4*>(h + j)), m0 = __ldg(reinterpret_cast<const uint4*>(m + j)),
+                  m1 = __ldg(reinterpret_cast<const uint4*>(m + next + j));
+      const T *ht = reinterpret_cast<const T*>(&hv), *t0 = reinterpret_cast<const T*>(&m0), *t1 = reinterpret_cast<const T*>(&m1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(to_f32<T>(ht[i]), to_f32<T>(mt[i]), sum);
+      for (int i = 0; i < 8; ++i) {
+        sum[0] = fmaf(to_f32<T>(ht[i]), to_f32<T>(t0[i]), sum[0]);
+        sum[1] = fmaf(to_f32<T>(ht[i]), to_f32<T>(t1[i]), sum[1]);
+      }
     }
   } else {
-    for (int j = 0; j < x.r; ++j) sum = fmaf(to_f32<T>(h[j]), to_f32<T>(__ldg(m + j * x.smj)), sum);
+    for (int j = 0; j < x.r; ++j) {
+      sum[0] = fmaf(to_f32<T>(h[j]), to_f32<T>(__ldg(m + j * x.smj)), sum[0]);
+      sum[1] = fmaf(to_f32<T>(h[j]), to_f32<T>(__ldg(m + next + j * x.smj)), sum[1]);
+    }
   }
-  return sum;
 }
 
 template <typename T, bool UP, bool KMAJOR>
@@ -268,7 +274,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   uint64_t* bars = reinterpret_cast<uint64_t*>(token + MAX_R);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * MAX_STAGES);
   int* joined = reinterpret_cast<int*>(bars + 2 * MAX_STAGES) + 1;
-  float* sums = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // down: [warp][T][rows + 1]; up: the listed slots' gates
+  float* sums = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // down: [warp][T][rows + 1]; up: the listed slots' gates (or adapters)
   const int pitch = p.rows + 1;
   const Args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -399,7 +405,12 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   if (UP) {
     for (int i = tid; i < listed; i += CONSUMERS * 32) {
       const int slot = plan->slots[i], t = token[i];
-      sums[i] = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
+      if (p.ext.ids) {      // the row's adapter
+        const int64_t id = p.ext.ids[t];
+        sums[i] = __int_as_float(id >= 0 && id < p.ext.n ? static_cast<int>(id) : -1);
+      } else {
+        sums[i] = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
+      }
     }
     consumers_sync();
   } else {
@@ -535,8 +546,9 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     else if (groups == 3) stream(std::integral_constant<int, 3>{});
     else stream(std::integral_constant<int, 4>{});
 
-    if (UP && team > 1) {
-      // the warps of a tile put their parts side by side; each then takes every team-th value of all
+    if (UP) {
+      // The sums go through shared memory, where the warps of a tile meet (each then takes every team-th value of all) and where a
+      // short loop can pick them up: unrolled over the registers the epilogue outgrew the instruction cache (10 us and more).
       float* red = sums + MAX_R;
 #pragma unroll
       for (int m = 0; m < M; ++m)
@@ -546,32 +558,20 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 #pragma unroll
             for (int q = 0; q < 4; ++q) red[(warp * 32 + (m * 4 + g) * 4 + q) * 32 + lane] = acc[m][g][q];
           }
-      consumers_sync();
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (g < groups && (g * 4 + q) % team == sub) {
-#pragma unroll
-            for (int m = 0; m < M; ++m) {
-              float v = 0.f;
-              for (int w = 0; w < team; ++w) v += red[((tl * team + w) * 32 + (m * 4 + g) * 4 + q) * 32 + lane];
-              acc[m][g][q] = v;
-            }
-          }
-      consumers_sync();
-    }
-    if (UP) {
+      if (team > 1) consumers_sync(); else __syncwarp();
       if (p.ext.ids) wait_for_previous_kernel();      // the rank rows of the extension
       // accumulator q of group g: slot g*8 + 2*(lane & 3) + (q & 1), weight row (lane >> 2) + 8*(q >> 1) of each 16-row half
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        if (g >= groups || !use0) continue;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (team > 1 && (g * 4 + q) % team != sub) continue;
+      if (use0) {
+#pragma unroll 1
+        for (int idx = sub; idx < groups * 4; idx += team) {
+          const int g = idx >> 2, q = idx & 3;
           const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = (lane >> 2) + (q >> 1) * 8;
-          float c[2][2] = {{acc[0][g][q], acc[M - 1][g][q]}, {0.f, 0.f}};       // (first, second column) of up to two values
+          float c[2][2] = {{0.f, 0.f}, {0.f, 0.f}};       // (first, second column) of up to two values
+          for (int w = 0; w < team; ++w) {
+            const float* part = red + ((tl * team + w) * 32 + idx) * 32 + lane;
+            c[0][0] += part[0];
+            c[0][1] += part[16 * 32];
+          }
           int v[2] = {row, -1};
           if (!pairs) {
             c[1][0] = c[0][1];
@@ -584,7 +584,10 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           }
           if (i >= n) continue;
           const int slot = plan->slots[beg + i];
-          const float gate = sums[beg + i];
+          const float gate = p.ext.ids ? 1.f : sums[beg + i];
+          float extra[2] = {0.f, 0.f};
+          if (p.ext.ids && v[0] < count)
+            extension_terms<T>(p.ext, slot, __float_as_int(sums[beg + i]), v0 + v[0], v[1] < count, extra);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (v[h] < 0 || v[h] >= count) continue;
@@ -595,12 +598,13 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
               c0 += to_f32<T>(bias[(woven ? 2 * pv : pv) * a.sb1n]);
               if (pairs) c1 += to_f32<T>(bias[(woven ? 2 * pv + 1 : a.F + pv) * a.sb1n]);
             }
-            if (p.ext.ids) c0 += extension_term<T>(p.ext, slot, pv);
+            c0 += extra[h];
             reinterpret_cast<T*>(p.hidden)[static_cast<int64_t>(slot) * a.F + pv] =
                 from_f32<T>(gate * hidden_fast(a.act_layout, a.act, a.alpha, a.limit, c0, c1));
           }
         }
       }
+      if (team > 1) consumers_sync(); else __syncwarp();
     } else {
       // add the job's slots to this warp's token sums. Slots of one token (the same expert twice) stand together and may sit in
       // neighbouring lanes: then the lanes take turns

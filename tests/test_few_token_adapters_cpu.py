@@ -45,7 +45,8 @@ def test_few_token_route_refuses(bad, word):
                                       (dict(T=-1), "T=-1"), (dict(C=0), "width"), (dict(dtype=3), "dtype"), (dict(X=None), "null")])
 def test_adapter_entry_points_refuse(bad, word):
     lib = _lib.load()
-    shrink = dict(X=256, T=4, sxm=64, M=256, sma=512, smj=64, smc=1, ids=256, scaling=None, scale=1.0, H=256, n=2, C=64, r=8, dtype=1, stream=None)
+    shrink = dict(X=256, T=4, sxm=64, M=256, sma=512, smj=64, smc=1, ids=256, scaling=None, scale=1.0, H=256, n=2, C=64, r=8, dtype=1,
+                  sorted_idx=None, offsets=None, stream=None)
     assert lib.smoe_adapter_shrink(*{**shrink, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
     linear = dict(X=256, T=4, sxm=64, W=256, swk=1, swn=64, bias=None, H=256, M=256, sma=512, smj=1, smo=8, ids=256, Y=256, sym=64,
                   n=2, C=64, O=64, r=8, dtype=1, flags=0, status=None, stream=None)
