@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import kernels
-from .parallel_experts import _rowmajor, flatten_sort_count
+from .parallel_experts import _rowmajor, _sort_count_impl, sort_count_compileable
 
 MAX_RANK = 256
 MAX_ADAPTERS = 4096
@@ -39,7 +39,7 @@ def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: O
     h = torch.empty((T, _padded(r)), dtype=x.dtype, device=x.device)
     with _lib.on_device_of(x.device):
         rc = _lib.load().smoe_adapter_shrink(
-            x.data_ptr(), T, x.stride(0), m.data_ptr(), m.stride(0), m.stride(1), m.stride(2), ids.data_ptr(),
+            x.data_ptr(), T, x.stride(0), m.data_ptr(), *m.stride(), ids.data_ptr(),
             scaling.data_ptr() if scaling is not None else None, scale, h.data_ptr(), n, C, r, _lib.DTYPE_CODE[x.dtype],
             sorted_idx.data_ptr() if sorted_idx is not None else None, offsets.data_ptr() if offsets is not None else None,
             _lib.stream_ptr(x.device))
@@ -56,8 +56,8 @@ def _linear_impl(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor],
     y = torch.empty((T, O), dtype=x.dtype, device=x.device)
     with _lib.on_device_of(x.device):
         rc = _lib.load().smoe_adapter_linear(
-            x.data_ptr(), T, x.stride(0), w.data_ptr(), w.stride(0), w.stride(1), bias.data_ptr() if bias is not None else None,
-            h.data_ptr(), m.data_ptr(), m.stride(0), m.stride(1), m.stride(2), ids.data_ptr(), y.data_ptr(), y.stride(0),
+            x.data_ptr(), T, x.stride(0), w.data_ptr(), *w.stride(), bias.data_ptr() if bias is not None else None,
+            h.data_ptr(), m.data_ptr(), *m.stride(), ids.data_ptr(), y.data_ptr(), O,
             n, C, O, r, _lib.DTYPE_CODE[x.dtype], _lib.path_flags() | (_lib.FLAG_AFTER_SHRINK if after_shrink else 0),
             _lib.status_word(x.device).data_ptr(), _lib.stream_ptr(x.device))
     _lib.check(rc, "smoe_adapter_linear")
@@ -155,7 +155,7 @@ class AdapterLinear_(torch.autograd.Function):
         # the gradients of the adapters need the rows sorted by adapter; the shrinks of both directions profit from it
         sorted_idx = offsets = None
         if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
-            _, sorted_idx, offsets = flatten_sort_count(ids, lora_a.size(0))
+            _, sorted_idx, offsets = _pick(sort_count_compileable, _sort_count_impl)(ids, lora_a.size(0))
         h = _pick(shrink_compileable, _shrink_impl)(x, lora_a, ids, scaling, scale, sorted_idx, offsets)
         y = _linear(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids, after_shrink=True)
         ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scaling, h, sorted_idx, offsets)
@@ -215,9 +215,15 @@ def adapter_linear(inputs, weight, lora_a, lora_b, adapter_idxs, scaling=1.0, bi
     assert bias is None or tuple(bias.shape) == (out,), "%s: bias %s" % (what, tuple(bias.shape))
     if inputs.dtype not in _lib.DTYPE_CODE:
         raise RuntimeError("%s: %s is not one of fp32, bf16, fp16" % (what, inputs.dtype))
+    dtype, dev = inputs.dtype, inputs.device
     for name, t in (("weight", weight), ("lora_a", lora_a), ("lora_b", lora_b), ("bias", bias)):
-        if t is not None and t.dtype != inputs.dtype:
-            raise RuntimeError("%s: `%s` is %s, the inputs are %s" % (what, name, t.dtype, inputs.dtype))
+        if t is not None:
+            if t.dtype != dtype:
+                raise RuntimeError("%s: `%s` is %s, the inputs are %s" % (what, name, t.dtype, dtype))
+            if t.device != dev:
+                raise RuntimeError("%s: `%s` is on %s, the inputs are on %s" % (what, name, t.device, dev))
+    if adapter_idxs.device != dev:
+        raise RuntimeError("%s: `adapter_idxs` is on %s, the inputs are on %s" % (what, adapter_idxs.device, dev))
     if adapter_idxs.dtype not in (torch.int64, torch.int32):
         raise RuntimeError("%s: adapter_idxs are %s, not integers of 64 or 32 bits" % (what, adapter_idxs.dtype))
     per_adapter = None
@@ -225,16 +231,25 @@ def adapter_linear(inputs, weight, lora_a, lora_b, adapter_idxs, scaling=1.0, bi
         assert tuple(scaling.shape) == (n,), "%s: scaling %s for %d adapters" % (what, tuple(scaling.shape), n)
         if scaling.requires_grad:
             raise RuntimeError("%s: `scaling` is a constant, it cannot require a gradient" % what)
+        if scaling.device != dev:
+            raise RuntimeError("%s: `scaling` is on %s, the inputs are on %s" % (what, scaling.device, dev))
         per_adapter, scaling = scaling.float().contiguous(), 1.0
-    for name, t in (("weight", weight), ("lora_a", lora_a), ("lora_b", lora_b), ("bias", bias), ("adapter_idxs", adapter_idxs),
-                    ("scaling", per_adapter)):
-        if t is not None and t.device != inputs.device:
-            raise RuntimeError("%s: `%s` is on %s, the inputs are on %s" % (what, name, t.device, inputs.device))
     lead = inputs.shape[:-1]
-    ids = adapter_idxs.reshape(-1).to(torch.int64).contiguous()
-    y = AdapterLinear_.apply(inputs.reshape(-1, width), weight, lora_a, lora_b, ids, per_adapter, float(scaling),
-                             bias.contiguous() if bias is not None else None)
-    return y.view(*lead, out)
+    x = inputs if inputs.dim() == 2 else inputs.reshape(-1, width)
+    ids = adapter_idxs.reshape(-1)
+    if ids.dtype != torch.int64:
+        ids = ids.to(torch.int64)
+    ids = ids.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    leaves = (x, weight, lora_a, lora_b, bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves) or torch.compiler.is_compiling():
+        y = AdapterLinear_.apply(x, weight, lora_a, lora_b, ids, per_adapter, float(scaling), bias)
+    else:      # no graph to build
+        x = _rowmajor(x)
+        h = _shrink_impl(x, lora_a, ids, per_adapter, float(scaling), None, None)
+        y = _linear_impl(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids, after_shrink=True)
+    return y if len(lead) == 1 else y.view(*lead, out)
 
 
 class AdapterLinear(nn.Module):

@@ -27,23 +27,33 @@ MAX_SLOTS = 1024
 MAX_EXPERTS = 1024
 
 
+_max_tokens = None
+
+
 def max_tokens() -> int:
-    return _lib.load().smoe_few_token_max_tokens()
+    global _max_tokens
+    if _max_tokens is None:
+        _max_tokens = _lib.load().smoe_few_token_max_tokens()
+    return _max_tokens
 
 
 def _refuse_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("%s has no backward pass: call it under torch.no_grad(), or use expert_mlp for training" % what)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("%s has no backward pass: call it under torch.no_grad(), or use expert_mlp for training" % what)
 
 
 def _same(what, x, **tensors):
+    """Operands on the tokens' device and, the router's outputs apart, of their dtype."""
+    dev, dtype = x.device, x.dtype
     for name, t in tensors.items():
         if t is None:
             continue
-        if t.device != x.device:
-            raise RuntimeError("%s: `%s` is on %s, the tokens are on %s" % (what, name, t.device, x.device))
-        if name not in ("gates", "expert_idxs") and t.dtype != x.dtype:
-            raise RuntimeError("%s: `%s` is %s, the tokens are %s" % (what, name, t.dtype, x.dtype))
+        if t.device != dev:
+            raise RuntimeError("%s: `%s` is on %s, the tokens are on %s" % (what, name, t.device, dev))
+        if t.dtype != dtype and name not in ("gates", "expert_idxs"):
+            raise RuntimeError("%s: `%s` is %s, the tokens are %s" % (what, name, t.dtype, dtype))
 
 
 def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Optional[torch.Tensor], ids: torch.Tensor,
@@ -60,13 +70,13 @@ def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Opti
     null = (None, 0, 0)
     with _lib.on_device_of(dev):
         rc = lib.smoe_few_token_mlp(
-            x.data_ptr(), T, x.stride(0), up.data_ptr(), up.stride(0), up.stride(1), up.stride(2),
-            *((up_b.data_ptr(), up_b.stride(0), up_b.stride(1)) if up_b is not None else null),
-            down.data_ptr(), down.stride(0), down.stride(1), down.stride(2),
-            *((down_b.data_ptr(), down_b.stride(0), down_b.stride(1)) if down_b is not None else null),
-            *((gates.data_ptr(), gates.stride(0), gates.stride(1), _lib.DTYPE_CODE[gates.dtype]) if gates is not None
+            x.data_ptr(), T, x.stride(0), up.data_ptr(), *up.stride(),
+            *((up_b.data_ptr(), *up_b.stride()) if up_b is not None else null),
+            down.data_ptr(), *down.stride(),
+            *((down_b.data_ptr(), *down_b.stride()) if down_b is not None else null),
+            *((gates.data_ptr(), *gates.stride(), _lib.DTYPE_CODE[gates.dtype]) if gates is not None
               else (None, 0, 0, 0)),
-            ids.data_ptr(), ids.stride(0), ids.stride(1), y.data_ptr(), y.stride(0), k, d, F, d_out, E, act_layout, act,
+            ids.data_ptr(), *ids.stride(), y.data_ptr(), d_out, k, d, F, d_out, E, act_layout, act,
             alpha, limit, _lib.DTYPE_CODE[x.dtype], _lib.path_flags() | (_lib.FLAG_AFTER_ROUTER if after_router else 0),
             ws.data_ptr(), ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_few_token_mlp")
@@ -92,7 +102,7 @@ def _check_mlp(what, x, up, down, act_layout, act, up_b, down_b):
     assert 0 <= act_layout <= 3 and 0 <= act <= 4, "%s: layout %s / function %s" % (what, act_layout, act)
     E, F = down.size(0), down.size(1)
     n_up = F if act_layout == _act.LAYOUT_PLAIN else 2 * F
-    assert tuple(up.shape) == (E, x.size(1), n_up), "%s: up-projection %s, expected %s" % (
+    assert up.shape == (E, x.size(1), n_up), "%s: up-projection %s, expected %s" % (
         what, tuple(up.shape), (E, x.size(1), n_up))
     assert E <= MAX_EXPERTS, "%s: %d experts, at most %d are taken" % (what, E, MAX_EXPERTS)
     assert up_b is None or tuple(up_b.shape) == (E, n_up), "%s: bias of the up-projection %s" % (what, tuple(up_b.shape))
@@ -109,7 +119,7 @@ def _check_slots(what, T, k):
 
 
 def _rows(t):
-    return t if t.stride(-1) == 1 or t.size(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 else t.contiguous()
 
 
 def _run_mlp(x, up, down, gates, ids, act_layout, act, up_b, down_b, alpha, limit, after_router=False):
@@ -143,8 +153,8 @@ def few_token_mlp(inputs, up_weights, down_weights, gates, expert_idxs, act_layo
     _check_slots(what, inputs.size(0), expert_idxs.size(1))
     if inputs.size(0) == 0:
         return inputs.new_empty((0, down_weights.size(2)))
-    return _run_mlp(_rows(inputs), up_weights, down_weights, gates, expert_idxs.to(torch.int64), act_layout, act, up_biases,
-                    down_biases, alpha, limit)
+    ids = expert_idxs if expert_idxs.dtype == torch.int64 else expert_idxs.to(torch.int64)
+    return _run_mlp(_rows(inputs), up_weights, down_weights, gates, ids, act_layout, act, up_biases, down_biases, alpha, limit)
 
 
 def _route_impl(x: torch.Tensor, wr: torch.Tensor, br: Optional[torch.Tensor], k: int, mode: int,
