@@ -42,10 +42,8 @@ enum smoe_flags {
   SMOE_FLAG_FORCE_SIMT = 2,   /* take the CUDA-core kernel even where a tensor-core kernel exists */
   SMOE_FLAG_FORCE_TC = 4,     /* fail with SMOE_ERR_UNSUPPORTED instead of taking the CUDA-core kernel */
   SMOE_FLAG_GATHER_ROWS = 8,  /* feed grouped inputs through the row-gather path too (testing / comparison) */
-  SMOE_FLAG_AFTER_ROUTER = 16, /* smoe_few_token_mlp: the call just before on this stream is the smoe_few_token_route that
+  SMOE_FLAG_AFTER_ROUTER = 16 /* smoe_few_token_mlp: the call just before on this stream is the smoe_few_token_route that
                                  writes expert_idxs and gates; the kernels may be scheduled while it still runs */
-  SMOE_FLAG_AFTER_SHRINK = 32 /* smoe_adapter_linear: the call just before on this stream is the smoe_adapter_shrink that
-                                 writes H, and only H comes from it: the kernel may read the rest while it still runs */
 };
 
 int smoe_version(void);
@@ -261,32 +259,33 @@ int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void
                          int64_t* expert_idxs, float* gates, int32_t dtype, void* stream);
 
 /* ---- low-rank adapters of many requests beside a shared projection (no counterpart in the reference) ---------------------
- * Each row names its adapter a = adapter_idxs[t]; ids outside [0, n) mean none. Three products make both directions:
- * smoe_adapter_shrink:  H[t, j] = s_a sum_c X[t, c] M[a][j, c]     zero rows without an adapter;
- *     s_a = scaling[a], or `scale` where `scaling` is null. M: lora_a forward, lora_b seen as (n, r, out) backward. H is
- *     (T, R) contiguous in `dtype`, R = r rounded up to a multiple of 8, the padding written as zeros. `sorted_idx` and
- *     `offsets` (nullable, both or neither) are smoe_sort_count's of adapter_idxs: rows in no order then cost no more than
- *     rows in runs.
- * smoe_adapter_linear:  Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum_j H[t, j] M[a][j, o]      (bias nullable, contiguous)
- * smoe_adapter_grad:    D[a][j, c] = sum over the rows t of adapter a of U[t, j] V[t, c], U as H above, rows listed by
- *     smoe_sort_count of adapter_idxs (sorted_scattered_idxs, expert_offsets); every element of D is written.
- * smoe_column_sum:      out[c] = sum_t V[t, c]   (the bias's gradient). Fixed summation order everywhere.
- * X, Y, V rows have inner stride 1; W, M, D in element strides. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31. Workspaces (16-byte
- * aligned, sized by the queries) belong to the call until its work has finished. */
-int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma, int64_t stride_mj,
-                        int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling, float scale, void* H, int32_t n,
-                        int32_t C, int32_t r, int32_t dtype, const int64_t* sorted_idx, const int64_t* offsets, void* stream);
-int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk, int64_t stride_wn,
-                        const void* bias, const void* H, const void* M, int64_t stride_ma, int64_t stride_mj,
-                        int64_t stride_mo, const int64_t* adapter_idxs, void* Y, int64_t stride_ym, int32_t n, int32_t C,
-                        int32_t O, int32_t r, int32_t dtype, int32_t flags, int32_t* status, void* stream);
-size_t smoe_adapter_grad_workspace_bytes(int64_t T, int32_t C, int32_t r);
-int smoe_adapter_grad(const void* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
-                      const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc, int32_t n,
-                      int32_t C, int32_t r, int32_t dtype, void* workspace, size_t workspace_bytes, void* stream);
-size_t smoe_column_sum_workspace_bytes(int64_t T, int32_t C);
-int smoe_column_sum(const void* V, int64_t T, int64_t stride_vm, int32_t C, void* out, int32_t dtype, void* workspace,
-                    size_t workspace_bytes, void* stream);
+ * Each row names its adapter a = adapter_idxs[t]; ids outside [0, n) mean none (H row 0, no term).
+ * forward:   H[t] = s_a A[a] X[t];   Y[t] = W X[t] + bias + B[a] H[t]
+ *     s_a = scaling[a], or `scale` where `scaling` is null; bias nullable, contiguous. With sorted_idx (T) and offsets (n) (both or
+ *     neither) the call first sorts the rows by adapter as smoe_sort_count does and hands the lists out: backward needs
+ *     them, and rows in no order then cost no more than rows in runs.
+ * backward:  G[t] = s_a B[a]^T DY[t];   DX[t] = W^T DY[t] + A[a]^T G[t];   DA[a] = sum G[t] X[t]^T;   DB[a] = sum DY[t] H[t]^T over
+ *     the adapter's rows (zeros without rows);   Dbias = sum DY[t].   Each of DX, DA, DB, Dbias may be null. H, sorted_idx and
+ *     offsets are forward's. Every sum has a fixed order.
+ * W (out, in), A (n, r, in), B (n, out, r) in element strides; X, DY rows with inner stride 1; Y, DX (T, .), H (T, r rounded up
+ * to a multiple of 8, in `dtype`), DA, DB, Dbias contiguous. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31 - 64. The workspace (16-byte aligned,
+ * smoe_adapter_workspace_bytes; forward without a sort needs none) belongs to the call until its work has finished. */
+size_t smoe_adapter_workspace_bytes(int64_t T, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype);
+int smoe_adapter_forward(const void* X, int64_t T, int64_t stride_xm,
+                         const void* W, int64_t stride_wo, int64_t stride_wi, const void* bias,
+                         const void* A, int64_t stride_aa, int64_t stride_aj, int64_t stride_ai,
+                         const void* B, int64_t stride_ba, int64_t stride_bo, int64_t stride_bj,
+                         const int64_t* adapter_idxs, const float* scaling, float scale, void* Y, void* H,
+                         int64_t* sorted_idx, int64_t* offsets, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype,
+                         int32_t flags, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+int smoe_adapter_backward(const void* DY, int64_t T, int64_t stride_dym, const void* X, int64_t stride_xm,
+                          const void* W, int64_t stride_wo, int64_t stride_wi,
+                          const void* A, int64_t stride_aa, int64_t stride_aj, int64_t stride_ai,
+                          const void* B, int64_t stride_ba, int64_t stride_bo, int64_t stride_bj,
+                          const int64_t* adapter_idxs, const float* scaling, float scale, const void* H,
+                          const int64_t* sorted_idx, const int64_t* offsets, void* DX, void* DA, void* DB, void* Dbias,
+                          int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype, int32_t flags,
+                          void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- expert-parallel row exchange over NVLink peer memory -----------------------------------------------
  * No counterpart in the reference (it has no multi-GPU code). `peer_*` arguments are HOST arrays of `world` device

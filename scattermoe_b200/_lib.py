@@ -29,7 +29,6 @@ FLAG_FORCE_SIMT = 2
 FLAG_FORCE_TC = 4
 FLAG_GATHER_ROWS = 8
 FLAG_AFTER_ROUTER = 16
-FLAG_AFTER_SHRINK = 32
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -103,14 +102,11 @@ SIGNATURES = {
                             _I32, _I32, _I32, _I32, _I32,    # k d F d_out E
                             _I32, _I32, c_float, c_float, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
     "smoe_few_token_route": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _I32, _P], c_int32),
-    "smoe_adapter_shrink": ([_P, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float, _P, _I32, _I32, _I32, _I32, _P, _P, _P],
-                            c_int32),
-    "smoe_adapter_linear": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32,
-                             _I32, _I32, _P, _P], c_int32),
-    "smoe_adapter_grad_workspace_bytes": ([_I64, _I32, _I32], c_size_t),
-    "smoe_adapter_grad": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, c_size_t, _P], c_int32),
-    "smoe_column_sum_workspace_bytes": ([_I64, _I32], c_size_t),
-    "smoe_column_sum": ([_P, _I64, _I64, _I32, _P, _I32, _P, c_size_t, _P], c_int32),
+    "smoe_adapter_workspace_bytes": ([_I64, _I32, _I32, _I32, _I32, _I32], c_size_t),
+    "smoe_adapter_forward": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float,
+                              _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
+    "smoe_adapter_backward": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float,
+                               _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
 }
 
 

@@ -21,131 +21,95 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import kernels
-from .parallel_experts import _rowmajor, _sort_count_impl, sort_count_compileable
+from .parallel_experts import _rowmajor
 
 MAX_RANK = 256
 MAX_ADAPTERS = 4096
 
 
-def _padded(r: int) -> int:
-    return (r + 7) // 8 * 8
-
-
-def _shrink_impl(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float,
-                 sorted_idx: Optional[torch.Tensor], offsets: Optional[torch.Tensor]) -> torch.Tensor:
-    """h[t, j] = s sum_c x[t, c] m[ids[t], j, c], (T, r padded to a multiple of 8); zero rows for ids outside [0, n)."""
-    T = x.size(0)
-    n, r, C = m.shape
-    h = torch.empty((T, _padded(r)), dtype=x.dtype, device=x.device)
-    with _lib.on_device_of(x.device):
-        rc = _lib.load().smoe_adapter_shrink(
-            x.data_ptr(), T, x.stride(0), m.data_ptr(), *m.stride(), ids.data_ptr(),
-            scaling.data_ptr() if scaling is not None else None, scale, h.data_ptr(), n, C, r, _lib.DTYPE_CODE[x.dtype],
-            sorted_idx.data_ptr() if sorted_idx is not None else None, offsets.data_ptr() if offsets is not None else None,
-            _lib.stream_ptr(x.device))
-    _lib.check(rc, "smoe_adapter_shrink")
-    return h
-
-
-def _linear_impl(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], h: torch.Tensor, m: torch.Tensor,
-                 ids: torch.Tensor, after_shrink: bool = False) -> torch.Tensor:
-    """y = x w + bias + h m[ids]; w is (C, O), m is (n, r, O), any strides."""
-    T, C = x.shape
-    O = w.size(1)
-    n, r, _ = m.shape
-    y = torch.empty((T, O), dtype=x.dtype, device=x.device)
-    with _lib.on_device_of(x.device):
-        rc = _lib.load().smoe_adapter_linear(
-            x.data_ptr(), T, x.stride(0), w.data_ptr(), *w.stride(), bias.data_ptr() if bias is not None else None,
-            h.data_ptr(), m.data_ptr(), *m.stride(), ids.data_ptr(), y.data_ptr(), O,
-            n, C, O, r, _lib.DTYPE_CODE[x.dtype], _lib.path_flags() | (_lib.FLAG_AFTER_SHRINK if after_shrink else 0),
-            _lib.status_word(x.device).data_ptr(), _lib.stream_ptr(x.device))
-    _lib.check(rc, "smoe_adapter_linear")
-    return y
-
-
-def _grad_impl(u: torch.Tensor, v: torch.Tensor, r: int, sorted_idx: torch.Tensor, offsets: torch.Tensor,
-               transposed: bool) -> torch.Tensor:
-    """d[a] = sum over the rows t of adapter a of u[t, :r]^T v[t]: (n, r, C), or its transpose (n, C, r)."""
-    n, C = offsets.size(0), v.size(1)
+def _forward_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], lora_a: torch.Tensor, lora_b: torch.Tensor,
+                  ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float, sort: bool) -> tuple[
+                      torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, h, sorted_idx, offsets): the output, the rows of the rank, and (empty unless `sort`) the rows sorted by adapter."""
+    T, width = x.shape
+    out = weight.size(0)
+    n, r, _ = lora_a.shape
+    dev, dtype = x.device, _lib.DTYPE_CODE[x.dtype]
     lib = _lib.load()
-    ws_bytes = lib.smoe_adapter_grad_workspace_bytes(u.size(0), C, r)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=v.device)
-    d = torch.empty((n, C, r) if transposed else (n, r, C), dtype=v.dtype, device=v.device)
-    view = d.transpose(1, 2) if transposed else d
-    with _lib.on_device_of(v.device):
-        rc = lib.smoe_adapter_grad(
-            u.data_ptr(), u.size(0), v.data_ptr(), v.stride(0), sorted_idx.data_ptr(), offsets.data_ptr(), d.data_ptr(),
-            view.stride(0), view.stride(1), view.stride(2), n, C, r, _lib.DTYPE_CODE[v.dtype], ws.data_ptr(), ws_bytes,
-            _lib.stream_ptr(v.device))
-    _lib.check(rc, "smoe_adapter_grad")
-    return d
+    y = torch.empty((T, out), dtype=x.dtype, device=dev)
+    h = torch.empty((T, (r + 7) // 8 * 8), dtype=x.dtype, device=dev)
+    lists = torch.empty(T + n if sort else 0, dtype=torch.int64, device=dev)
+    sorted_idx, offsets = (lists[:T], lists[T:]) if sort else (lists, lists)
+    ws_bytes = lib.smoe_adapter_workspace_bytes(T, n, width, out, r, dtype) if sort else 0
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if sort else None
+    with _lib.on_device_of(dev):
+        rc = lib.smoe_adapter_forward(
+            x.data_ptr(), T, x.stride(0), weight.data_ptr(), *weight.stride(), bias.data_ptr() if bias is not None else None,
+            lora_a.data_ptr(), *lora_a.stride(), lora_b.data_ptr(), *lora_b.stride(), ids.data_ptr(),
+            scaling.data_ptr() if scaling is not None else None, scale, y.data_ptr(), h.data_ptr(),
+            lists.data_ptr() if sort else None, offsets.data_ptr() if sort else None, n, width, out, r, dtype, _lib.path_flags(),
+            ws.data_ptr() if sort else None, ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc, "smoe_adapter_forward")
+    return y, h, sorted_idx, offsets
 
 
-def _column_sum_impl(v: torch.Tensor) -> torch.Tensor:
-    T, C = v.shape
+def _backward_impl(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                   ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float, h: torch.Tensor, sorted_idx: torch.Tensor,
+                   offsets: torch.Tensor, need_x: bool, need_a: bool, need_b: bool, need_bias: bool) -> tuple[
+                       torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(d_x, d_a, d_b, d_bias), empty where not needed."""
+    T, width = x.shape
+    out = weight.size(0)
+    n, r, _ = lora_a.shape
+    dev, dtype = x.device, _lib.DTYPE_CODE[x.dtype]
     lib = _lib.load()
-    out = torch.empty((C,), dtype=v.dtype, device=v.device)
-    ws_bytes = lib.smoe_column_sum_workspace_bytes(T, C)
-    ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=v.device)
-    with _lib.on_device_of(v.device):
-        rc = lib.smoe_column_sum(v.data_ptr(), T, v.stride(0), C, out.data_ptr(), _lib.DTYPE_CODE[v.dtype], ws.data_ptr(), ws_bytes,
-                                 _lib.stream_ptr(v.device))
-    _lib.check(rc, "smoe_column_sum")
-    return out
+
+    def result(wanted, *shape):
+        return torch.empty(shape if wanted else (0,), dtype=x.dtype, device=dev)
+
+    d_x, d_a, d_b, d_bias = (result(need_x, T, width), result(need_a, n, r, width), result(need_b, n, out, r), result(need_bias, out))
+    ws_bytes = lib.smoe_adapter_workspace_bytes(T, n, width, out, r, dtype)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    with _lib.on_device_of(dev):
+        rc = lib.smoe_adapter_backward(
+            dy.data_ptr(), T, dy.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(), *weight.stride(), lora_a.data_ptr(),
+            *lora_a.stride(), lora_b.data_ptr(), *lora_b.stride(), ids.data_ptr(), scaling.data_ptr() if scaling is not None else None,
+            scale, h.data_ptr(), sorted_idx.data_ptr() or None, offsets.data_ptr() or None, d_x.data_ptr() or None,
+            d_a.data_ptr() or None, d_b.data_ptr() or None, d_bias.data_ptr() or None, n, width, out, r, dtype, _lib.path_flags(),
+            ws.data_ptr(), ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+    _lib.check(rc, "smoe_adapter_backward")
+    return d_x, d_a, d_b, d_bias
 
 
 # The registered forms are used while torch.compile traces, as everywhere in this package.
-@torch.library.custom_op("scattermoe_b200::adapter_shrink", mutates_args={})
-def shrink_compileable(x: torch.Tensor, m: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float,
-                       sorted_idx: Optional[torch.Tensor], offsets: Optional[torch.Tensor]) -> torch.Tensor:
-    return _shrink_impl(x, m, ids, scaling, scale, sorted_idx, offsets)
+@torch.library.custom_op("scattermoe_b200::adapter_forward", mutates_args={})
+def forward_compileable(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor], lora_a: torch.Tensor,
+                        lora_b: torch.Tensor, ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float, sort: bool) -> tuple[
+                            torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    y, h, sorted_idx, offsets = _forward_impl(x, weight, bias, lora_a, lora_b, ids, scaling, scale, sort)
+    return y, h, sorted_idx.clone(), offsets.clone()      # outputs of a registered operator do not share memory
 
 
-@shrink_compileable.register_fake
-def _(x, m, ids, scaling, scale, sorted_idx, offsets):
-    return torch.empty((x.size(0), _padded(m.size(1))), dtype=x.dtype, device=x.device)
+@forward_compileable.register_fake
+def _(x, weight, bias, lora_a, lora_b, ids, scaling, scale, sort):
+    T, n, r = x.size(0), lora_a.size(0), lora_a.size(1)
+    i64 = dict(dtype=torch.int64, device=x.device)
+    return (x.new_empty((T, weight.size(0))), x.new_empty((T, (r + 7) // 8 * 8)), torch.empty(T if sort else 0, **i64),
+            torch.empty(n if sort else 0, **i64))
 
 
-@torch.library.custom_op("scattermoe_b200::adapter_linear", mutates_args={})
-def linear_compileable(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], h: torch.Tensor, m: torch.Tensor,
-                       ids: torch.Tensor) -> torch.Tensor:
-    return _linear_impl(x, w, bias, h, m, ids)
+@torch.library.custom_op("scattermoe_b200::adapter_backward", mutates_args={})
+def backward_compileable(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                         ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float, h: torch.Tensor,
+                         sorted_idx: torch.Tensor, offsets: torch.Tensor, need_x: bool, need_a: bool, need_b: bool,
+                         need_bias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _backward_impl(dy, x, weight, lora_a, lora_b, ids, scaling, scale, h, sorted_idx, offsets, need_x, need_a, need_b, need_bias)
 
 
-@linear_compileable.register_fake
-def _(x, w, bias, h, m, ids):
-    return torch.empty((x.size(0), w.size(1)), dtype=x.dtype, device=x.device)
-
-
-@torch.library.custom_op("scattermoe_b200::adapter_grad", mutates_args={})
-def grad_compileable(u: torch.Tensor, v: torch.Tensor, r: int, sorted_idx: torch.Tensor, offsets: torch.Tensor,
-                     transposed: bool) -> torch.Tensor:
-    return _grad_impl(u, v, r, sorted_idx, offsets, transposed)
-
-
-@grad_compileable.register_fake
-def _(u, v, r, sorted_idx, offsets, transposed):
-    n, C = offsets.size(0), v.size(1)
-    return torch.empty((n, C, r) if transposed else (n, r, C), dtype=v.dtype, device=v.device)
-
-
-@torch.library.custom_op("scattermoe_b200::column_sum", mutates_args={})
-def column_sum_compileable(v: torch.Tensor) -> torch.Tensor:
-    return _column_sum_impl(v)
-
-
-@column_sum_compileable.register_fake
-def _(v):
-    return torch.empty((v.size(1),), dtype=v.dtype, device=v.device)
-
-
-def _pick(compiled, direct):
-    return compiled if torch.compiler.is_compiling() else direct
-
-
-def _linear(*args, after_shrink):
-    return linear_compileable(*args) if torch.compiler.is_compiling() else _linear_impl(*args, after_shrink=after_shrink)
+@backward_compileable.register_fake
+def _(dy, x, weight, lora_a, lora_b, ids, scaling, scale, h, sorted_idx, offsets, need_x, need_a, need_b, need_bias):
+    return (x.new_empty(x.shape if need_x else (0,)), x.new_empty(lora_a.shape if need_a else (0,)),
+            x.new_empty(lora_b.shape if need_b else (0,)), x.new_empty((weight.size(0) if need_bias else 0,)))
 
 
 class AdapterLinear_(torch.autograd.Function):
@@ -153,11 +117,9 @@ class AdapterLinear_(torch.autograd.Function):
     def forward(ctx, x, weight, lora_a, lora_b, ids, scaling, scale, bias):
         x = _rowmajor(x)
         # the gradients of the adapters need the rows sorted by adapter; the shrinks of both directions profit from it
-        sorted_idx = offsets = None
-        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
-            _, sorted_idx, offsets = _pick(sort_count_compileable, _sort_count_impl)(ids, lora_a.size(0))
-        h = _pick(shrink_compileable, _shrink_impl)(x, lora_a, ids, scaling, scale, sorted_idx, offsets)
-        y = _linear(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids, after_shrink=True)
+        sort = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+        run = forward_compileable if torch.compiler.is_compiling() else _forward_impl
+        y, h, sorted_idx, offsets = run(x, weight, bias, lora_a, lora_b, ids, scaling, scale, sort)
         ctx.save_for_backward(x, weight, lora_a, lora_b, ids, scaling, h, sorted_idx, offsets)
         ctx.scale = scale
         return y
@@ -171,26 +133,21 @@ class AdapterLinear_(torch.autograd.Function):
         dy = _rowmajor(dy)
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
-        d_x = d_w = d_a = d_b = d_bias = None
-        if need_x or need_a:
-            g = _pick(shrink_compileable, _shrink_impl)(dy, lora_b.transpose(1, 2), ids, scaling, ctx.scale, sorted_idx, offsets)
-        if need_x:
-            d_x = _linear(dy, weight, None, g, lora_a, ids, after_shrink=True)
-        if need_a or need_b:
-            grad = _pick(grad_compileable, _grad_impl)
-            if need_a:
-                d_a = grad(g, x, lora_a.size(1), sorted_idx, offsets, False)
-            if need_b:
-                d_b = grad(h, dy, lora_a.size(1), sorted_idx, offsets, True)
+        d_w = d_bias_w = None
         if need_w:
             rows = torch.full((1,), x.size(0), dtype=torch.int64, device=x.device)
             d_w, db = kernels.ops.group_bwd_W(DY=dy, X=x, expert_offsets=rows, E=1, has_bias=need_bias)
             d_w = d_w[0].t()
             if need_bias:
-                d_bias = db[0]
-        elif need_bias:
-            d_bias = _pick(column_sum_compileable, _column_sum_impl)(dy)
-        return d_x, d_w, d_a, d_b, None, None, None, d_bias
+                d_bias_w = db[0]
+        d_x = d_a = d_b = d_bias = None
+        own_bias = need_bias and not need_w
+        if need_x or need_a or need_b or own_bias:
+            run = backward_compileable if torch.compiler.is_compiling() else _backward_impl
+            d_x, d_a, d_b, d_bias = run(dy, x, weight, lora_a, lora_b, ids, scaling, ctx.scale, h, sorted_idx, offsets, need_x, need_a,
+                                        need_b, own_bias)
+        return (d_x if need_x else None, d_w, d_a if need_a else None, d_b if need_b else None, None, None, None,
+                d_bias if own_bias else d_bias_w)
 
 
 def adapter_linear(inputs, weight, lora_a, lora_b, adapter_idxs, scaling=1.0, bias=None):
@@ -246,9 +203,7 @@ def adapter_linear(inputs, weight, lora_a, lora_b, adapter_idxs, scaling=1.0, bi
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in leaves) or torch.compiler.is_compiling():
         y = AdapterLinear_.apply(x, weight, lora_a, lora_b, ids, per_adapter, float(scaling), bias)
     else:      # no graph to build
-        x = _rowmajor(x)
-        h = _shrink_impl(x, lora_a, ids, per_adapter, float(scaling), None, None)
-        y = _linear_impl(x, weight.t(), bias, h, lora_b.transpose(1, 2), ids, after_shrink=True)
+        y = _forward_impl(_rowmajor(x), weight, bias, lora_a, lora_b, ids, per_adapter, float(scaling), False)[0]
     return y if len(lead) == 1 else y.view(*lead, out)
 
 

@@ -236,89 +236,55 @@ static int launch_linear_few(const LinearArgs& a) {
   f.stream = a.stream;
   const bool aligned = (reinterpret_cast<uintptr_t>(a.M) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.H) & 15) == 0;
   ft::Extension x{a.H, rank_pitch(a.r), a.M, a.sma, a.smj, a.smo, a.ids, a.n, a.r,
-                  a.smj == 1 && a.smo % 8 == 0 && a.sma % 8 == 0 && a.r % 8 == 0 && aligned ? 1 : 0, a.after_shrink};
+                  a.smj == 1 && a.smo % 8 == 0 && a.sma % 8 == 0 && a.r % 8 == 0 && aligned ? 1 : 0};
   return ft::launch_linear(f, x);
 }
 
-static int check_common(const char* who, int64_t T, int n, int C, int r, int dtype) {
+static int check_common(const char* who, int64_t T, int n, int in, int out, int r, int dtype) {
   SMOE_CHECK_ARG(dtype == SMOE_F32 || dtype == SMOE_BF16 || dtype == SMOE_F16, "%s: unknown dtype %d", who, dtype);
-  SMOE_CHECK_ARG(T >= 0 && T < (int64_t(1) << 31), "%s: T=%lld out of range [0, 2^31)", who, (long long)T);
+  SMOE_CHECK_ARG(T >= 0 && T < (int64_t(1) << 31) - 64, "%s: T=%lld out of range [0, 2^31 - 64)", who, (long long)T);
   SMOE_CHECK_ARG(n >= 1 && n <= 4096, "%s: %d adapters, 1 to 4096 are taken", who, n);
   SMOE_CHECK_ARG(r >= 1 && r <= MAX_RANK, "%s: rank %d, 1 to %d are taken", who, r, MAX_RANK);
-  SMOE_CHECK_ARG(C >= 1 && C < (1 << 28), "%s: bad width %d", who, C);
+  SMOE_CHECK_ARG(in >= 1 && in < (1 << 28) && out >= 1 && out < (1 << 28), "%s: bad widths in=%d out=%d", who, in, out);
   return SMOE_OK;
 }
 
-}  // namespace ad
-}  // namespace smoe
-
-using namespace smoe;
-
-extern "C" int smoe_adapter_shrink(const void* X, int64_t T, int64_t stride_xm, const void* M, int64_t stride_ma,
-                                   int64_t stride_mj, int64_t stride_mc, const int64_t* adapter_idxs, const float* scaling,
-                                   float scale, void* H, int32_t n, int32_t C, int32_t r, int32_t dtype,
-                                   const int64_t* sorted_idx, const int64_t* offsets, void* stream) {
-  if (int rc = ad::check_common("adapter_shrink", T, n, C, r, dtype)) return rc;
-  if (T == 0) return SMOE_OK;
-  SMOE_CHECK_ARG(X && M && adapter_idxs && H, "adapter_shrink: null pointer");
-  ad::ShrinkArgs a{X, T, stride_xm, M, stride_ma, stride_mj, stride_mc, adapter_idxs, scaling, scale, H, n, C, r, dtype,
-                   offsets ? sorted_idx : nullptr, offsets, static_cast<cudaStream_t>(stream)};
-  const int rc = ad::launch_shrink_tc(a);
-  return rc != SMOE_ERR_UNSUPPORTED ? rc : ad::launch_shrink_simt(a);
+static int shrink(const ShrinkArgs& a, int flags) {
+  if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
+    const int rc = launch_shrink_tc(a);
+    if (rc != SMOE_ERR_UNSUPPORTED) return rc;
+  }
+  return launch_shrink_simt(a);
 }
 
-extern "C" int smoe_adapter_linear(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wk,
-                                   int64_t stride_wn, const void* bias, const void* H, const void* M, int64_t stride_ma,
-                                   int64_t stride_mj, int64_t stride_mo, const int64_t* adapter_idxs, void* Y,
-                                   int64_t stride_ym, int32_t n, int32_t C, int32_t O, int32_t r, int32_t dtype,
-                                   int32_t flags, int32_t* status, void* stream) {
-  if (int rc = ad::check_common("adapter_linear", T, n, C, r, dtype)) return rc;
-  SMOE_CHECK_ARG(O >= 1 && O < (1 << 28), "adapter_linear: bad width %d", O);
-  if (T == 0) return SMOE_OK;
-  SMOE_CHECK_ARG(X && W && H && M && adapter_idxs && Y, "adapter_linear: null pointer");
-  ad::LinearArgs a{X, T, stride_xm, W, stride_wk, stride_wn, bias, H, M, stride_ma, stride_mj, stride_mo, adapter_idxs, Y,
-                   stride_ym, n, C, O, r, dtype, (flags & SMOE_FLAG_AFTER_SHRINK) ? 1 : 0, status, static_cast<cudaStream_t>(stream)};
+static int linear(const LinearArgs& a, int flags) {
   if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
-    int rc = ad::launch_linear_few(a);
-    if (rc == SMOE_ERR_UNSUPPORTED) rc = ad::launch_linear_tc(a);
+    int rc = launch_linear_few(a);
+    if (rc == SMOE_ERR_UNSUPPORTED) rc = launch_linear_tc(a);
     if (rc != SMOE_ERR_UNSUPPORTED) {
       if (rc == SMOE_OK) set_last_path(1);
       return rc;
     }
     if (flags & SMOE_FLAG_FORCE_TC) {
-      set_error("adapter_linear: no tensor-core kernel for this dtype/alignment (dtype=%d in=%d out=%d)", dtype, C, O);
+      set_error("adapter_linear: no tensor-core kernel for this dtype/alignment (dtype=%d in=%d out=%d)", a.dtype, a.C, a.O);
       return rc;
     }
   }
   set_last_path(0);
-  return ad::launch_linear_simt(a);
+  return launch_linear_simt(a);
 }
 
-extern "C" size_t smoe_adapter_grad_workspace_bytes(int64_t T, int32_t C, int32_t r) {
-  if (T < 0 || C < 1 || r < 1) return 0;
-  return ad::grad_workspace_bytes(T, C, r);
-}
-
-extern "C" int smoe_adapter_grad(const void* U, int64_t T, const void* V, int64_t stride_vm, const int64_t* sorted_idx,
-                                 const int64_t* offsets, void* D, int64_t stride_da, int64_t stride_dj, int64_t stride_dc,
-                                 int32_t n, int32_t C, int32_t r, int32_t dtype, void* workspace, size_t workspace_bytes,
-                                 void* stream) {
-  if (int rc = ad::check_common("adapter_grad", T, n, C, r, dtype)) return rc;
-  SMOE_CHECK_ARG(D && offsets && (T == 0 || (U && V && sorted_idx)), "adapter_grad: null pointer");
-  if (workspace == nullptr || workspace_bytes < smoe_adapter_grad_workspace_bytes(T, C, r)) {
-    set_error("adapter_grad: workspace of %zu bytes needed, %zu given", smoe_adapter_grad_workspace_bytes(T, C, r), workspace_bytes);
-    return SMOE_ERR_WORKSPACE;
+static int outer(const GradArgs& a, int flags) {
+  if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
+    const int rc = launch_grad_tc(a);
+    if (rc != SMOE_ERR_UNSUPPORTED) return rc;
   }
-  ad::GradArgs a{U, T, V, stride_vm, sorted_idx, offsets, D, stride_da, stride_dj, stride_dc, n, C, r, dtype,
-                 workspace, workspace_bytes, static_cast<cudaStream_t>(stream)};
-  const int rc = ad::launch_grad_tc(a);
-  return rc != SMOE_ERR_UNSUPPORTED ? rc : ad::launch_grad_simt(a);
+  return launch_grad_simt(a);
 }
+
+static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 // ---- column sums (the shared bias's gradient): fp32 partial sums over slices of the rows, added up in order ----
-namespace smoe {
-namespace ad {
-
 constexpr int SUM_COLS = 256, SUM_MAX_SLICES = 64;
 
 static int sum_slices(int64_t T, int C) {
@@ -356,28 +322,103 @@ column_total_kernel(const float* __restrict__ partial, int slices, int C, T* __r
   out[c] = from_f32<T>(s);
 }
 
+static size_t column_sum_bytes(int64_t T, int C) { return static_cast<size_t>(sum_slices(T, C)) * C * 4; }
+
+static int column_sum(const void* V, int64_t T, int64_t svm, int C, void* out, int dtype, void* ws, cudaStream_t st) {
+  const int slices = sum_slices(T, C);
+  float* partial = static_cast<float*>(ws);
+  dim3 grid(static_cast<unsigned>(cdiv(C, SUM_COLS)), static_cast<unsigned>(slices));
+  SMOE_AD_DTYPE(dtype, column_partial_kernel<T_><<<grid, SUM_COLS, 0, st>>>(static_cast<const T_*>(V), T, svm, C, partial);
+                column_total_kernel<T_><<<grid.x, SUM_COLS, 0, st>>>(partial, slices, C, static_cast<T_*>(out));)
+  SMOE_LAUNCH_CHECK();
+  return SMOE_OK;
+}
+
 }  // namespace ad
 }  // namespace smoe
 
-extern "C" size_t smoe_column_sum_workspace_bytes(int64_t T, int32_t C) {
-  if (T < 0 || C < 1) return 0;
-  return static_cast<size_t>(ad::sum_slices(T, C)) * C * 4;
+using namespace smoe;
+
+// forward: sorted ids and the sort's histograms; backward: g, the outer products' parts, the column sums' parts
+extern "C" size_t smoe_adapter_workspace_bytes(int64_t T, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype) {
+  if (T < 0 || n < 1 || in < 1 || out < 1 || r < 1 || dtype < 0 || dtype > 2) return 0;
+  const size_t forward = ad::up256(static_cast<size_t>(T) * 8) + ad::up256(smoe_sort_count_workspace_bytes(T, n));
+  size_t parts = ad::grad_workspace_bytes(T, in, r);
+  const size_t parts_out = ad::grad_workspace_bytes(T, out, r), sums = ad::column_sum_bytes(T, out);
+  parts = parts > parts_out ? parts : parts_out;
+  parts = parts > sums ? parts : sums;
+  const size_t backward = ad::up256(static_cast<size_t>(T) * ad::rank_pitch(r) * dtype_size(dtype)) + ad::up256(parts);
+  return (forward > backward ? forward : backward) + 256;
 }
 
-extern "C" int smoe_column_sum(const void* V, int64_t T, int64_t stride_vm, int32_t C, void* out, int32_t dtype, void* workspace,
-                               size_t workspace_bytes, void* stream) {
-  if (int rc = ad::check_common("column_sum", T, 1, C, 1, dtype)) return rc;
-  SMOE_CHECK_ARG(out && (T == 0 || V), "column_sum: null pointer");
-  if (workspace == nullptr || workspace_bytes < smoe_column_sum_workspace_bytes(T, C)) {
-    set_error("column_sum: workspace of %zu bytes needed, %zu given", smoe_column_sum_workspace_bytes(T, C), workspace_bytes);
+extern "C" int smoe_adapter_forward(const void* X, int64_t T, int64_t stride_xm, const void* W, int64_t stride_wo,
+                                    int64_t stride_wi, const void* bias, const void* A, int64_t stride_aa, int64_t stride_aj,
+                                    int64_t stride_ai, const void* B, int64_t stride_ba, int64_t stride_bo, int64_t stride_bj,
+                                    const int64_t* adapter_idxs, const float* scaling, float scale, void* Y, void* H,
+                                    int64_t* sorted_idx, int64_t* offsets, int32_t n, int32_t in, int32_t out, int32_t r,
+                                    int32_t dtype, int32_t flags, void* workspace, size_t workspace_bytes, int32_t* status,
+                                    void* stream) {
+  const char* who = "adapter_forward";
+  if (int rc = ad::check_common(who, T, n, in, out, r, dtype)) return rc;
+  SMOE_CHECK_ARG((sorted_idx == nullptr) == (offsets == nullptr), "%s: sorted_idx and offsets go together", who);
+  if (T > 0) SMOE_CHECK_ARG(X && W && A && B && adapter_idxs && Y && H, "%s: null pointer", who);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (offsets) {
+    const size_t need = smoe_adapter_workspace_bytes(T, n, in, out, r, dtype);
+    if (workspace == nullptr || workspace_bytes < need) {
+      set_error("%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+      return SMOE_ERR_WORKSPACE;
+    }
+    int64_t* sorted_ids = static_cast<int64_t*>(workspace);
+    uint8_t* rest = static_cast<uint8_t*>(workspace) + ad::up256(static_cast<size_t>(T) * 8);
+    if (int rc = smoe_sort_count(adapter_idxs, T, n, sorted_ids, sorted_idx, offsets, rest, smoe_sort_count_workspace_bytes(T, n), stream))
+      return rc;
+  }
+  if (T == 0) return SMOE_OK;
+  ad::ShrinkArgs s{X, T, stride_xm, A, stride_aa, stride_aj, stride_ai, adapter_idxs, scaling, scale, H, n, in, r, dtype, sorted_idx, offsets, st};
+  if (int rc = ad::shrink(s, flags)) return rc;
+  ad::LinearArgs l{X, T, stride_xm, W, stride_wi, stride_wo, bias, H, B, stride_ba, stride_bj, stride_bo, adapter_idxs, Y,
+                   out, n, in, out, r, dtype, status, st};
+  return ad::linear(l, flags);
+}
+
+extern "C" int smoe_adapter_backward(const void* DY, int64_t T, int64_t stride_dym, const void* X, int64_t stride_xm, const void* W,
+                                     int64_t stride_wo, int64_t stride_wi, const void* A, int64_t stride_aa, int64_t stride_aj,
+                                     int64_t stride_ai, const void* B, int64_t stride_ba, int64_t stride_bo, int64_t stride_bj,
+                                     const int64_t* adapter_idxs, const float* scaling, float scale, const void* H,
+                                     const int64_t* sorted_idx, const int64_t* offsets, void* DX, void* DA, void* DB,
+                                     void* Dbias, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype, int32_t flags,
+                                     void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+  const char* who = "adapter_backward";
+  if (int rc = ad::check_common(who, T, n, in, out, r, dtype)) return rc;
+  const size_t need = smoe_adapter_workspace_bytes(T, n, in, out, r, dtype);
+  if (workspace == nullptr || workspace_bytes < need) {
+    set_error("%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
     return SMOE_ERR_WORKSPACE;
   }
-  const int slices = ad::sum_slices(T, C);
-  float* partial = static_cast<float*>(workspace);
+  SMOE_CHECK_ARG((!DA && !DB) || (offsets && (T == 0 || sorted_idx)), "%s: the adapters' gradients need the sorted rows", who);
+  if (T > 0) SMOE_CHECK_ARG(DY && X && W && A && B && adapter_idxs && H, "%s: null pointer", who);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  dim3 grid(static_cast<unsigned>(cdiv(C, ad::SUM_COLS)), static_cast<unsigned>(slices));
-  SMOE_AD_DTYPE(dtype, ad::column_partial_kernel<T_><<<grid, ad::SUM_COLS, 0, st>>>(static_cast<const T_*>(V), T, stride_vm, C, partial);
-                ad::column_total_kernel<T_><<<grid.x, ad::SUM_COLS, 0, st>>>(partial, slices, C, static_cast<T_*>(out));)
-  SMOE_LAUNCH_CHECK();
+  void* G = workspace;
+  uint8_t* parts = static_cast<uint8_t*>(workspace) + ad::up256(static_cast<size_t>(T) * ad::rank_pitch(r) * dtype_size(dtype));
+  const size_t parts_bytes = workspace_bytes - (parts - static_cast<uint8_t*>(workspace));
+  if (T > 0 && (DX || DA)) {
+    ad::ShrinkArgs s{DY, T, stride_dym, B, stride_ba, stride_bj, stride_bo, adapter_idxs, scaling, scale, G, n, out, r, dtype, sorted_idx, offsets, st};
+    if (int rc = ad::shrink(s, flags)) return rc;
+  }
+  if (T > 0 && DX) {
+    ad::LinearArgs l{DY, T, stride_dym, W, stride_wo, stride_wi, nullptr, G, A, stride_aa, stride_aj, stride_ai, adapter_idxs, DX,
+                     in, n, out, in, r, dtype, status, st};
+    if (int rc = ad::linear(l, flags)) return rc;
+  }
+  if (DA) {
+    ad::GradArgs g{G, T, X, stride_xm, sorted_idx, offsets, DA, static_cast<int64_t>(r) * in, in, 1, n, in, r, dtype, parts, parts_bytes, st};
+    if (int rc = ad::outer(g, flags)) return rc;
+  }
+  if (DB) {
+    ad::GradArgs g{H, T, DY, stride_dym, sorted_idx, offsets, DB, static_cast<int64_t>(r) * out, 1, r, n, out, r, dtype, parts, parts_bytes, st};
+    if (int rc = ad::outer(g, flags)) return rc;
+  }
+  if (Dbias) return ad::column_sum(DY, T, stride_dym, out, Dbias, dtype, parts, st);
   return SMOE_OK;
 }

@@ -29,6 +29,7 @@ struct ShrinkArgs {           // H[t, j] = s_a sum_c X[t, c] M[a][j, c]
   cudaStream_t stream;
 };
 
+// The launch before on the stream is the shrink that writes H.
 struct LinearArgs {           // Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum_j H[t, j] M[a][j, o]
   const void* X; int64_t T, sxm;
   const void* W; int64_t swk, swn;
@@ -38,7 +39,6 @@ struct LinearArgs {           // Y[t, o] = sum_c X[t, c] W[c, o] + bias[o] + sum
   const int64_t* ids;
   void* Y; int64_t sym;
   int n, C, O, r, dtype;
-  int after_shrink;         // the launch before on this stream is the shrink that writes H
   int32_t* status;
   cudaStream_t stream;
 };

@@ -810,7 +810,7 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (!UP || a.after_router || p.ext.after_shrink) ? 1 : 0;
+  cfg.numAttrs = (!UP || a.after_router || p.ext.ids) ? 1 : 0;
   SMOE_CUDA(cudaLaunchKernelEx(&cfg, ft_stream_kernel<T, UP, KMAJOR>, map, p));
   return SMOE_OK;
 }

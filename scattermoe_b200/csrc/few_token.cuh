@@ -34,13 +34,13 @@ struct Args {
   cudaStream_t stream;
 };
 
-// What an adapter adds to the values of a plain linear (adapter.cuh): sum over j of h[t, j] m[ids[t]][j, o].
+// What an adapter adds to the values of a plain linear (adapter.cuh): sum over j of h[t, j] m[ids[t]][j, o]. The launch before on the
+// stream writes h, and nothing else that the kernel reads.
 struct Extension {
   const void* h; int64_t h_pitch;
   const void* m; int64_t sma, smj, smo;
   const int64_t* ids;      // null: nothing is added
   int n, r, m_vec;
-  int after_shrink;        // the launch before on this stream writes h, and nothing else that is read here
 };
 
 inline int n_up(const Args& a) { return a.act_layout == 0 ? a.F : 2 * a.F; }

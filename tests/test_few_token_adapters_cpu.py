@@ -42,30 +42,32 @@ def test_few_token_route_refuses(bad, word):
 
 
 @pytest.mark.parametrize("bad,word", [(dict(n=0), "adapters"), (dict(n=4097), "adapters"), (dict(r=0), "rank"), (dict(r=257), "rank"),
-                                      (dict(T=-1), "T=-1"), (dict(C=0), "width"), (dict(dtype=3), "dtype"), (dict(X=None), "null")])
+                                      (dict(T=-1), "T=-1"), (dict(width=0), "width"), (dict(out=0), "width"), (dict(dtype=3), "dtype"),
+                                      (dict(X=None), "null"), (dict(H=None), "null")])
 def test_adapter_entry_points_refuse(bad, word):
     lib = _lib.load()
-    shrink = dict(X=256, T=4, sxm=64, M=256, sma=512, smj=64, smc=1, ids=256, scaling=None, scale=1.0, H=256, n=2, C=64, r=8, dtype=1,
-                  sorted_idx=None, offsets=None, stream=None)
-    assert lib.smoe_adapter_shrink(*{**shrink, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
-    linear = dict(X=256, T=4, sxm=64, W=256, swk=1, swn=64, bias=None, H=256, M=256, sma=512, smj=1, smo=8, ids=256, Y=256, sym=64,
-                  n=2, C=64, O=64, r=8, dtype=1, flags=0, status=None, stream=None)
-    assert lib.smoe_adapter_linear(*{**linear, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
-    grad = dict(U=256, T=4, V=256, svm=64, idx=256, off=256, D=256, sda=512, sdj=64, sdc=1, n=2, C=64, r=8, dtype=1, ws=256, ws_bytes=1 << 24, stream=None)
-    bad = {("V" if k == "X" else k): v for k, v in bad.items()}
-    assert lib.smoe_adapter_grad(*{**grad, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
+    forward = dict(X=256, T=4, sxm=64, W=256, swo=64, swi=1, bias=None, A=256, saa=512, saj=64, sai=1, B=256, sba=512, sbo=8, sbj=1,
+                   ids=256, scaling=None, scale=1.0, Y=256, H=256, sorted_idx=None, offsets=None, n=2, width=64, out=64, r=8, dtype=1,
+                   flags=0, ws=None, ws_bytes=0, status=None, stream=None)
+    assert lib.smoe_adapter_forward(*{**forward, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
+    backward = dict(DY=256, T=4, sdy=64, X=256, sxm=64, W=256, swo=64, swi=1, A=256, saa=512, saj=64, sai=1, B=256, sba=512, sbo=8,
+                    sbj=1, ids=256, scaling=None, scale=1.0, H=256, sorted_idx=256, offsets=256, DX=256, DA=256, DB=256, Db=256, n=2,
+                    width=64, out=64, r=8, dtype=1, flags=0, ws=256, ws_bytes=1 << 24, status=None, stream=None)
+    assert lib.smoe_adapter_backward(*{**backward, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
 
 
-def test_column_sum_and_gradient_workspaces():
+def test_adapter_workspaces_and_lists():
     lib = _lib.load()
-    need = lib.smoe_adapter_grad_workspace_bytes(100, 64, 8)
-    assert need > 0
-    assert lib.smoe_adapter_grad(256, 100, 256, 64, 256, 256, 256, 512, 64, 1, 2, 64, 8, 1, 256, need - 1, None) == 4
-    assert "workspace" in _lib.last_error()
-    need = lib.smoe_column_sum_workspace_bytes(100, 64)
-    assert need >= 64 * 4
-    assert lib.smoe_column_sum(256, 100, 64, 64, 256, 1, 256, need - 1, None) == 4
-    assert lib.smoe_column_sum(256, 100, 64, 64, None, 1, 256, need, None) == _lib.SMOE_ERR_BAD_ARG
+    need = lib.smoe_adapter_workspace_bytes(100, 3, 64, 96, 8, 1)
+    assert need > 0 and lib.smoe_adapter_workspace_bytes(-1, 3, 64, 96, 8, 1) == 0
+    tail = [3, 64, 96, 8, 1, 0]
+    head = [256, 100, 64, 256, 64, 1, None, 256, 512, 64, 1, 256, 768, 8, 1, 256, None, 1.0, 256, 256]
+    assert lib.smoe_adapter_forward(*head, 256, 256, *tail, 256, need - 1, None, None) == 4 and "workspace" in _lib.last_error()
+    assert lib.smoe_adapter_forward(*head, 256, None, *tail, 256, need, None, None) == _lib.SMOE_ERR_BAD_ARG
+    head = [256, 100, 96, 256, 64, 256, 64, 1, 256, 512, 64, 1, 256, 768, 8, 1, 256, None, 1.0, 256]
+    assert lib.smoe_adapter_backward(*head, 256, 256, 256, 256, 256, 256, *tail, 256, need - 1, None, None) == 4
+    assert lib.smoe_adapter_backward(*head, None, None, 256, 256, None, None, *tail, 256, need, None, None) == _lib.SMOE_ERR_BAD_ARG
+    assert "sorted" in _lib.last_error()
 
 
 def test_cpu_tensors_fail_loudly():
