@@ -288,7 +288,7 @@ static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 constexpr int SUM_COLS = 256, SUM_MAX_SLICES = 64;
 
 static int sum_slices(int64_t T, int C) {
-  const int64_t by_rows = cdiv64(T, 64), by_grid = cdiv64(148 * 4, cdiv(C, SUM_COLS));
+  const int64_t by_rows = cdiv64(T, 32), by_grid = cdiv64(148 * 8, cdiv(C, SUM_COLS));
   const int64_t s = by_rows < by_grid ? by_rows : by_grid;
   return static_cast<int>(s < 1 ? 1 : (s > SUM_MAX_SLICES ? SUM_MAX_SLICES : s));
 }
@@ -300,16 +300,14 @@ column_partial_kernel(const T* __restrict__ V, int64_t rows, int64_t svm, int C,
   if (c >= C) return;
   const int64_t per = (rows + gridDim.y - 1) / gridDim.y;
   const int64_t beg = min(rows, per * blockIdx.y), end = min(rows, beg + per);
-  float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+  float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   int64_t t = beg;
-  for (; t + 4 <= end; t += 4) {
-    s0 += to_f32<T>(__ldg(V + t * svm + c));
-    s1 += to_f32<T>(__ldg(V + (t + 1) * svm + c));
-    s2 += to_f32<T>(__ldg(V + (t + 2) * svm + c));
-    s3 += to_f32<T>(__ldg(V + (t + 3) * svm + c));
+  for (; t + 8 <= end; t += 8) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] += to_f32<T>(__ldg(V + (t + i) * svm + c));
   }
-  for (; t < end; ++t) s0 += to_f32<T>(__ldg(V + t * svm + c));
-  partial[static_cast<int64_t>(blockIdx.y) * C + c] = (s0 + s1) + (s2 + s3);
+  for (; t < end; ++t) s[0] += to_f32<T>(__ldg(V + t * svm + c));
+  partial[static_cast<int64_t>(blockIdx.y) * C + c] = ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
 }
 
 template <typename T>

@@ -5,7 +5,7 @@
 // A persistent 128 x BN GEMM (TMA -> shared-memory ring -> tcgen05.mma -> tensor memory, double-buffered) whose K loop goes on after W: for
 // every adapter that occurs among the tile's 128 rows, up to 64 of the rank are one more stage. Four warps build it: the rows of H
 // that name the adapter, zeros for the others (so a row only meets its own adapter), and the adapter's slice
-// of M, both in the swizzled layout of the ring. (Zero times infinity is not zero: infinities and NaN of M are left out of the product
+// of M, both in a swizzled layout of the ring. (Zero times infinity is not zero: infinities and NaN of M are left out of the product
 // and added by the epilogue to the rows they belong to, so that one broken adapter leaves its neighbours' rows alone.) One instruction of 16 per stage at rank 16: the expansion adds 1/256 of the product at
 // C = 4096 where a tile's rows share an adapter, and the output is neither read back nor rounded twice.
 // Bound: the tensor cores.
@@ -40,10 +40,13 @@ struct GemmParams {
   const uint8_t* bias;
   uint8_t* Y; int64_t y_row_bytes;
   int64_t T;
-  int n, C, O, r, is_bf16, m_vec, wide_rows, group_m;
+  int n, C, O, r, is_bf16, m_pieces, wide_rows, group_m;
   uint32_t idesc, idesc_ext;
   int32_t* status;
 };
+
+// how M is read: element by element, 16-byte pieces of the rank (of a column), or 8 columns (of a rank row)
+enum { PIECES_NONE = 0, PIECES_RANK = 1, PIECES_COLUMNS = 2 };
 
 struct OutTile { int64_t t0; int rows, o0; };
 
@@ -142,7 +145,7 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   static_assert((3 * STAGES + 4) * 8 + 8 <= 256, "the barriers do not fit");
   // entry i % 16: 1 + the block's last tile i whose extension met values of M that are not finite. The builders are at most
-  // STAGES + 2 tiles ahead of the epilogue, so an entry is read before it is needed again.
+  // STAGES + 3 tiles ahead of the epilogue, so an entry is read before it is needed again.
   volatile int* not_finite = reinterpret_cast<volatile int*>(reinterpret_cast<uint8_t*>(bars) + 256);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -246,7 +249,8 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             const int steps = (min(BK, p.r - rb * BK) + UMMA_K - 1) / UMMA_K;
             for (int j = 0; j < steps; ++j)
               umma_f16(d_tmem, make_smem_desc_sw128(a_addr + j * (UMMA_K * 2), 16, 1024),
-                       make_smem_desc_sw128(b_addr + j * (UMMA_K * 2), 16, 1024), p.idesc_ext, 1u);
+                       p.m_pieces == PIECES_COLUMNS ? make_smem_desc_sw128(b_addr + j * (UMMA_K * 128), 64 * BK * 2, 1024)
+                                                    : make_smem_desc_sw128(b_addr + j * (UMMA_K * 2), 16, 1024), p.idesc_ext, 1u);
             umma_commit(empty_bar(at.s));
           }
           __syncwarp();
@@ -276,39 +280,77 @@ adapter_gemm_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const uint8_t* m = p.M + static_cast<int64_t>(e) * p.sma * 2;
         for (int rb = 0; rb < rank_blocks; ++rb, at.next()) {
           const int s = at.s, j0 = rb * BK, len = min(BK, p.r - j0), chunks = (len + UMMA_K - 1) / UMMA_K * 2;
+          // Where M comes in 16-byte pieces everything is fetched before the wait, and at once (a piece at a time cost 3 us an
+          // adapter). By rank: a thread holds two columns' rank rows, stored K-major. By column: 8 columns of one rank row, N-major.
+          constexpr int PIECES = BN / 128 * 8;
+          uint4 hv[8], mv[PIECES];
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch)            // H rows are padded to a multiple of 8 with zeros
+            hv[ch] = mine == e && ch * 8 < len ? __ldg(h + j0 / 8 + ch) : make_uint4(0u, 0u, 0u, 0u);
+          bool broken = false;
+          if (p.m_pieces != PIECES_NONE) {
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) {
+              bool in;
+              const uint8_t* src;
+              if (p.m_pieces == PIECES_RANK) {
+                const int o = (i >> 3) * 128 + row, ch = i & 7;
+                in = tl.o0 + o < p.O && ch * 8 < len;
+                src = m + (static_cast<int64_t>(tl.o0 + o) * p.smo + j0 + ch * 8) * 2;
+              } else {
+                const int idx = i * 128 + row, j = idx / (BN / 8), o = idx % (BN / 8) * 8;
+                in = j < len && tl.o0 + o < p.O;
+                src = m + (static_cast<int64_t>(j0 + j) * p.smj + tl.o0 + o) * 2;
+              }
+              mv[i] = in ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) broken |= drop_not_finite(mv[i], p.is_bf16);
+          }
           if (ok) ok = mbar_wait_warp(build_bar(s), (passes >> s) & 1, abort_flag, p.status, 36);
           passes ^= 1u << s;
           if (ok) {
             uint8_t* da = sA + s * A_BYTES + row * 128;
-            for (int ch = 0; ch < chunks; ++ch)       // H rows are padded to a multiple of 8 with zeros
-              *reinterpret_cast<uint4*>(da + ((ch ^ (row & 7)) << 4)) =
-                  mine == e && ch * 8 < len ? __ldg(h + j0 / 8 + ch) : make_uint4(0u, 0u, 0u, 0u);
+            uint8_t* sb = sB + s * B_BYTES;
 #pragma unroll
-            for (int half = 0; half < BN / 128; ++half) {
-              const int o = half * 128 + row;
-              uint8_t* db = sB + s * B_BYTES + o * 128;
-              const bool in = tl.o0 + o < p.O;
-              const uint8_t* src = m + (static_cast<int64_t>(tl.o0 + o) * p.smo + j0 * p.smj) * 2;
-              for (int ch = 0; ch < chunks; ++ch) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (in && p.m_vec && ch * 8 + 8 <= len) {
-                  v = __ldg(reinterpret_cast<const uint4*>(src + ch * 16));
-                } else if (in) {
+            for (int ch = 0; ch < 8; ++ch)
+              if (ch < chunks) *reinterpret_cast<uint4*>(da + ((ch ^ (row & 7)) << 4)) = hv[ch];
+            if (p.m_pieces == PIECES_RANK) {
+#pragma unroll
+              for (int i = 0; i < PIECES; ++i) {
+                const int o = (i >> 3) * 128 + row, ch = i & 7;
+                if (ch < chunks) *reinterpret_cast<uint4*>(sb + o * 128 + ((ch ^ (o & 7)) << 4)) = mv[i];
+              }
+            } else if (p.m_pieces == PIECES_COLUMNS) {
+#pragma unroll
+              for (int i = 0; i < PIECES; ++i) {
+                const int idx = i * 128 + row, j = idx / (BN / 8), c = idx % (BN / 8);      // 64 columns x 64 rank rows of 128 bytes each
+                if (j < chunks * 8) *reinterpret_cast<uint4*>(sb + (c >> 3) * (64 * BK * 2) + j * 128 + (((c & 7) ^ (j & 7)) << 4)) = mv[i];
+              }
+            } else {
+#pragma unroll 1
+              for (int half = 0; half < BN / 128; ++half) {
+                const int o = half * 128 + row;
+                const bool in = tl.o0 + o < p.O;
+                const uint8_t* src = m + (static_cast<int64_t>(tl.o0 + o) * p.smo + j0 * p.smj) * 2;
+#pragma unroll 1
+                for (int ch = 0; ch < chunks; ++ch) {
                   uint32_t w[4];
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
                     const int j = ch * 8 + 2 * i;
-                    const uint32_t lo = j < len ? __ldg(reinterpret_cast<const uint16_t*>(src + j * p.smj * 2)) : 0u;
-                    const uint32_t hi = j + 1 < len ? __ldg(reinterpret_cast<const uint16_t*>(src + (j + 1) * p.smj * 2)) : 0u;
+                    const uint32_t lo = in && j < len ? __ldg(reinterpret_cast<const uint16_t*>(src + j * p.smj * 2)) : 0u;
+                    const uint32_t hi = in && j + 1 < len ? __ldg(reinterpret_cast<const uint16_t*>(src + (j + 1) * p.smj * 2)) : 0u;
                     w[i] = lo | hi << 16;
                   }
-                  v = make_uint4(w[0], w[1], w[2], w[3]);
+                  uint4 v = make_uint4(w[0], w[1], w[2], w[3]);
+                  broken |= drop_not_finite(v, p.is_bf16);
+                  *reinterpret_cast<uint4*>(sb + o * 128 + ((ch ^ (o & 7)) << 4)) = v;
                 }
-                if (drop_not_finite(v, p.is_bf16)) not_finite[tile_iter & 15] = tile_iter + 1;
-                *reinterpret_cast<uint4*>(db + ((ch ^ (o & 7)) << 4)) = v;
               }
             }
           }
+          if (broken) not_finite[tile_iter & 15] = tile_iter + 1;
           fence_proxy_async_smem();
           asm volatile("bar.sync 1, 128;" ::: "memory");
           if (ok && row == 0) mbar_arrive(full_bar(s));
@@ -422,13 +464,17 @@ int launch_linear_tc(const LinearArgs& a) {
   p.bias = static_cast<const uint8_t*>(a.bias);
   p.Y = static_cast<uint8_t*>(a.Y); p.y_row_bytes = a.sym * 2;
   p.T = a.T; p.n = a.n; p.C = a.C; p.O = a.O; p.r = a.r; p.is_bf16 = bf16 ? 1 : 0;
-  p.m_vec = a.smj == 1 && a.smo % 8 == 0 && a.sma % 8 == 0 && al16(a.M) ? 1 : 0;
+  p.m_pieces = PIECES_NONE;
+  if (a.sma % 8 == 0 && al16(a.M)) {
+    if (a.smj == 1 && a.r % 8 == 0 && a.smo % 8 == 0) p.m_pieces = PIECES_RANK;
+    else if (a.smo == 1 && a.smj % 8 == 0) p.m_pieces = PIECES_COLUMNS;
+  }
   p.wide_rows = a.O % 16 == 0 && a.sym % 16 == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 31) == 0 ? 1 : 0;
   // while the rows of X fit L2 beside W every row tile runs beside each column tile, else groups of 16
   p.group_m = static_cast<double>(a.T) * a.C * 2.0 <= 48e6 ? (1 << 20) : 16;
   if (p.group_m > m_tiles) p.group_m = static_cast<int>(m_tiles);
   p.idesc = make_idesc_f16(bf16, false, !k_major, BM, BN);
-  p.idesc_ext = make_idesc_f16(bf16, false, false, BM, BN);
+  p.idesc_ext = make_idesc_f16(bf16, false, p.m_pieces == PIECES_COLUMNS, BM, BN);
   p.status = a.status;
   const int64_t total = m_tiles * cdiv(a.O, BN);
   const int grid = static_cast<int>(total < di.sm_count ? total : di.sm_count);
