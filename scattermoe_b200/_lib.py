@@ -225,6 +225,14 @@ def status_word(device: torch.device) -> torch.Tensor:
     return t
 
 
+def status_ptr(device: torch.device):
+    """The status word's address, None (nothing is reported) where it would have to be made while a graph is being captured: its memory
+    would belong to that graph."""
+    if device.index not in _status_words and torch.cuda.is_current_stream_capturing():
+        return None
+    return status_word(device).data_ptr()
+
+
 def check_device_status(device=None):
     """Synchronise and raise if a kernel reported a timed-out wait since the last check."""
     if device is None:

@@ -9,7 +9,11 @@ The ids may be in any order; tokens of one request usually stand together, which
 Two launches forward: the shrink into the rank (h = s A x; in 16 bits rounded once, as the tensor cores take it) and the shared product, whose accumulators take up
 B h before they are rounded once: the adapted output is never read back. Backward mirrors it (g = s B^T dy, then
 dx = W^T dy + A^T g in one launch) and sums the outer products dA_a = sum g x^T, dB_a = sum dy h^T per adapter in a fixed
-order. Gradients nobody asked for are not computed; adapters without rows get zeros; `scaling` is a constant.
+order. Gradients nobody asked for are not computed; adapters without rows get zeros; `scaling` is a constant. Infinities and NaN
+in one adapter, or in one row, stay with the rows they belong to.
+
+A training step can be captured into a CUDA graph as any other autograd function: warm up on the capturing side stream, and let go of
+eager graphs of the same leaves first (torch ends the process where a captured backward meets one).
 """
 from __future__ import annotations
 
@@ -48,7 +52,7 @@ def _forward_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
             lora_a.data_ptr(), *lora_a.stride(), lora_b.data_ptr(), *lora_b.stride(), ids.data_ptr(),
             scaling.data_ptr() if scaling is not None else None, scale, y.data_ptr(), h.data_ptr(),
             lists.data_ptr() if sort else None, offsets.data_ptr() if sort else None, n, width, out, r, dtype, _lib.path_flags(),
-            ws.data_ptr() if sort else None, ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+            ws.data_ptr() if sort else None, ws_bytes, _lib.status_ptr(dev), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_adapter_forward")
     return y, h, sorted_idx, offsets
 
@@ -76,7 +80,7 @@ def _backward_impl(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora
             *lora_a.stride(), lora_b.data_ptr(), *lora_b.stride(), ids.data_ptr(), scaling.data_ptr() if scaling is not None else None,
             scale, h.data_ptr(), sorted_idx.data_ptr() or None, offsets.data_ptr() or None, d_x.data_ptr() or None,
             d_a.data_ptr() or None, d_b.data_ptr() or None, d_bias.data_ptr() or None, n, width, out, r, dtype, _lib.path_flags(),
-            ws.data_ptr(), ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+            ws.data_ptr(), ws_bytes, _lib.status_ptr(dev), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_adapter_backward")
     return d_x, d_a, d_b, d_bias
 

@@ -468,7 +468,7 @@ extern "C" int smoe_few_token_mlp(const void* X, int64_t T, int64_t stride_xm, c
     return SMOE_ERR_WORKSPACE;
   }
   SMOE_CHECK_ARG((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "few_token_mlp: the workspace is not 16-byte aligned");
-  ft::Args a{X, stride_xm, W1, stride_w1e, stride_w1k, stride_w1n, b1, stride_b1e, stride_b1n,
+  ft::Args a{X, T == 1 ? 0 : stride_xm, W1, stride_w1e, stride_w1k, stride_w1n, b1, stride_b1e, stride_b1n,
              W2, stride_w2e, stride_w2k, stride_w2n, b2, stride_b2e, stride_b2n,
              gates, stride_gt, stride_gk, gates_dtype, expert_idxs, stride_it, stride_ik, Y, stride_ym,
              static_cast<int>(T), k, d, F, d_out, E, act_layout, act, dtype, alpha, limit,

@@ -78,7 +78,7 @@ def _mlp_impl(x: torch.Tensor, up: torch.Tensor, down: torch.Tensor, gates: Opti
               else (None, 0, 0, 0)),
             ids.data_ptr(), *ids.stride(), y.data_ptr(), d_out, k, d, F, d_out, E, act_layout, act,
             alpha, limit, _lib.DTYPE_CODE[x.dtype], _lib.path_flags() | (_lib.FLAG_AFTER_ROUTER if after_router else 0),
-            ws.data_ptr(), ws_bytes, _lib.status_word(dev).data_ptr(), _lib.stream_ptr(dev))
+            ws.data_ptr(), ws_bytes, _lib.status_ptr(dev), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_few_token_mlp")
     return y
 

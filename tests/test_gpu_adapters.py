@@ -312,6 +312,37 @@ def test_a_decode_step_runs_both_operators():
     assert out.shape == (T, d) and torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("T", [20, 400])
+def test_which_kernels_run(T, monkeypatch):
+    """16-bit operands run on the tensor cores; forced onto the CUDA cores they give the same step; widths no 16-byte access can read
+    are refused when the tensor cores are asked for."""
+    from scattermoe_b200.kernels import ops
+    p = problem(T, 192, 264, 24, 5, torch.float16, "shuffled", bias=True, bare=0.1)
+    for path in ("tc", "simt"):
+        monkeypatch.setattr(ops, "FORCE_PATH", path)
+        call(p)
+        assert ops.last_path_was_tensor_core() == (path == "tc")
+        verify(p, ("x", "a", "b", "bias"))
+    monkeypatch.setattr(ops, "FORCE_PATH", "tc")
+    with pytest.raises(RuntimeError, match="no tensor-core kernel"):
+        call(problem(T, 33, 64, 8, 3, torch.bfloat16))
+
+
+def test_compiles():
+    """torch.compile traces forward and backward as one graph."""
+    import scattermoe_b200 as sm
+    p = problem(200, 128, 96, 16, 3, torch.bfloat16, "shuffled", bias=True)
+    q = dict(p, **{n: p[n].clone().requires_grad_() for n in ("x", "a", "b")})
+    f = torch.compile(lambda x, a, b: sm.adapter_linear(x, p["weight"], a, b, p["ids"], scaling=p["scaling"], bias=p["bias"]),
+                      backend="aot_eager", fullgraph=True)
+    dy = torch.randn(200, 96, device="cuda").bfloat16()
+    leaves = [q[n] for n in ("x", "a", "b")]
+    got, want = f(*leaves), call(q)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)):
+        assert torch.equal(a, b)
+
+
 def test_refusals():
     import scattermoe_b200 as sm
     p = problem(4, 64, 96, 8, 3, torch.bfloat16)

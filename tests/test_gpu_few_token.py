@@ -302,6 +302,34 @@ def test_module_decode_matches_forward(bias):
         check(a.view(10, 128), y, bound)
 
 
+def test_which_kernels_run(monkeypatch):
+    """16-bit operands run on the streaming kernels; forced onto the CUDA cores they give the same layer; what the streaming kernels
+    cannot address is refused when they are asked for."""
+    from scattermoe_b200.kernels import ops
+    for order, layout in (("out_in", SECOND), ("in_out", FIRST), ("out_in", OSS), ("in_out", OSS), ("in_out", PLAIN)):
+        p = problem(19, 192, 136, 6, 2, torch.float16, layout, order, bias=True, d_out=151 if order == "out_in" else 152)
+        for path in ("tc", "simt"):
+            monkeypatch.setattr(ops, "FORCE_PATH", path)
+            verify(p, layout)
+            assert ops.last_path_was_tensor_core() == (path == "tc")
+    monkeypatch.setattr(ops, "FORCE_PATH", "tc")
+    with pytest.raises(RuntimeError, match="no tensor-core kernel"):
+        run(problem(3, 50, 30, 4, 2, torch.bfloat16, FIRST), FIRST)
+
+
+def test_compiles():
+    """torch.compile traces the calls as one graph each."""
+    import scattermoe_b200 as sm
+    p = problem(6, 64, 64, 4, 2, torch.bfloat16, FIRST)
+    wr = torch.randn(4, 64, device="cuda").bfloat16()
+    f = torch.compile(lambda x: sm.few_token_mlp(x, p["up"], p["down"], p["gates"], p["ids"], FIRST, SILU), backend="aot_eager", fullgraph=True)
+    g = torch.compile(lambda x: sm.few_token_moe(x, wr, p["up"], p["down"], 2, FIRST, SILU), backend="aot_eager", fullgraph=True)
+    with torch.no_grad():
+        assert torch.equal(f(p["x"]), run(p, FIRST))
+        for a, b in zip(g(p["x"]), sm.few_token_moe(p["x"], wr, p["up"], p["down"], 2, FIRST, SILU)):
+            assert torch.equal(a, b)
+
+
 def test_refusals():
     import scattermoe_b200 as sm
     p = problem(4, 64, 64, 4, 2, torch.bfloat16, FIRST)
