@@ -40,6 +40,9 @@ constexpr int SH_MAX_SMEM = 226 * 1024;      // 1 KB less than a block can have:
 constexpr int SH_TOKENS = 32, SH_COLS = 64, SH_K = 64;
 constexpr int SH_SMALL_RING = 13 * 1024;      // per warp: two blocks fit an SM
 
+// padded against bank conflicts, but for the shortest rows: two of them then fit beside each other on an SM
+__host__ __device__ inline int rank_row_bytes(int cols) { return cols <= 16 ? cols * 2 : cols * 2 + 16; }
+
 struct ShrinkParams {
   ShrinkArgs a;
   int k_major;       // M has the contracted axis contiguous
@@ -98,7 +101,7 @@ shrink_tc_kernel(const ShrinkParams p) {
     __syncthreads();
     for (int j0 = 0; j0 < a.r; j0 += p.width) {
       const int cols = adapters * p.width, groups = cols >> 3;
-      const int m_pitch = cols * 2 + 16;         // M with the rank contiguous: bytes of a row in shared memory
+      const int m_pitch = rank_row_bytes(cols);  // M with the rank contiguous: bytes of a row in shared memory
       const int stage_bytes = SH_TOKENS * 128 + (p.k_major ? (groups + 1) / 2 * 2048 : SH_K * m_pitch);
       float acc[2][8][4];
 #pragma unroll
@@ -169,19 +172,26 @@ shrink_tc_kernel(const ShrinkParams p) {
         }
         cp_async_commit();
       };
+      // One loop in which the loads run `stages - 1` turns ahead of the products: with a copy of both for every depth, and the first
+      // loads unrolled, the warps waited for instructions more than for data.
       constexpr int TURN = 8 * SH_K;
-      auto run = [&](auto S_) {
-      constexpr int S = decltype(S_)::value;      // stages of the ring
-      int k0 = warp * SH_K, s = 0, ahead = k0;
-#pragma unroll
-      for (int i = 0; i < S - 1; ++i, ahead += TURN)
-        if (ahead < a.C) load(i, ahead); else cp_async_commit();
-      for (; k0 < a.C; k0 += TURN, ahead += TURN, s = s + 1 == S ? 0 : s + 1) {
-        if (ahead < a.C) load(s == 0 ? S - 1 : s - 1, ahead); else cp_async_commit();
-        cp_async_wait<S - 1>();
+      const int turns = a.C > warp * SH_K ? (a.C - warp * SH_K + TURN - 1) / TURN : 0;
+      const int stages = min(4, p.ring_bytes / stage_bytes);
+      int in = 0, out = 0;
+#pragma unroll 1
+      for (int i = 0; i < turns + stages - 1; ++i) {
+        if (i < turns) {
+          load(in, warp * SH_K + i * TURN);
+          in = in + 1 == stages ? 0 : in + 1;
+        } else {
+          cp_async_commit();
+        }
+        if (i < stages - 1) continue;
+        if (stages == 4) cp_async_wait<3>(); else if (stages == 3) cp_async_wait<2>(); else cp_async_wait<1>();
         __syncwarp();
-        const uint32_t x = ring + s * stage_bytes, m = x + SH_TOKENS * 128;
-#pragma unroll
+        const uint32_t x = ring + out * stage_bytes, m = x + SH_TOKENS * 128;
+        out = out + 1 == stages ? 0 : out + 1;
+#pragma unroll 1
         for (int st = 0; st < SH_K / 16; ++st) {
           uint32_t af[2][4];
           const int row = (lane & 7) + ((lane >> 3) & 1) * 8;
@@ -207,10 +217,6 @@ shrink_tc_kernel(const ShrinkParams p) {
         }
         __syncwarp();
       }
-      };
-      if (4 * stage_bytes <= p.ring_bytes) run(std::integral_constant<int, 4>{});
-      else if (3 * stage_bytes <= p.ring_bytes) run(std::integral_constant<int, 3>{});
-      else run(std::integral_constant<int, 2>{});
       cp_async_wait<0>();
       __syncthreads();
       // join the warps: [warp][token][column]
@@ -253,7 +259,7 @@ int launch_shrink_tc(const ShrinkArgs& a) {
   p.m_vec = aligned && (p.k_major ? a.smj % 8 == 0 : a.smj == 1 && a.smc % 8 == 0 && a.r % 8 == 0) ? 1 : 0;
   // Two stages of one adapter are the least. Where that is little the ring stays small enough for two blocks per SM, which is what
   // tokens in runs want; rows in no order (and not sorted) want as many adapters in a pass as fit.
-  auto stage_of = [&](int cols) { return SH_TOKENS * 128 + (p.k_major ? cdiv(cols, 16) * 2048 : SH_K * (cols * 2 + 16)); };
+  auto stage_of = [&](int cols) { return SH_TOKENS * 128 + (p.k_major ? cdiv(cols, 16) * 2048 : SH_K * rank_row_bytes(cols)); };
   const int one = 2 * stage_of(p.width);
   p.ring_bytes = one <= SH_SMALL_RING ? SH_SMALL_RING : (one > 20 * 1024 ? one : 20 * 1024);
   p.per_pass = 1;
@@ -284,10 +290,10 @@ int launch_shrink_tc(const ShrinkArgs& a) {
 
 // ---- outer products --------------------------------------------------------------------------------------------------
 // D[a][j, c] = sum over the adapter's rows of U[t, j] V[t, c]. The adapter-sorted rows are cut into equal chunks; a block owns 128
-// columns of V and up to 64 of the rank for one chunk and walks the adapters in it, 64 rows at a time (gathered by cp.async, three
+// columns of V and up to 64 of the rank for one chunk and walks the adapters in it, 64 rows at a time (gathered by cp.async, four
 // buffers). An adapter that lies in one chunk is written at once; one that spans chunks leaves fp32 parts (at most two per
 // chunk: its first and its last adapter), which a second kernel adds up in the chunks' order. No atomics.
-constexpr int GR_COLS = 128, GR_J = 64, GR_ROWS = 64, GR_STAGES = 3, GR_MAX_CHUNKS = 16;
+constexpr int GR_COLS = 128, GR_J = 64, GR_ROWS = 64, GR_STAGES = 4, GR_MAX_CHUNKS = 16;
 constexpr int GR_V_PITCH = GR_COLS * 2 + 16, GR_U_PITCH = GR_J * 2 + 16;
 constexpr int GR_STAGE = GR_ROWS * (GR_V_PITCH + GR_U_PITCH);
 constexpr int GR_SMEM = GR_STAGES * GR_STAGE;
@@ -363,14 +369,16 @@ grad_tc_kernel(const GradParams p) {
       fetch_rows(i + 1);
     };
     fetch_rows(0);
-    for (int i = 0; i < GR_STAGES - 1; ++i)
-      if (i < tiles) load(i); else cp_async_commit();
-    for (int i = 0; i < tiles; ++i) {
-      cp_async_wait<GR_STAGES - 2>();
+#pragma unroll 1
+    for (int ahead = 0; ahead < tiles + GR_STAGES - 1; ++ahead) {      // the loads run GR_STAGES - 1 tiles ahead
+      if (ahead >= GR_STAGES) __syncthreads();                         // everyone has read the buffer that comes next
+      if (ahead < tiles) load(ahead); else cp_async_commit();
+      const int i = ahead - (GR_STAGES - 1);
+      if (i < 0) continue;
+      cp_async_wait<GR_STAGES - 1>();
       __syncthreads();
-      if (i + GR_STAGES - 1 < tiles) load(i + GR_STAGES - 1); else cp_async_commit();
       const uint32_t v = ring + (i % GR_STAGES) * GR_STAGE, u = v + GR_ROWS * GR_V_PITCH;
-#pragma unroll
+#pragma unroll 2
       for (int st = 0; st < GR_ROWS / 16; ++st) {
         uint32_t af[4];          // 16 columns of V (the M side) x 16 rows
         ldsm4_trans(af, v + (st * 16 + (lane & 7) + (lane >> 4) * 8) * GR_V_PITCH + (warp * 16 + ((lane >> 3) & 1) * 8) * 2);
