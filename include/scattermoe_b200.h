@@ -265,10 +265,10 @@ int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void
  *     neither) the call first sorts the rows by adapter as smoe_sort_count does and hands the lists out: backward needs
  *     them, and rows in no order then cost no more than rows in runs.
  * backward:  G[t] = s_a B[a]^T DY[t];   DX[t] = W^T DY[t] + A[a]^T G[t];   DA[a] = sum G[t] X[t]^T;   DB[a] = sum DY[t] H[t]^T over
- *     the adapter's rows (zeros without rows);   Dbias = sum DY[t].   Each of DX, DA, DB, Dbias may be null. H, sorted_idx and
- *     offsets are forward's. Every sum has a fixed order.
+ *     the adapter's rows (zeros without rows);   DW = sum DY[t] X[t]^T;   Dbias = sum DY[t].   Each of DX, DA, DB, DW, Dbias may be
+ *     null. H, sorted_idx and offsets are forward's. Every sum has a fixed order.
  * W (out, in), A (n, r, in), B (n, out, r) in element strides; X, DY rows with inner stride 1; Y, DX (T, .), H (T, r rounded up
- * to a multiple of 8, in `dtype`), DA, DB, Dbias contiguous. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31 - 64. The workspace (16-byte aligned,
+ * to a multiple of 8, in `dtype`), DA, DB, DW (out, in), Dbias contiguous. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31 - 64. The workspace (16-byte aligned,
  * smoe_adapter_workspace_bytes; forward without a sort needs none) belongs to the call until its work has finished. */
 size_t smoe_adapter_workspace_bytes(int64_t T, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype);
 int smoe_adapter_forward(const void* X, int64_t T, int64_t stride_xm,
@@ -283,7 +283,8 @@ int smoe_adapter_backward(const void* DY, int64_t T, int64_t stride_dym, const v
                           const void* A, int64_t stride_aa, int64_t stride_aj, int64_t stride_ai,
                           const void* B, int64_t stride_ba, int64_t stride_bo, int64_t stride_bj,
                           const int64_t* adapter_idxs, const float* scaling, float scale, const void* H,
-                          const int64_t* sorted_idx, const int64_t* offsets, void* DX, void* DA, void* DB, void* Dbias,
+                          const int64_t* sorted_idx, const int64_t* offsets, void* DX, void* DA, void* DB, void* DW,
+                          void* Dbias,
                           int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype, int32_t flags,
                           void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 

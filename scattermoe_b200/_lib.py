@@ -106,7 +106,7 @@ SIGNATURES = {
     "smoe_adapter_forward": ([_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float,
                               _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
     "smoe_adapter_backward": ([_P, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, c_float,
-                               _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
+                               _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _P, c_size_t, _P, _P], c_int32),
 }
 
 

@@ -24,7 +24,6 @@ from torch import nn
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from . import kernels
 from .parallel_experts import _rowmajor
 
 MAX_RANK = 256
@@ -59,9 +58,9 @@ def _forward_impl(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
 
 def _backward_impl(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                    ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float, h: torch.Tensor, sorted_idx: torch.Tensor,
-                   offsets: torch.Tensor, need_x: bool, need_a: bool, need_b: bool, need_bias: bool) -> tuple[
-                       torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(d_x, d_a, d_b, d_bias), empty where not needed."""
+                   offsets: torch.Tensor, need_x: bool, need_a: bool, need_b: bool, need_w: bool, need_bias: bool) -> tuple[
+                       torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(d_x, d_a, d_b, d_weight, d_bias), empty where not needed."""
     T, width = x.shape
     out = weight.size(0)
     n, r, _ = lora_a.shape
@@ -71,7 +70,8 @@ def _backward_impl(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora
     def result(wanted, *shape):
         return torch.empty(shape if wanted else (0,), dtype=x.dtype, device=dev)
 
-    d_x, d_a, d_b, d_bias = (result(need_x, T, width), result(need_a, n, r, width), result(need_b, n, out, r), result(need_bias, out))
+    d_x, d_a, d_b = result(need_x, T, width), result(need_a, n, r, width), result(need_b, n, out, r)
+    d_w, d_bias = result(need_w, out, width), result(need_bias, out)
     ws_bytes = lib.smoe_adapter_workspace_bytes(T, n, width, out, r, dtype)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     with _lib.on_device_of(dev):
@@ -79,10 +79,10 @@ def _backward_impl(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora
             dy.data_ptr(), T, dy.stride(0), x.data_ptr(), x.stride(0), weight.data_ptr(), *weight.stride(), lora_a.data_ptr(),
             *lora_a.stride(), lora_b.data_ptr(), *lora_b.stride(), ids.data_ptr(), scaling.data_ptr() if scaling is not None else None,
             scale, h.data_ptr(), sorted_idx.data_ptr() or None, offsets.data_ptr() or None, d_x.data_ptr() or None,
-            d_a.data_ptr() or None, d_b.data_ptr() or None, d_bias.data_ptr() or None, n, width, out, r, dtype, _lib.path_flags(),
+            d_a.data_ptr() or None, d_b.data_ptr() or None, d_w.data_ptr() or None, d_bias.data_ptr() or None, n, width, out, r, dtype, _lib.path_flags(),
             ws.data_ptr(), ws_bytes, _lib.status_ptr(dev), _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_adapter_backward")
-    return d_x, d_a, d_b, d_bias
+    return d_x, d_a, d_b, d_w, d_bias
 
 
 # The registered forms are used while torch.compile traces, as everywhere in this package.
@@ -105,15 +105,17 @@ def _(x, weight, bias, lora_a, lora_b, ids, scaling, scale, sort):
 @torch.library.custom_op("scattermoe_b200::adapter_backward", mutates_args={})
 def backward_compileable(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                          ids: torch.Tensor, scaling: Optional[torch.Tensor], scale: float, h: torch.Tensor,
-                         sorted_idx: torch.Tensor, offsets: torch.Tensor, need_x: bool, need_a: bool, need_b: bool,
-                         need_bias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _backward_impl(dy, x, weight, lora_a, lora_b, ids, scaling, scale, h, sorted_idx, offsets, need_x, need_a, need_b, need_bias)
+                         sorted_idx: torch.Tensor, offsets: torch.Tensor, need_x: bool, need_a: bool, need_b: bool, need_w: bool,
+                         need_bias: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _backward_impl(dy, x, weight, lora_a, lora_b, ids, scaling, scale, h, sorted_idx, offsets, need_x, need_a, need_b, need_w,
+                          need_bias)
 
 
 @backward_compileable.register_fake
-def _(dy, x, weight, lora_a, lora_b, ids, scaling, scale, h, sorted_idx, offsets, need_x, need_a, need_b, need_bias):
+def _(dy, x, weight, lora_a, lora_b, ids, scaling, scale, h, sorted_idx, offsets, need_x, need_a, need_b, need_w, need_bias):
     return (x.new_empty(x.shape if need_x else (0,)), x.new_empty(lora_a.shape if need_a else (0,)),
-            x.new_empty(lora_b.shape if need_b else (0,)), x.new_empty((weight.size(0) if need_bias else 0,)))
+            x.new_empty(lora_b.shape if need_b else (0,)), x.new_empty(weight.shape if need_w else (0,)),
+            x.new_empty((weight.size(0) if need_bias else 0,)))
 
 
 class AdapterLinear_(torch.autograd.Function):
@@ -137,21 +139,11 @@ class AdapterLinear_(torch.autograd.Function):
         dy = _rowmajor(dy)
         if dy.dtype != x.dtype:
             dy = dy.to(x.dtype)
-        d_w = d_bias_w = None
-        if need_w:
-            rows = torch.full((1,), x.size(0), dtype=torch.int64, device=x.device)
-            d_w, db = kernels.ops.group_bwd_W(DY=dy, X=x, expert_offsets=rows, E=1, has_bias=need_bias)
-            d_w = d_w[0].t()
-            if need_bias:
-                d_bias_w = db[0]
-        d_x = d_a = d_b = d_bias = None
-        own_bias = need_bias and not need_w
-        if need_x or need_a or need_b or own_bias:
-            run = backward_compileable if torch.compiler.is_compiling() else _backward_impl
-            d_x, d_a, d_b, d_bias = run(dy, x, weight, lora_a, lora_b, ids, scaling, ctx.scale, h, sorted_idx, offsets, need_x, need_a,
-                                        need_b, own_bias)
-        return (d_x if need_x else None, d_w, d_a if need_a else None, d_b if need_b else None, None, None, None,
-                d_bias if own_bias else d_bias_w)
+        run = backward_compileable if torch.compiler.is_compiling() else _backward_impl
+        d_x, d_a, d_b, d_w, d_bias = run(dy, x, weight, lora_a, lora_b, ids, scaling, ctx.scale, h, sorted_idx, offsets, need_x, need_a,
+                                         need_b, need_w, need_bias)
+        return (d_x if need_x else None, d_w if need_w else None, d_a if need_a else None, d_b if need_b else None, None, None, None,
+                d_bias if need_bias else None)
 
 
 def adapter_linear(inputs, weight, lora_a, lora_b, adapter_idxs, scaling=1.0, bias=None):

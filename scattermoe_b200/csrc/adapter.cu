@@ -81,21 +81,34 @@ linear_simt_kernel(const LinearArgs a) {
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  for (int k0 = 0; k0 < a.C; k0 += TK) {
+  // the next step's values are fetched while this one's are multiplied
+  float xn[TM * TK / 256], wn[TN * TK / 256];
+  auto fetch = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < TM * TK / 256; ++i) {
       const int idx = tid + i * 256, kk = idx % TK, m = idx / TK;
       const int64_t t = t0 + m;
-      xs[kk][m] = (t < a.T && k0 + kk < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.X) + t * a.sxm + k0 + kk)) : 0.f;
+      xn[i] = (t < a.T && k0 + kk < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.X) + t * a.sxm + k0 + kk)) : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < TN * TK / 256; ++i) {
       const int idx = tid + i * 256;
       const int kk = k_contig ? idx % TK : idx / TN, n = k_contig ? idx / TK : idx % TN;
-      ws[kk][n] = (o0 + n < a.O && k0 + kk < a.C)
-                      ? to_f32<T>(__ldg(static_cast<const T*>(a.W) + (k0 + kk) * a.swk + (o0 + n) * a.swn)) : 0.f;
+      wn[i] = (o0 + n < a.O && k0 + kk < a.C)
+                  ? to_f32<T>(__ldg(static_cast<const T*>(a.W) + (k0 + kk) * a.swk + (o0 + n) * a.swn)) : 0.f;
+    }
+  };
+  fetch(0);
+  for (int k0 = 0; k0 < a.C; k0 += TK) {
+#pragma unroll
+    for (int i = 0; i < TM * TK / 256; ++i) xs[(tid + i * 256) % TK][(tid + i * 256) / TK] = xn[i];
+#pragma unroll
+    for (int i = 0; i < TN * TK / 256; ++i) {
+      const int idx = tid + i * 256;
+      ws[k_contig ? idx % TK : idx / TN][k_contig ? idx / TK : idx % TN] = wn[i];
     }
     __syncthreads();
+    fetch(k0 + TK);
 #pragma unroll
     for (int kk = 0; kk < TK; ++kk) {
       const float4 x4 = *reinterpret_cast<const float4*>(&xs[kk][ty * 4]);
@@ -150,16 +163,21 @@ grad_simt_kernel(const GradArgs a) {
     const int cnt = static_cast<int>(min(static_cast<int64_t>(32), end - m0));
     if (tid < 32) rows[tid] = tid < cnt ? a.sorted_idx[m0 + tid] : -1;
     __syncthreads();
-    for (int i = tid; i < 32 * 16; i += 256) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int i = tid + q * 256;
       const int m = i >> 4, j = i & 15;
       us[m][j] = (m < cnt && j0 + j < a.r) ? to_f32<T>(static_cast<const T*>(a.U)[rows[m] * rank_pitch(a.r) + j0 + j]) : 0.f;
     }
-    for (int i = tid; i < 32 * 64; i += 256) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const int i = tid + q * 256;
       const int m = i >> 6, c = i & 63;
       vs[m][c] = (m < cnt && c0 + c < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.V) + rows[m] * a.svm + c0 + c)) : 0.f;
     }
     __syncthreads();
-    for (int m = 0; m < cnt; ++m) {
+#pragma unroll 8
+    for (int m = 0; m < 32; ++m) {      // rows past the last are zeros
       const float v = vs[m][cx];
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = fmaf(us[m][jg * 4 + i], v, acc[i]);
@@ -282,6 +300,8 @@ static int outer(const GradArgs& a, int flags) {
   return launch_grad_simt(a);
 }
 
+__global__ void set_rows_kernel(int64_t* rows, int64_t T) { *rows = T; }
+
 static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 
 // ---- column sums (the shared bias's gradient): fp32 partial sums over slices of the rows, added up in order ----
@@ -385,7 +405,7 @@ extern "C" int smoe_adapter_backward(const void* DY, int64_t T, int64_t stride_d
                                      int64_t stride_ai, const void* B, int64_t stride_ba, int64_t stride_bo, int64_t stride_bj,
                                      const int64_t* adapter_idxs, const float* scaling, float scale, const void* H,
                                      const int64_t* sorted_idx, const int64_t* offsets, void* DX, void* DA, void* DB,
-                                     void* Dbias, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype, int32_t flags,
+                                     void* DW, void* Dbias, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype, int32_t flags,
                                      void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   const char* who = "adapter_backward";
   if (int rc = ad::check_common(who, T, n, in, out, r, dtype)) return rc;
@@ -416,6 +436,13 @@ extern "C" int smoe_adapter_backward(const void* DY, int64_t T, int64_t stride_d
   if (DB) {
     ad::GradArgs g{H, T, DY, stride_dym, sorted_idx, offsets, DB, static_cast<int64_t>(r) * out, 1, r, n, out, r, dtype, parts, parts_bytes, st};
     if (int rc = ad::outer(g, flags)) return rc;
+  }
+  if (DW) {      // the shared weight: one segment of the grouped weight gradient, its bias with it
+    int64_t* rows = reinterpret_cast<int64_t*>(parts);
+    ad::set_rows_kernel<<<1, 1, 0, st>>>(rows, T);
+    SMOE_LAUNCH_CHECK();
+    return smoe_group_bwd_w(DY, stride_dym, 1, X, T, stride_xm, 1, rows, nullptr, 1, DW, static_cast<int64_t>(out) * in, 1, in, Dbias,
+                            out, 1, T, in, out, 1, dtype, flags & SMOE_FLAG_FORCE_SIMT, status, stream);
   }
   if (Dbias) return ad::column_sum(DY, T, stride_dym, out, Dbias, dtype, parts, st);
   return SMOE_OK;

@@ -51,7 +51,7 @@ def test_adapter_entry_points_refuse(bad, word):
                    flags=0, ws=None, ws_bytes=0, status=None, stream=None)
     assert lib.smoe_adapter_forward(*{**forward, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
     backward = dict(DY=256, T=4, sdy=64, X=256, sxm=64, W=256, swo=64, swi=1, A=256, saa=512, saj=64, sai=1, B=256, sba=512, sbo=8,
-                    sbj=1, ids=256, scaling=None, scale=1.0, H=256, sorted_idx=256, offsets=256, DX=256, DA=256, DB=256, Db=256, n=2,
+                    sbj=1, ids=256, scaling=None, scale=1.0, H=256, sorted_idx=256, offsets=256, DX=256, DA=256, DB=256, DW=256, Db=256, n=2,
                     width=64, out=64, r=8, dtype=1, flags=0, ws=256, ws_bytes=1 << 24, status=None, stream=None)
     assert lib.smoe_adapter_backward(*{**backward, **bad}.values()) == _lib.SMOE_ERR_BAD_ARG and word in _lib.last_error()
 
@@ -65,8 +65,8 @@ def test_adapter_workspaces_and_lists():
     assert lib.smoe_adapter_forward(*head, 256, 256, *tail, 256, need - 1, None, None) == 4 and "workspace" in _lib.last_error()
     assert lib.smoe_adapter_forward(*head, 256, None, *tail, 256, need, None, None) == _lib.SMOE_ERR_BAD_ARG
     head = [256, 100, 96, 256, 64, 256, 64, 1, 256, 512, 64, 1, 256, 768, 8, 1, 256, None, 1.0, 256]
-    assert lib.smoe_adapter_backward(*head, 256, 256, 256, 256, 256, 256, *tail, 256, need - 1, None, None) == 4
-    assert lib.smoe_adapter_backward(*head, None, None, 256, 256, None, None, *tail, 256, need, None, None) == _lib.SMOE_ERR_BAD_ARG
+    assert lib.smoe_adapter_backward(*head, 256, 256, 256, 256, 256, 256, 256, *tail, 256, need - 1, None, None) == 4
+    assert lib.smoe_adapter_backward(*head, None, None, 256, 256, None, None, None, *tail, 256, need, None, None) == _lib.SMOE_ERR_BAD_ARG
     assert "sorted" in _lib.last_error()
 
 
