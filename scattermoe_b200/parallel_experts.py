@@ -24,7 +24,7 @@ def _sort_count_impl(flat: torch.Tensor, num_experts: int):
     offsets = torch.empty(num_experts, dtype=torch.int64, device=dev)
     ws_bytes = lib.smoe_sort_count_workspace_bytes(R, num_experts)
     ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=dev)
-    with _lib.on_device_of(dev):
+    with torch.cuda.device(dev):
         rc = lib.smoe_sort_count(flat.data_ptr(), R, num_experts, sorted_e.data_ptr(), sorted_idx.data_ptr(),
                                  offsets.data_ptr(), ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
     _lib.check(rc, "smoe_sort_count")
