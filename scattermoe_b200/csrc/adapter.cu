@@ -65,7 +65,7 @@ shrink_simt_kernel(const ShrinkArgs a) {
 }
 
 // ---- shared product + expansion: 64 x 64 tiles, 4 x 4 outputs per thread ----------------------------------------
-constexpr int TM = 64, TN = 64, TK = 16;
+constexpr int TM = 64, TN = 64, TK = 32;      // long steps: with few tiles the kernel is bound by their number
 
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -149,35 +149,36 @@ linear_simt_kernel(const LinearArgs a) {
 }
 
 // ---- per-adapter outer products: a block per (64 columns, 16 rank rows, adapter), over the adapter's rows in order ----
+constexpr int GR_SIMT_ROWS = 128;      // of a step: the kernel is bound by the latency of its steps
 template <typename T>
 __global__ void __launch_bounds__(256)
 grad_simt_kernel(const GradArgs a) {
-  __shared__ float us[32][17];
-  __shared__ float vs[32][65];
-  __shared__ int64_t rows[32];
+  __shared__ float us[GR_SIMT_ROWS][17];
+  __shared__ float vs[GR_SIMT_ROWS][65];
+  __shared__ int64_t rows[GR_SIMT_ROWS];
   const int tid = threadIdx.x, cx = tid & 63, jg = tid >> 6;
   const int c0 = blockIdx.x * 64, j0 = blockIdx.y * 16, e = blockIdx.z;
   const int64_t beg = e ? a.offsets[e - 1] : 0, end = a.offsets[e];
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t m0 = beg; m0 < end; m0 += 32) {
-    const int cnt = static_cast<int>(min(static_cast<int64_t>(32), end - m0));
-    if (tid < 32) rows[tid] = tid < cnt ? a.sorted_idx[m0 + tid] : -1;
+  for (int64_t m0 = beg; m0 < end; m0 += GR_SIMT_ROWS) {
+    const int cnt = static_cast<int>(min(static_cast<int64_t>(GR_SIMT_ROWS), end - m0));
+    if (tid < GR_SIMT_ROWS) rows[tid] = tid < cnt ? a.sorted_idx[m0 + tid] : -1;
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
+    for (int q = 0; q < GR_SIMT_ROWS * 16 / 256; ++q) {
       const int i = tid + q * 256;
       const int m = i >> 4, j = i & 15;
       us[m][j] = (m < cnt && j0 + j < a.r) ? to_f32<T>(static_cast<const T*>(a.U)[rows[m] * rank_pitch(a.r) + j0 + j]) : 0.f;
     }
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
+    for (int q = 0; q < GR_SIMT_ROWS * 64 / 256; ++q) {
       const int i = tid + q * 256;
       const int m = i >> 6, c = i & 63;
       vs[m][c] = (m < cnt && c0 + c < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.V) + rows[m] * a.svm + c0 + c)) : 0.f;
     }
     __syncthreads();
 #pragma unroll 8
-    for (int m = 0; m < 32; ++m) {      // rows past the last are zeros
+    for (int m = 0; m < cnt; ++m) {
       const float v = vs[m][cx];
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[i] = fmaf(us[m][jg * 4 + i], v, acc[i]);
