@@ -180,6 +180,22 @@ __device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* __
   __syncthreads();
 }
 
+// 32 values per lane -> lane l holds the sum over the lanes of value l.
+__device__ __forceinline__ float transpose_reduce(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool upper = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < o) {
+        const float send = upper ? v[i] : v[i + o];
+        const float keep = upper ? v[i + o] : v[i];
+        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      }
+  }
+  return v[0];
+}
+
 __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
   if (dtype == SMOE_F32) return static_cast<const float*>(p)[i];
   if (dtype == SMOE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);

@@ -61,22 +61,6 @@ __device__ __forceinline__ void emit(const SimtParams& q, int e, int slot, int p
   }
 }
 
-// 32 values per lane -> lane l holds the sum over the lanes of value l.
-__device__ __forceinline__ float transpose_reduce(float (&v)[32], int lane) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const bool upper = (lane & o) != 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < o) {
-        const float send = upper ? v[i] : v[i + o];
-        const float keep = upper ? v[i + o] : v[i];
-        v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-      }
-  }
-  return v[0];
-}
-
 // V consecutive values as floats; V == 1 or one 16-byte load
 template <typename T, int V>
 __device__ __forceinline__ void load_v(const T* p, float (&out)[V]) {
