@@ -39,6 +39,7 @@
 
 #include "act_math.cuh"
 #include "few_token.cuh"
+#include "few_token_stages.h"
 #include "ptx.cuh"
 #include "tensor_map.cuh"
 
@@ -55,7 +56,6 @@ constexpr int GATHER_THREADS = GATHERERS * 32 / GATHER_TURNS;
 constexpr int DOWN_TURNS = 4;                      // down: pairs of multiplying warps that take the stages in turn
 constexpr int THREADS = (CONSUMERS + LOADERS + GATHERERS) * 32;
 // The number of stages is a multiple of the turns: every stage then always belongs to the same warps, which wait for each of its passes.
-constexpr int MAX_STAGES = 16;
 constexpr int TILE = 32;                           // weight rows (output columns) of a warp's tile
 constexpr int BLOCK_K = 64;                        // K of a box: one 128-byte line of 16-bit values
 constexpr int MAX_CTAS = 160;
@@ -71,9 +71,9 @@ struct StreamParams {
   int NT;                     // slots of a job
   int K, blocks;              // K and its boxes
   int box_bytes, load_bytes;  // bytes a box takes in the ring, and bytes it loads
-  int steps_of[4][4];         // steps of K of a stage: 1, 2, 3-4, 5-8 boxes wide x a job of 1-8, 9-16, 17-24, 25-32 slots
   Extension ext;              // up: added to the values before they are rounded (adapter_linear)
-  int stages, stage_bytes, ring_bytes;
+  Stages ring;
+  int ring_bytes;
   int rows;                   // down: rows of a tile's token sums (the tile's columns)
 };
 
@@ -219,7 +219,7 @@ template <bool UP, bool KMAJOR>
 __device__ __forceinline__ void shape_of(const StreamParams& p, Run& r, int n) {
   r.groups = (n + 7) >> 3;
   r.boxes = KMAJOR ? r.tiles : (r.tiles + 1) >> 1;
-  r.nb = p.steps_of[r.boxes <= 2 ? r.boxes - 1 : (r.boxes <= 4 ? 2 : 3)][r.groups - 1];
+  r.nb = p.ring.steps_of[width_class(r.boxes)][r.groups - 1];
   r.x_offset = r.boxes * r.nb * p.box_bytes;
 }
 
@@ -285,7 +285,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   auto empty_bar = [&](int s) { return bar0 + 8u * (MAX_STAGES + s); };
 
   if (tid == 0) {
-    for (int s = 0; s < p.stages; ++s) {
+    for (int s = 0; s < p.ring.stages; ++s) {
       mbar_init(full_bar(s), LOADERS + GATHER_THREADS);      // the weights (expect_tx) and the gatherers' threads
       mbar_init(empty_bar(s), UP ? CONSUMERS : CONSUMERS / DOWN_TURNS);
     }
@@ -334,11 +334,11 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     while (walk.next(r) && ok) {
       const int e = plan->job_expert[r.job];
       shape_of<UP, KMAJOR>(p, r, plan->job_count[r.job]);
-      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
+      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.ring.stages)) {
         const int s = at.stage, steps = min(r.nb, r.b1 - b);
         if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 21)) { ok = false; break; }
         mbar_arrive_expect_tx(full_bar(s), ((UP ? r.boxes * steps : steps) - mine + LOADERS - 1) / LOADERS * p.load_bytes);
-        uint32_t to = ring0 + s * p.stage_bytes;
+        uint32_t to = ring0 + s * p.ring.stage_bytes;
         int v = r.p0, i = mine;
         for (int t = 0; t < r.boxes; ++t, i -= steps, to += r.nb * p.box_bytes, v += UP ? (KMAJOR ? 1 : 2) * walk.per_tile : 0)
           for (; i < steps; i += LOADERS) {
@@ -371,7 +371,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
       const int x_block = r.groups * 1024;
       const uint8_t* src[4];
       bool have = false;
-      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
+      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.ring.stages)) {
         const int s = at.stage, steps = min(r.nb, r.b1 - b);
         if ((s & (GATHER_TURNS - 1)) != turn) continue;
         if (!have) {
@@ -385,7 +385,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
             }
         }
         if (!mbar_wait(empty_bar(s), at.phase ^ 1, abort_flag, p.status, 23)) { ok = false; break; }
-        const uint32_t dst = ring0 + s * p.stage_bytes + r.x_offset + mine;
+        const uint32_t dst = ring0 + s * p.ring.stage_bytes + r.x_offset + mine;
         const int k0 = b * BLOCK_K + chunk * 8;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -475,14 +475,14 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int q = 0; q < 4; ++q) part[c][m][g][q] = 0.f;
-      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.stages)) {
+      for (int b = r.b0; b < r.b1; b += r.nb, at.next(p.ring.stages)) {
         const int s = at.stage;
         if (!UP && (s & (DOWN_TURNS - 1)) != (warp >> 1)) continue;
         mine = true;
         if (ok) ok = mbar_wait_warp(full_bar(s), at.phase, abort_flag, p.status, 22);
         if (ok && use0) {
           const int steps = min(r.nb, r.b1 - b);
-          uint32_t w = ring0 + s * p.stage_bytes + (UP ? (KMAJOR ? tl : tl >> 1) * r.nb * p.box_bytes : 0), x = ring0 + s * p.stage_bytes + r.x_offset;
+          uint32_t w = ring0 + s * p.ring.stage_bytes + (UP ? (KMAJOR ? tl : tl >> 1) * r.nb * p.box_bytes : 0), x = ring0 + s * p.ring.stage_bytes + r.x_offset;
           auto step = [&](int i, float (&to)[M][G][4]) {       // the i-th 16 of K of a box
             uint32_t a0[4], a1[4], bx[G + 1][2];
             if (KMAJOR) {
@@ -765,31 +765,10 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   p.load_bytes = rows * BLOCK_K * 2;
   p.box_bytes = cdiv(rows, 8) * 1024;                      // boxes start on the swizzle's period
   p.blocks = cdiv(p.K, BLOCK_K);
-  const int slack = 2048;      // ldmatrix reads whole 16-row blocks: past a box of fewer rows (never used, but inside the ring)
-  // Stages of up to 48 KB, weights and beside them the rows of the job's slots: four, or as many more (a multiple of the turns) as the
-  // ring holds where the whole of K needs less.
   constexpr int TURNS = UP ? GATHER_TURNS : DOWN_TURNS;
   static_assert(4 % TURNS == 0, "every stage belongs to the same warps in every pass");
-  const int most_groups = a.T < 32 ? cdiv(a.T, 8) : 4;
-  p.stage_bytes = (budget - slack) / 4 / 1024 * 1024;
-  if (p.stage_bytes > 48 * 1024) p.stage_bytes = 48 * 1024;
-  const int whole = p.blocks * (p.box_bytes + most_groups * 1024);
-  if (!UP && whole < p.stage_bytes) p.stage_bytes = whole;
-  p.stages = (budget - slack) / p.stage_bytes;
-  p.stages = (p.stages > MAX_STAGES ? MAX_STAGES : p.stages) / TURNS * TURNS;
-  if (p.stages < TURNS) return SMOE_ERR_UNSUPPORTED;
-  for (int c = 0; c < 4; ++c)
-    for (int g = 0; g < 4; ++g) {
-      const int boxes = 1 << c;      // the most of their class; never more than 32 KB of weights in the up-projection's rounds
-      int steps = p.stage_bytes / (boxes * p.box_bytes + (g + 1) * 1024);
-      if (UP && steps > 32768 / (boxes * p.box_bytes)) steps = 32768 / (boxes * p.box_bytes);
-      if (steps < 1) {
-        if (g < most_groups && boxes * p.box_bytes <= (UP ? 32768 : p.box_bytes)) return SMOE_ERR_UNSUPPORTED;
-        steps = 1;                   // never asked for
-      }
-      p.steps_of[c][g] = cdiv(p.blocks, cdiv(p.blocks, steps));
-    }
-  p.ring_bytes = p.stages * p.stage_bytes + slack;
+  if (!make_stages(&p.ring, UP, budget, p.box_bytes, p.blocks, a.T, a.k, TURNS)) return SMOE_ERR_UNSUPPORTED;
+  p.ring_bytes = p.ring.stages * p.ring.stage_bytes + RING_SLACK;
   const int scratch = (plan_scratch_bytes(a.E) + 15) / 16 * 16;      // the plan sorts in the ring before the first copy
   if (scratch > budget) return SMOE_ERR_UNSUPPORTED;
   if (p.ring_bytes < scratch) p.ring_bytes = scratch;

@@ -348,3 +348,19 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="no backward"):
         sm.mlp.GLUMLP(64, 64, 4, 2).cuda()
         sm.few_token_mlp(p["x"].float(), p["up"].float().requires_grad_(), p["down"].float(), None, p["ids"], FIRST, SILU)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+@pytest.mark.parametrize("T,k,F", [(1, 8, 64), (1, 32, 128), (2, 16, 8), (8, 4, 64), (8, 8, 128), (9, 3, 72), (16, 2, 64), (16, 8, 128)])
+def test_few_tokens_that_name_an_expert_many_times(dtype, order, T, k, F):
+    """Jobs of more slots than there are tokens beside short sums over K: a stage has to hold the rows of them all. Three experts, so
+    that neighbouring stages are in flight; then one."""
+    for d_out in (64, 2416):
+        p = problem(T, 64, F, 40, k, DT[dtype], FIRST, order, d_out=d_out)
+        g = torch.Generator().manual_seed(T * k + F)
+        p["ids"] = torch.randint(3, 6, (T, k), generator=g).cuda()
+        verify(p, FIRST)
+        p["ids"][:] = 7
+        got = verify(p, FIRST)
+        assert torch.equal(got, run(p, FIRST))
