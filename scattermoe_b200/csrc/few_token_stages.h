@@ -38,9 +38,9 @@ inline bool make_stages(Stages* out, bool up, int ring, int box_bytes, int block
   out->stage_bytes = (ring - RING_SLACK) / 4 / 1024 * 1024;
   if (out->stage_bytes > MAX_STAGE_BYTES) out->stage_bytes = MAX_STAGE_BYTES;
   const int least = box_bytes + most_groups * GROUP_BYTES;
-  int whole = blocks * (box_bytes + usual_groups * GROUP_BYTES);
+  int64_t whole = static_cast<int64_t>(blocks) * (box_bytes + usual_groups * GROUP_BYTES);
   if (whole < least) whole = least;
-  if (!up && whole < out->stage_bytes) out->stage_bytes = whole;
+  if (!up && whole < out->stage_bytes) out->stage_bytes = static_cast<int>(whole);
   if (out->stage_bytes < least) return false;
   out->stages = (ring - RING_SLACK) / out->stage_bytes;
   out->stages = (out->stages > MAX_STAGES ? MAX_STAGES : out->stages) / turns * turns;

@@ -83,3 +83,14 @@ def test_slots_of_few_tokens_on_one_expert(lib):
     ring, box, _ = launch(False, True, 64, 64, 8)
     assert box == 1024 and lib.stages(0, ring, box, 1, 8, 8, 4, out)
     assert out[1] >= 1024 + 4 * 1024 and out[2 + 3] == 1
+
+
+@pytest.mark.parametrize("k_major", [True, False])
+def test_long_sums(lib, k_major):
+    """The whole of K as bytes passes 32 bits long before K reaches its limit of 2^28: the stages are those of any other long K."""
+    ring, box, _ = launch(False, k_major, 1 << 20, 64, 24)
+    out, long = (ctypes.c_int * 18)(), (ctypes.c_int * 18)()
+    assert lib.stages(0, ring, box, (1 << 20) // 64, 24, 2, 4, out)
+    for K in ((1 << 25) + 8, 1 << 26, (1 << 27) + 64, (1 << 28) - 8):
+        assert lib.stages(0, ring, box, ceil(K, 64), 24, 2, 4, long)
+        assert list(long[:2]) == list(out[:2]), K
