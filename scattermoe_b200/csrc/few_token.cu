@@ -236,7 +236,8 @@ __device__ __forceinline__ float hidden_fast(int layout, int act, float alpha, f
   return r * lin;
 }
 
-// What adapter `id` adds to columns o and o + 16 of row t (second: whether the latter is wanted).
+// What adapter `id` adds to columns o and o + 16 of row t (second: whether the latter is wanted). h is read coherently: the kernel before
+// this one writes it while this one already runs.
 template <typename T>
 __device__ __forceinline__ void extension_terms(const Extension& x, int t, int id, int o, bool second, float (&sum)[2]) {
   sum[0] = sum[1] = 0.f;
@@ -247,7 +248,7 @@ __device__ __forceinline__ void extension_terms(const Extension& x, int t, int i
   if (x.m_vec) {
 #pragma unroll 4
     for (int j = 0; j < x.r; j += 8) {
-      const uint4 hv = __ldg(reinterpret_cast<const uint4*>(h + j)), m0 = __ldg(reinterpret_cast<const uint4*>(m + j)),
+      const uint4 hv = *reinterpret_cast<const uint4*>(h + j), m0 = __ldg(reinterpret_cast<const uint4*>(m + j)),
                   m1 = __ldg(reinterpret_cast<const uint4*>(m + next + j));
       const T *ht = reinterpret_cast<const T*>(&hv), *t0 = reinterpret_cast<const T*>(&m0), *t1 = reinterpret_cast<const T*>(&m1);
 #pragma unroll

@@ -68,8 +68,8 @@ __host__ __device__ inline int plan_scratch_bytes(int E) { return PLAN_WARPS * E
 
 // Whole-block call (at least PLAN_WARPS warps). Ids outside [0, E) belong to no job; without `ids` every slot is expert 0's. Ends with a
 // barrier.
-__device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* __restrict__ ids, int64_t sit, int64_t sik, int T,
-                                 int k, int E, int NT) {
+__device__ inline void make_plan(Plan* plan, uint8_t* scratch, const int64_t* ids, int64_t sit, int64_t sik, int T, int k,
+                                 int E, int NT) {
   const int tid = threadIdx.x, nthreads = blockDim.x, warp = tid >> 5, lane = tid & 31;
   uint32_t* packed = reinterpret_cast<uint32_t*>(scratch);                    // [E] count | jobs << 16, then their prefixes
   uint16_t* hist = reinterpret_cast<uint16_t*>(scratch + ((E * 4 + 15) & ~15));   // [PLAN_WARPS][E]
