@@ -12,6 +12,7 @@ import threading
 from ctypes import c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 
 from . import build as _build
 
@@ -177,6 +178,16 @@ def require_cuda(t: torch.Tensor, name: str):
         raise RuntimeError(
             "scattermoe_b200: `%s` is on %s; this package runs on CUDA (sm_100a) only and has no CPU path"
             % (name, t.device))
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raise if an operand carries a forward-mode tangent. For entry points that may launch without an autograd function: a dual tensor
+    does not require a gradient, and its tangent would be dropped. (While torch.compile traces, the registered operators refuse.)"""
+    if torch.compiler.is_compiling() or getattr(forward_ad, "_current_level", 0) < 0:      # outside any dual level: the usual case
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s has no forward-mode derivative: an operand carries a tangent" % what)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -10,7 +10,7 @@ Two launches forward: the shrink into the rank (h = s A x; in 16 bits rounded on
 B h before they are rounded once: the adapted output is never read back. Backward mirrors it (g = s B^T dy, then
 dx = W^T dy + A^T g in one launch) and sums the outer products dA_a = sum g x^T, dB_a = sum dy h^T per adapter in a fixed
 order. Gradients nobody asked for are not computed; adapters without rows get zeros; `scaling` is a constant. Infinities and NaN
-in one adapter, or in one row, stay with the rows they belong to.
+in one adapter, or in one row, stay with the rows they belong to. Forward-mode derivatives are refused.
 
 A training step can be captured into a CUDA graph as any other autograd function: warm up on the capturing side stream, and let go of
 eager graphs of the same leaves first (torch ends the process where a captured backward meets one).
@@ -186,7 +186,9 @@ def adapter_linear(inputs, weight, lora_a, lora_b, adapter_idxs, scaling=1.0, bi
             raise RuntimeError("%s: `scaling` is a constant, it cannot require a gradient" % what)
         if scaling.device != dev:
             raise RuntimeError("%s: `scaling` is on %s, the inputs are on %s" % (what, scaling.device, dev))
+        _lib.refuse_tangents(what, scaling)
         per_adapter, scaling = scaling.float().contiguous(), 1.0
+    _lib.refuse_tangents(what, inputs, weight, lora_a, lora_b, bias)
     lead = inputs.shape[:-1]
     x = inputs if inputs.dim() == 2 else inputs.reshape(-1, width)
     ids = adapter_idxs.reshape(-1)

@@ -11,7 +11,7 @@ here are that form:
 At most `max_tokens()` tokens and 1024 slots (tokens x k); the sort into experts happens inside the kernels, so no
 `flatten_sort_count` is needed. A slot whose id lies outside [0, E) contributes nothing (a padded batch marks its empty rows
 with -1; a row without any expert comes out as zeros, whatever its input holds). Results are bit-equal from call to call.
-Nothing is kept for backward: inputs that require gradients are refused while gradients are enabled.
+Nothing is kept for backward: inputs that require gradients are refused while gradients are enabled, forward-mode tangents always.
 """
 from __future__ import annotations
 
@@ -38,6 +38,7 @@ def max_tokens() -> int:
 
 
 def _refuse_grad(what, *tensors):
+    _lib.refuse_tangents(what, *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
