@@ -10,6 +10,19 @@ namespace smoe {
 enum { LAYOUT_PLAIN = 0, LAYOUT_GLU_SECOND = 1, LAYOUT_GLU_FIRST = 2, LAYOUT_GPT_OSS = 3 };
 enum { ACT_SILU = 0, ACT_GELU_ERF = 1, ACT_GELU_TANH = 2, ACT_RELU = 3, ACT_IDENTITY = 4 };
 
+// The smaller and the larger of two values, NaN where either is: clamps and ReLU keep a NaN as torch's do (fminf, fmaxf and a comparison
+// give the other value, and a broken layer returns plausible numbers). One instruction, as fminf.
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // FAST (16-bit storage): hardware exp2 / reciprocal approximations, relative error ~1e-6, far below the 2^-9 of
 // the rounding to bf16 that follows; the IEEE expf + division of the exact path made these kernels ALU-bound
 // (2.7 TB/s measured on the backward pass). fp32 storage keeps the exact path.
@@ -29,7 +42,7 @@ __device__ __forceinline__ float act_fwd(float x) {
     const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
     return 0.5f * x * (1.0f + tanhf(u));
   }
-  if (ACT == ACT_RELU) return x > 0.f ? x : 0.f;
+  if (ACT == ACT_RELU) return max_nan(x, 0.f);
   return x;
 }
 

@@ -69,8 +69,8 @@ act_forward_kernel(const T* __restrict__ U, int64_t su, T* __restrict__ H, int64
     for (int i = 0; i < V; ++i) {
       const float g0 = (2 * i < V) ? a[(2 * i) % V] : b[(2 * i) % V];
       const float u0 = (2 * i + 1 < V) ? a[(2 * i + 1) % V] : b[(2 * i + 1) % V];
-      const float g = fminf(g0, limit);
-      const float uc = fminf(fmaxf(u0, -limit), limit);
+      const float g = min_nan(g0, limit);
+      const float uc = min_nan(max_nan(u0, -limit), limit);
       out[i] = (uc + 1.0f) * (g * sigmoidf_<FAST>(alpha * g));
     }
   } else {
@@ -114,8 +114,8 @@ act_backward_kernel(const T* __restrict__ U, int64_t su, const T* __restrict__ D
     for (int i = 0; i < V; ++i) {
       const float g0 = (2 * i < V) ? a[(2 * i) % V] : b[(2 * i) % V];
       const float u0 = (2 * i + 1 < V) ? a[(2 * i + 1) % V] : b[(2 * i + 1) % V];
-      const float g = fminf(g0, limit);
-      const float uc = fminf(fmaxf(u0, -limit), limit);
+      const float g = min_nan(g0, limit);
+      const float uc = min_nan(max_nan(u0, -limit), limit);
       const float s = sigmoidf_<FAST>(alpha * g);
       const float glu = g * s;
       const float d_u = (u0 >= -limit && u0 <= limit) ? dh[i] * glu : 0.f;

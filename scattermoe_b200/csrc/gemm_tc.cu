@@ -392,8 +392,8 @@ __device__ __forceinline__ void epilogue_rows(const S2SParams& p, int n0, uint32
           for (int jj = 0; jj < 8; ++jj) {
             const float g0 = (jj < 4) ? v0[2 * jj] : v1[2 * jj - 8];
             const float u0 = (jj < 4) ? v0[2 * jj + 1] : v1[2 * jj - 7];
-            const float gc = fminf(g0, p.limit);
-            const float uc = fminf(fmaxf(u0, -p.limit), p.limit);
+            const float gc = min_nan(g0, p.limit);
+            const float uc = min_nan(max_nan(u0, -p.limit), p.limit);
             h[jj] = hscale * (uc + 1.0f) * (gc * sigmoidf_<true>(p.alpha * gc));
           }
           py[2 * gg] = pack8(v0, p.is_bf16);
@@ -546,8 +546,8 @@ __device__ __forceinline__ bool epilogue_act_bwd(const S2SParams& p, int n0, uin
             const float up0 = (jj < 4) ? u0[2 * jj + 1] : u1[2 * jj - 7];
             const float a0 = __uint_as_float(acc[hh * 16 + g * 8 + jj]);
             const float dh = rg * a0;
-            const float gc = fminf(g0, p.limit);
-            const float uc = fminf(fmaxf(up0, -p.limit), p.limit);
+            const float gc = min_nan(g0, p.limit);
+            const float uc = min_nan(max_nan(up0, -p.limit), p.limit);
             const float sg = sigmoidf_<true>(p.alpha * gc);
             dot = fmaf(a0, (uc + 1.0f) * (gc * sg), dot);
             const float d_u = (up0 >= -p.limit && up0 <= p.limit) ? dh * (gc * sg) : 0.f;
