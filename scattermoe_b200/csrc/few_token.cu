@@ -226,7 +226,7 @@ __device__ __forceinline__ void shape_of(const StreamParams& p, Run& r, int n) {
 // hidden value from the up-projection's one or two columns (act_math.cuh has the layouts)
 __device__ __forceinline__ float hidden_fast(int layout, int act, float alpha, float limit, float c0, float c1) {
   if (layout == LAYOUT_GPT_OSS) {
-    const float g = fminf(c0, limit), u = fminf(fmaxf(c1, -limit), limit);
+    const float g = min_nan(c0, limit), u = min_nan(max_nan(c1, -limit), limit);
     return (u + 1.0f) * (g * sigmoidf_<true>(alpha * g));
   }
   const float gate = layout == LAYOUT_GLU_SECOND ? c1 : c0;

@@ -29,7 +29,7 @@ __device__ __forceinline__ float act_exact(float x) { return act_fwd<ACT, false>
 // hidden value from the up-projection's one or two columns (biases added), see act_math.cuh for the layouts
 __device__ __forceinline__ float hidden_value(int layout, int act, float alpha, float limit, float c0, float c1) {
   if (layout == LAYOUT_GPT_OSS) {
-    const float g = fminf(c0, limit), u = fminf(fmaxf(c1, -limit), limit);
+    const float g = min_nan(c0, limit), u = min_nan(max_nan(c1, -limit), limit);
     return (u + 1.0f) * (g * sigmoidf_<false>(alpha * g));
   }
   const float gate = layout == LAYOUT_GLU_SECOND ? c1 : c0;
