@@ -30,7 +30,8 @@
 //
 // The down-projection starts (programmatic launch) while the up-projection drains: it plans and fills its ring with weights, which do not
 // depend on the hidden rows, and waits only before the first hidden row is read.
-// fp32 accumulation; the hidden rows carry the gate and are rounded once, as the tensor cores need them.
+// fp32 accumulation; the hidden rows are rounded once, as the tensor cores need them, and carry the gate's power of two (see `carried`),
+// the token sums take the rest of it.
 #include <cuda.h>
 #include <string.h>
 
@@ -223,6 +224,14 @@ __device__ __forceinline__ void shape_of(const StreamParams& p, Run& r, int n) {
   r.x_offset = r.boxes * r.nb * p.box_bytes;
 }
 
+// The part of a gate that its hidden row carries: the power of two at or below it, between 1/16 and 1. Scaling by it costs no bit, and
+// it leaves fp16 the headroom that a gate below 1 gives. A whole gate of 2^-18 would push fp16's rows below their normal range, where
+// the step no longer shrinks (4 times the error that the rounding itself explains); no more than 1/16 keeps that at 2^-21 of a hidden
+// value of 1.
+__device__ __forceinline__ int carried_exponent(float gate) { return min(max(__float_as_int(gate) >> 23 & 0xff, 127 - 4), 127); }
+__device__ __forceinline__ float carried(float gate) { return __int_as_float(carried_exponent(gate) << 23); }
+__device__ __forceinline__ float rest_of(float gate) { return gate * __int_as_float((254 - carried_exponent(gate)) << 23); }
+
 // hidden value from the up-projection's one or two columns (act_math.cuh has the layouts)
 __device__ __forceinline__ float hidden_fast(int layout, int act, float alpha, float limit, float c0, float c1) {
   if (layout == LAYOUT_GPT_OSS) {
@@ -277,7 +286,8 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
   uint64_t* bars = reinterpret_cast<uint64_t*>(token + MAX_R);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + 2 * MAX_STAGES);
   int* joined = reinterpret_cast<int*>(bars + 2 * MAX_STAGES) + 1;
-  float* sums = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // down: [warp][T][rows + 1]; up: the listed slots' gates (or adapters)
+  float* per_slot = reinterpret_cast<float*>(bars + 2 * MAX_STAGES + 2);  // the listed slots' parts of the gate (or, as integers, adapters)
+  float* sums = per_slot + MAX_R;                                    // down: [warp][T][rows + 1]; up: the warps' accumulators
   const int pitch = p.rows + 1;
   const Args& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -301,12 +311,19 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     if (blockIdx.x == 0)
       for (int i = tid; i < p.n_counters; i += THREADS) p.counters[i] = 0;
   }
-  // ids are older than the up-projection, so the down-projection plans before it waits
+  // ids and gates are older than the up-projection, so the down-projection plans before it waits
   make_plan(plan, ring, a.ids, a.sit, a.sik, a.T, a.k, a.E, p.NT);
   const int listed = plan->jobs ? plan->job_begin[plan->jobs - 1] + plan->job_count[plan->jobs - 1] : 0;
   for (int i = tid; i < listed; i += THREADS) {
     const int slot = plan->slots[i], t = slot / a.k;
     token[i] = static_cast<uint8_t>(t);
+    if (UP && p.ext.ids) {      // the row's adapter
+      const int64_t id = p.ext.ids[t];
+      per_slot[i] = __int_as_float(id >= 0 && id < p.ext.n ? static_cast<int>(id) : -1);
+    } else {
+      const float gate = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
+      per_slot[i] = UP ? carried(gate) : rest_of(gate);
+    }
   }
   fence_proxy_async_smem();            // the plan's scratch in the ring was written with ordinary stores
   __syncthreads();
@@ -405,20 +422,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 
   // ---------------- products -----------------------------------------------------------------------------------
   // a wait that runs out does not leave the loops: the barriers below stay matched, the results are reported as invalid
-  if (UP) {
-    for (int i = tid; i < listed; i += CONSUMERS * 32) {
-      const int slot = plan->slots[i], t = token[i];
-      if (p.ext.ids) {      // the row's adapter
-        const int64_t id = p.ext.ids[t];
-        sums[i] = __int_as_float(id >= 0 && id < p.ext.n ? static_cast<int>(id) : -1);
-      } else {
-        sums[i] = a.gates ? load_any(a.gates, t * a.sgt + (slot - t * a.k) * a.sgk, a.gates_dtype) : 1.f;
-      }
-    }
-    consumers_sync();
-  } else {
-    wait_for_previous_kernel();
-  }
+  if (!UP) wait_for_previous_kernel();
   bool ok = true;
   RingPos at;
   Run r;
@@ -552,7 +556,7 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
     if (UP) {
       // The sums go through shared memory, where the warps of a tile meet (each then takes every team-th value of all) and where a
       // short loop can pick them up: unrolled over the registers the epilogue outgrew the instruction cache (10 us and more).
-      float* red = sums + MAX_R;
+      float* red = sums;
 #pragma unroll
       for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -587,10 +591,10 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
           }
           if (i >= n) continue;
           const int slot = plan->slots[beg + i];
-          const float gate = p.ext.ids ? 1.f : sums[beg + i];
+          const float gate = p.ext.ids ? 1.f : per_slot[beg + i];
           float extra[2] = {0.f, 0.f};
           if (p.ext.ids && v[0] < count)
-            extension_terms<T>(p.ext, slot, __float_as_int(sums[beg + i]), v0 + v[0], v[1] < count, extra);
+            extension_terms<T>(p.ext, slot, __float_as_int(per_slot[beg + i]), v0 + v[0], v[1] < count, extra);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (v[h] < 0 || v[h] >= count) continue;
@@ -620,11 +624,13 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
 #pragma unroll
           for (int m = 0; m < M; ++m) {
             float* to[4];
+            float gate[4];
             bool in[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               const int i = g * 8 + (lane & 3) * 2 + (q & 1), row = m * 16 + (lane >> 2) + (q >> 1) * 8;
               to[q] = own + token[beg + min(i, n - 1)] * pitch + row;
+              gate[q] = per_slot[beg + min(i, n - 1)];
               in[q] = i < n && m0 + row < count;
             }
             if (!twice) {      // all different: read, add, write
@@ -633,13 +639,13 @@ ft_stream_kernel(const __grid_constant__ CUtensorMap tmap, const StreamParams p)
               for (int q = 0; q < 4; ++q) v[q] = in[q] ? *to[q] : 0.f;
 #pragma unroll
               for (int q = 0; q < 4; ++q)
-                if (in[q]) *to[q] = v[q] + acc[m][g][q];
+                if (in[q]) *to[q] = fmaf(gate[q], acc[m][g][q], v[q]);
             } else {
               for (int turn = 0; turn < 4; ++turn) {
                 if ((lane & 3) == turn) {
 #pragma unroll
                   for (int q = 0; q < 4; ++q)
-                    if (in[q]) *to[q] += acc[m][g][q];
+                    if (in[q]) *to[q] = fmaf(gate[q], acc[m][g][q], *to[q]);
                 }
                 __syncwarp();
               }
@@ -759,8 +765,8 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
   const Args& a = p.a;
   p.rows = UP ? 0 : (KMAJOR ? down_rows(a.d_out, grid) : 2 * TILE);
   // shared memory that is not the ring
-  const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 +
-                    (UP ? MAX_R * 4 + CONSUMERS * 32 * 32 * 4 : (p.rows > 16 ? CONSUMERS / 2 : CONSUMERS) * a.T * (p.rows + 1) * 4) + 1024 + 64;
+  const int fixed = static_cast<int>(sizeof(Plan)) + MAX_R + (2 * MAX_STAGES + 2) * 8 + MAX_R * 4 +
+                    (UP ? CONSUMERS * 32 * 32 * 4 : (p.rows > 16 ? CONSUMERS / 2 : CONSUMERS) * a.T * (p.rows + 1) * 4) + 1024 + 64;
   const int budget = (di.max_smem_optin < 232448 ? di.max_smem_optin : 232448) - fixed;
   const int rows = KMAJOR ? (UP ? TILE : p.rows) : 2 * TILE;
   p.load_bytes = rows * BLOCK_K * 2;

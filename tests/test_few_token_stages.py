@@ -47,7 +47,7 @@ def ceil(a, b):
 def launch(up, k_major, K, d_out, T):
     """(bytes for the ring, bytes of a box, boxes a stage can be wide) as the launcher derives them."""
     rows = min(ceil(d_out, GRID), TILE) if k_major else 2 * TILE
-    sums = MAX_R * 4 + CONSUMERS * 32 * 32 * 4 if up else (CONSUMERS // 2 if rows > 16 else CONSUMERS) * T * (rows + 1) * 4
+    sums = MAX_R * 4 + (CONSUMERS * 32 * 32 * 4 if up else (CONSUMERS // 2 if rows > 16 else CONSUMERS) * T * (rows + 1) * 4)
     box_rows = (TILE if up else rows) if k_major else 2 * TILE
     widths = range(1, (CONSUMERS if k_major else CONSUMERS // 2) + 1) if up else [1]
     return MOST_SMEM - (PLAN + MAX_R + BARRIERS + sums + 1024 + 64), ceil(box_rows, 8) * 1024, widths

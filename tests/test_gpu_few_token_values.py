@@ -1,4 +1,4 @@
-"""The few-token MoE layer on values that are not numbers and on wide outputs. Bounds as in test_gpu_few_token.py."""
+"""The few-token MoE layer on values that are not numbers, on small gates and on wide outputs. Bounds as in test_gpu_few_token.py."""
 import pytest
 import torch
 
@@ -52,6 +52,38 @@ def test_infinities_meet_the_clamps(dtype):
             far = dict(p, up_b=p["up_b"].clone())
             far["up_b"][:, col] = 1000.0 if v > 0 else -1000.0
             assert torch.equal(run(q, OSS), run(far, OSS))
+
+
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+@pytest.mark.parametrize("layout", [PLAIN, FIRST, OSS])
+def test_small_gates(order, layout):
+    """Gates of 2^-18 on outputs of ordinary size, in fp16. A hidden row that carried the whole gate would lie below fp16's normal range,
+    where a rounding is off by 2^-25 whatever the value. It carries at least 1/16: the bound has half a step of the hidden value, and
+    16 x 2^-25 where that is less."""
+    p = problem(9, 96, 64, 5, 2, torch.float16, layout, order)
+    p["down"] = p["down"] * 512
+    p["gates"] = torch.full((9, 2), 2.0 ** -18, device="cuda")
+    for _ in range(2):
+        y, bound = reference(p["x"], p["up"], p["down"], p["gates"], p["ids"], layout, SILU)
+        columns = p["down"].cpu().double().abs().sum(1)                      # (E, d_out)
+        bound = bound + 2.0 ** -21 * (p["gates"].cpu().double().unsqueeze(2) * columns[p["ids"].cpu()]).sum(1)
+        check(run(p, layout), y, bound)
+        p["gates"] = p["gates"] * torch.rand(9, 2, generator=torch.Generator().manual_seed(3)).cuda()
+
+
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+@pytest.mark.parametrize("gate", [1 / 16, 0.1, 0.5])
+def test_gates_leave_headroom(order, gate):
+    """Hidden values past fp16's largest, 65504, whose gated values are not: finite and right, as the gate's power of two goes in front
+    of the rounding."""
+    p = problem(9, 96, 64, 5, 1, torch.float16, PLAIN, order)
+    h = p["x"].cpu().double() @ p["up"].cpu().double()[0]
+    p["x"] = (p["x"].float() * 80000 / h.abs().max().item() ** 0.5 / 256).half()
+    p["up"] = (p["up"].float() * 256 / h.abs().max().item() ** 0.5).half()       # hidden values of up to about 80000
+    p["down"] = p["down"] / 16
+    p["gates"] = torch.full((9, 1), gate, device="cuda")
+    y, bound = reference(p["x"], p["up"], p["down"], p["gates"], p["ids"], PLAIN, IDENT)
+    check(run(p, PLAIN, IDENT), y, bound)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
