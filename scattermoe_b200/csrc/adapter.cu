@@ -225,12 +225,16 @@ grad_simt_kernel(const GradArgs a) {
       vs[m][c] = (m < cnt && c0 + c < a.C) ? to_f32<T>(__ldg(static_cast<const T*>(a.V) + rows[m] * a.svm + c0 + c)) : 0.f;
     }
     __syncthreads();
+    // a sum of its own for every step: one chain over all rows of an adapter would be off by as many roundings as there are rows
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
     for (int m = 0; m < cnt; ++m) {
       const float v = vs[m][cx];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(us[m][jg * 4 + i], v, acc[i]);
+      for (int i = 0; i < 4; ++i) part[i] = fmaf(us[m][jg * 4 + i], v, part[i]);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[i] += part[i];
     __syncthreads();
   }
   if (c0 + cx >= a.C) return;
