@@ -330,10 +330,18 @@ static int check_common(const char* who, int64_t T, int n, int in, int out, int 
   return SMOE_OK;
 }
 
+static int refuse_tc(const char* what, int dtype, int C) {
+  set_error("adapter_linear: no tensor-core kernel for this dtype/alignment (%s, dtype=%d width=%d)", what, dtype, C);
+  return SMOE_ERR_UNSUPPORTED;
+}
+
 static int shrink(const ShrinkArgs& a, int flags) {
-  if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
+  // A warp per token and 4 rank rows reads M again for every token, but spreads few tokens over the GPU: the choice for them, not a way out.
+  const bool few = a.T <= SHRINK_FEW_TOKENS && a.smc == 1;
+  if (!(flags & SMOE_FLAG_FORCE_SIMT) && !few) {
     const int rc = launch_shrink_tc(a);
     if (rc != SMOE_ERR_UNSUPPORTED) return rc;
+    if (flags & SMOE_FLAG_FORCE_TC) return refuse_tc("shrink", a.dtype, a.C);
   }
   return launch_shrink_simt(a);
 }
@@ -359,6 +367,7 @@ static int outer(const GradArgs& a, int flags) {
   if (!(flags & SMOE_FLAG_FORCE_SIMT)) {
     const int rc = launch_grad_tc(a);
     if (rc != SMOE_ERR_UNSUPPORTED) return rc;
+    if (flags & SMOE_FLAG_FORCE_TC) return refuse_tc("outer products", a.dtype, a.C);
   }
   return launch_grad_simt(a);
 }
@@ -505,7 +514,7 @@ extern "C" int smoe_adapter_backward(const void* DY, int64_t T, int64_t stride_d
     ad::set_rows_kernel<<<1, 1, 0, st>>>(rows, T);
     SMOE_LAUNCH_CHECK();
     return smoe_group_bwd_w(DY, stride_dym, 1, X, T, stride_xm, 1, rows, nullptr, 1, DW, static_cast<int64_t>(out) * in, 1, in, Dbias,
-                            out, 1, T, in, out, 1, dtype, flags & SMOE_FLAG_FORCE_SIMT, status, stream);
+                            out, 1, T, in, out, 1, dtype, flags & (SMOE_FLAG_FORCE_SIMT | SMOE_FLAG_FORCE_TC), status, stream);
   }
   if (Dbias) return ad::column_sum(DY, T, stride_dym, out, Dbias, dtype, parts, st);
   return SMOE_OK;

@@ -16,6 +16,7 @@ namespace ad {
 
 constexpr int MAX_RANK = 256;
 constexpr int FEW_TOKENS = 128;      // up to here the product is a read of W (few_token.cu)
+constexpr int SHRINK_FEW_TOKENS = 256;      // up to here a shrink with contiguous inputs takes a warp per token (adapter.cu)
 constexpr int64_t rank_pitch(int r) { return (r + 7) / 8 * 8; }
 
 struct ShrinkArgs {           // H[t, j] = s_a sum_c X[t, c] M[a][j, c]

@@ -248,8 +248,6 @@ shrink_tc_kernel(const ShrinkParams p) {
 int launch_shrink_tc(const ShrinkArgs& a) {
   if (a.dtype != SMOE_BF16 && a.dtype != SMOE_F16) return SMOE_ERR_UNSUPPORTED;
   if (a.C % 8 || a.sxm % 8 || !al16(a.X) || a.T >= (int64_t(1) << 31) - 64) return SMOE_ERR_UNSUPPORTED;
-  // A warp per token and 4 rank rows reads M again for every token, but spreads few tokens over the GPU.
-  if (a.T <= 256 && a.smc == 1) return SMOE_ERR_UNSUPPORTED;
   ShrinkParams p;
   p.a = a;
   const int r8 = static_cast<int>(rank_pitch(a.r));
