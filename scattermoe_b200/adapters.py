@@ -209,8 +209,8 @@ class AdapterLinear(nn.Module):
     """A linear layer with `num_adapters` low-rank adapters beside it; each row names its adapter.
 
     Parameters: weight (out, in) and bias (out,) as nn.Linear, lora_a (n, r, in) ~ N(0, 1/in), lora_b (n, out, r) zeros (a new
-    adapter changes nothing). `scaling` (n,) is a buffer, alpha / rank by default. `freeze_shared=True` (default) trains the adapters
-    alone."""
+    adapter changes nothing). `scaling` (n,) is a buffer, alpha / rank by default, and stays fp32 when
+    the module is cast. `freeze_shared=True` (default) trains the adapters alone."""
 
     def __init__(self, in_features, out_features, num_adapters, rank, bias=False, alpha=None, freeze_shared=True) -> None:
         super().__init__()
@@ -220,8 +220,17 @@ class AdapterLinear(nn.Module):
         self.bias = nn.Parameter(torch.zeros(out_features), requires_grad=not freeze_shared) if bias else None
         self.lora_a = nn.Parameter(torch.empty(num_adapters, rank, in_features))
         self.lora_b = nn.Parameter(torch.zeros(num_adapters, out_features, rank))
-        self.register_buffer("scaling", torch.full((num_adapters,), (alpha if alpha is not None else rank) / rank))
+        self.register_buffer("scaling", torch.full((num_adapters,), (alpha if alpha is not None else rank) / rank,
+                                                    dtype=torch.float32))
         self.reset_parameters()
+
+    def _apply(self, fn, recurse=True):
+        """Casts and moves of a module come through here: `scaling` moves, but keeps its 32 bits (0.1 would be off by 2^-10 of itself in bf16)."""
+        scaling = self.scaling
+        super()._apply(fn, recurse)
+        if self.scaling.dtype != scaling.dtype:
+            self.scaling = scaling.to(self.scaling.device)
+        return self
 
     def reset_parameters(self) -> None:
         nn.init.normal_(self.weight, std=0.02)
