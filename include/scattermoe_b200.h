@@ -268,7 +268,8 @@ int smoe_few_token_route(const void* X, int64_t T, int64_t stride_xm, const void
  *     the adapter's rows (zeros without rows);   DW = sum DY[t] X[t]^T;   Dbias = sum DY[t].   Each of DX, DA, DB, DW, Dbias may be
  *     null. H, sorted_idx and offsets are forward's. Every sum has a fixed order.
  * W (out, in), A (n, r, in), B (n, out, r) in element strides; X, DY rows with inner stride 1; Y, DX (T, .), H (T, r rounded up
- * to a multiple of 8, in `dtype`), DA, DB, DW (out, in), Dbias contiguous. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31 - 64. The workspace (16-byte aligned,
+ * to a multiple of 8, in `dtype`), DA, DB, DW (out, in), Dbias contiguous. SMOE_FLAG_FORCE_TC covers every product but a shrink of up to
+ * 256 rows over contiguous inputs, a CUDA-core kernel by choice. 1 <= r <= 256, 1 <= n <= 4096, T < 2^31 - 64. The workspace (16-byte aligned,
  * smoe_adapter_workspace_bytes; forward without a sort needs none) belongs to the call until its work has finished. */
 size_t smoe_adapter_workspace_bytes(int64_t T, int32_t n, int32_t in, int32_t out, int32_t r, int32_t dtype);
 int smoe_adapter_forward(const void* X, int64_t T, int64_t stride_xm,

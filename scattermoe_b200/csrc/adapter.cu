@@ -254,9 +254,9 @@ grad_simt_kernel(const GradArgs a) {
 
 int launch_shrink_simt(const ShrinkArgs& a) {
   // four rank rows per warp read the token's row a quarter as often; one each where there are too few warps to fill the GPU
-  const bool single = a.T * (rank_pitch(a.r) / 4) < 148 * 16;
+  const bool single = a.T * (rank_pitch(a.r) / 4) < SM_COUNT * 16;
   const int64_t warps = a.T * (rank_pitch(a.r) / (single ? 1 : 4));
-  const int grid = static_cast<int>(min(cdiv64(warps, 8), static_cast<int64_t>(148 * 32)));
+  const int grid = static_cast<int>(min(cdiv64(warps, 8), static_cast<int64_t>(SM_COUNT * 32)));
   const int v = 16 / dtype_size(a.dtype);
   auto al16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   const bool vec = a.smc == 1 && a.C % v == 0 && a.sxm % v == 0 && a.smj % v == 0 && a.sma % v == 0 && al16(a.X) && al16(a.M);
@@ -336,7 +336,9 @@ static int refuse_tc(const char* what, int dtype, int C) {
 }
 
 static int shrink(const ShrinkArgs& a, int flags) {
-  // A warp per token and 4 rank rows reads M again for every token, but spreads few tokens over the GPU: the choice for them, not a way out.
+  // A warp per token and 4 rank rows reads M again for every token, but spreads few tokens over the GPU: the choice for them, not a way
+  // out. The whole call, 4096 x 4096, rank 16, bf16: 129 to 256 rows of one adapter 34-35 us against 44-45 on tensor cores, of 8 adapters in
+  // no order 41-42 against 146; rank 64, 64 adapters 142-158 against 950 and more.
   const bool few = a.T <= SHRINK_FEW_TOKENS && a.smc == 1;
   if (!(flags & SMOE_FLAG_FORCE_SIMT) && !few) {
     const int rc = launch_shrink_tc(a);
@@ -380,7 +382,7 @@ static size_t up256(size_t b) { return (b + 255) / 256 * 256; }
 constexpr int SUM_COLS = 256, SUM_MAX_SLICES = 64;
 
 static int sum_slices(int64_t T, int C) {
-  const int64_t by_rows = cdiv64(T, 32), by_grid = cdiv64(148 * 8, cdiv(C, SUM_COLS));
+  const int64_t by_rows = cdiv64(T, 32), by_grid = cdiv64(SM_COUNT * 8, cdiv(C, SUM_COLS));
   const int64_t s = by_rows < by_grid ? by_rows : by_grid;
   return static_cast<int>(s < 1 ? 1 : (s > SUM_MAX_SLICES ? SUM_MAX_SLICES : s));
 }

@@ -6,7 +6,10 @@
 // Three products cover both directions: the SHRINK into the rank (h, g), the shared product with the EXPANSION out of the rank
 // added while the accumulators are at hand (y, dx), and the per-adapter sum of outer products (dA, dB).
 // h and g are rows of the rank padded with zeros to a multiple of 8 (rank_pitch), in the storage type: fp32, or rounded once to the
-// 16 bits that the tensor cores multiply (each rounding is at most half a step of a value that adds a correction to the product).
+// 16 bits that the tensor cores multiply (each rounding is at most half a step of a value that adds a correction to the product). CUDA
+// cores could do without that rounding. They share the form because the products of a call choose their kernels each for itself (the
+// input's width may be odd and the output's not) and backward reads the rows forward wrote; the output's error stays below 1.4 times
+// that of rounding it alone.
 #pragma once
 
 #include "smoe_common.cuh"
@@ -15,6 +18,8 @@ namespace smoe {
 namespace ad {
 
 constexpr int MAX_RANK = 256;
+constexpr int SM_COUNT = 148;        // of a B200. Grids, and the counts of parts that size a workspace: the size query needs no device and agrees
+                                     // with the launch
 constexpr int FEW_TOKENS = 128;      // up to here the product is a read of W (few_token.cu)
 constexpr int SHRINK_FEW_TOKENS = 256;      // up to here a shrink with contiguous inputs takes a warp per token (adapter.cu)
 constexpr int64_t rank_pitch(int r) { return (r + 7) / 8 * 8; }

@@ -297,7 +297,7 @@ constexpr int GR_STAGE = GR_ROWS * (GR_V_PITCH + GR_U_PITCH);
 constexpr int GR_SMEM = GR_STAGES * GR_STAGE;
 
 static int grad_chunks(int64_t T, int C, int r) {
-  const int64_t by_grid = cdiv64(2 * 148, static_cast<int64_t>(cdiv(C, GR_COLS)) * cdiv(r, GR_J)), by_rows = cdiv64(T, 256);
+  const int64_t by_grid = cdiv64(2 * SM_COUNT, static_cast<int64_t>(cdiv(C, GR_COLS)) * cdiv(r, GR_J)), by_rows = cdiv64(T, 256);
   const int64_t s = by_grid < by_rows ? by_grid : by_rows;
   return static_cast<int>(s < 1 ? 1 : (s > GR_MAX_CHUNKS ? GR_MAX_CHUNKS : s));
 }

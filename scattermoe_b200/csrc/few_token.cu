@@ -3,11 +3,12 @@
 //
 // Bound: the weights of the experts that occur cross HBM once; everything else is small. So the kernels are built around
 // that stream. One block per SM; four threads keep a ring of weight boxes in flight by TMA (4 KB each: 32 weight rows x 64 of K), two
-// warps gather the slots' rows beside them (cp.async), eight warps multiply what has arrived with mma.sync: 16 weight rows x 8 slots x
-// 16 of K per instruction. Weights are the M side, the job's slots the N side, so a job of 1 to 8 slots costs one instruction
-// per 16x16 weights and the tensor pipe stays far below its limit; a tcgen05 tile would need 128 weight rows at a time,
-// and with a handful of active experts the rows could not be spread evenly over 148 SMs. Here the split is exact: a block owns a
-// contiguous range of hidden values (up) or of output columns (down).
+// pairs of warps gather the slots' rows beside them, a stage each in turn (cp.async), eight warps multiply what has arrived with mma.sync:
+// 16 weight rows x 8 slots x 16 of K per instruction. Weights are the M side, the job's slots the N side, so a job of 1 to 8 slots costs
+// one instruction per 16x16 weights and the tensor pipe stays far below its limit up to about 16 slots. A tcgen05 tile is 64 or 128 weight
+// rows at least, and 4096 output columns are 28 per SM: tiles of a handful of active experts cannot be dealt evenly over 148 SMs, and a
+// stream has no use for the rate. Here the split is exact: a block owns a contiguous range of hidden values (up) or of output columns
+// (down).
 //
 //   up    A round is up to 8 tiles of one job, a tile 32 weight rows: 16 hidden values with their two columns, or 32 without a gate. Each
 //         warp owns a tile over the whole of K and makes its hidden values in registers: no exchange between warps, no barrier; the

@@ -1,4 +1,4 @@
-// Host-side tensor maps for the streaming kernels: 16-bit elements, up to three axes.
+// Host-side tensor maps for the streaming kernels: 16-bit elements, up to five axes.
 #pragma once
 
 #include <cuda.h>

@@ -136,7 +136,10 @@ def few_token_mlp(inputs, up_weights, down_weights, gates, expert_idxs, act_layo
     inputs (T, d); up_weights (E, d, n_up) and down_weights (E, hidden, d_out) as `expert_mlp` takes them (any strides);
     gates (T, k) in any of the three dtypes, or None for a plain sum; expert_idxs (T, k), ids outside [0, E) contribute
     nothing; layout / function codes as in `scattermoe_b200.activation`. Weights and biases have the tokens' dtype.
-    Returns (T, d_out). fp32 accumulation; on the tensor-core path the hidden rows are rounded once to the tokens' dtype."""
+    Returns (T, d_out). fp32 accumulation; on the tensor-core path the hidden rows are rounded once to the tokens' dtype.
+
+    The fast path is 16-bit, d and hidden multiples of 8, tokens and weights whose rows start on 16 bytes. fp32 and everything else take
+    CUDA-core kernels, exact but not tuned: measured at 0.85 to 6 times the speed of the same layer in elementary torch operations."""
     what = "few_token_mlp"
     _refuse_grad(what, inputs, up_weights, down_weights, gates, up_biases, down_biases)
     _lib.require_cuda(inputs, "inputs")
