@@ -730,8 +730,9 @@ size_t stream_workspace_bytes(int64_t T, int k, int F, int d_out) {
 }
 
 struct Order { bool k_major, n_major; };
-static Order weight_order(const void* W, int64_t se, int64_t sk, int64_t sn, int K, int N) {
-  if (!al16(W) || se % 8 || se < 0) return {false, false};
+// Experts that share one matrix (stride 0 of a broadcast view) are left to the CUDA cores: a tensor map's strides are not to be zero.
+static Order weight_order(const void* W, int E, int64_t se, int64_t sk, int64_t sn, int K, int N) {
+  if (!al16(W) || se % 8 || se < 0 || (se == 0 && E > 1)) return {false, false};
   return {sk == 1 && sn % 8 == 0 && sn >= K, sn == 1 && sk % 8 == 0 && sk >= N && N % 8 == 0};
 }
 
@@ -807,7 +808,7 @@ static int launch_one(StreamParams p, const CUtensorMap& map, const DeviceInfo& 
 template <typename T>
 static int launch_typed(const Args& a, const DeviceInfo& di) {
   const int n_up_cols = n_up(a);
-  const Order o1 = weight_order(a.W1, a.s1e, a.s1k, a.s1n, a.d, n_up_cols), o2 = weight_order(a.W2, a.s2e, a.s2k, a.s2n, a.F, a.d_out);
+  const Order o1 = weight_order(a.W1, a.E, a.s1e, a.s1k, a.s1n, a.d, n_up_cols), o2 = weight_order(a.W2, a.E, a.s2e, a.s2k, a.s2n, a.F, a.d_out);
   if (!(o1.k_major || o1.n_major) || !(o2.k_major || o2.n_major)) return SMOE_ERR_UNSUPPORTED;
   const bool bf16 = a.dtype == SMOE_BF16;
   StreamParams p;
@@ -842,7 +843,7 @@ static int launch_typed(const Args& a, const DeviceInfo& di) {
 // result (T, F), contiguous.
 template <typename T>
 static int launch_linear_typed(const Args& a, const Extension& ext, const DeviceInfo& di) {
-  const Order o = weight_order(a.W1, 0, a.s1k, a.s1n, a.d, a.F);
+  const Order o = weight_order(a.W1, 1, 0, a.s1k, a.s1n, a.d, a.F);
   if (!o.k_major && !o.n_major) return SMOE_ERR_UNSUPPORTED;
   const bool bf16 = a.dtype == SMOE_BF16;
   StreamParams p;

@@ -96,3 +96,24 @@ def test_wide_outputs(dtype, order, d_out):
     got = run(p, SECOND)
     assert (got[3] == 0).all()
     check(got, *reference(p["x"], p["up"], p["down"], p["gates"], p["ids"], SECOND, SILU, p["up_b"], p["down_b"]))
+
+
+@pytest.mark.parametrize("order", ["out_in", "in_out"])
+def test_experts_that_share_a_matrix(order, monkeypatch):
+    """Broadcast views: one matrix for all experts (stride 0), one row of inputs for all tokens, one bias. The streaming kernels' tensor
+    maps take no stride of zero, so the layer runs on CUDA cores and says so when the tensor cores are asked for."""
+    from scattermoe_b200.kernels import ops
+    p = problem(7, 64, 72, 5, 2, torch.bfloat16, FIRST, order, bias=True)
+    q = dict(p, x=p["x"][:1].expand(7, 64), up_b=p["up_b"][:1].expand(5, -1), down_b=p["down_b"][:1].expand(5, -1))
+    verify(q, FIRST)
+    assert ops.last_path_was_tensor_core()
+    for names in (("up",), ("down",), ("up", "down")):
+        r = dict(q, **{n: q[n][:1].expand(5, -1, -1) for n in names})
+        verify(r, FIRST)
+        assert not ops.last_path_was_tensor_core()
+    one = {n: p[n][:1].expand(1, -1, -1) for n in ("up", "down")}      # a single expert has no stride to speak of
+    verify(dict(p, **one, up_b=None, down_b=None, ids=torch.zeros_like(p["ids"])), FIRST)
+    assert ops.last_path_was_tensor_core()
+    monkeypatch.setattr(ops, "FORCE_PATH", "tc")
+    with pytest.raises(RuntimeError, match="no tensor-core kernel"):
+        run(dict(q, up=q["up"][:1].expand(5, -1, -1)), FIRST)
